@@ -1,0 +1,241 @@
+// What the attention kernels share: element types, matrix fragments, the staging of a tile of rows through LDS,
+// and the work items that faith_attention_plan lays down on the host.
+//
+// Every product here has the query rows (forward, gradient of the queries) or the keys (gradients of keys and
+// values) along the 32 columns of v_mfma_f32_32x32x{16,2}: lane l holds column l % 32, and of a result's 32 rows
+// those with ((row >> 2) & 1) == l / 32, row = (r & 3) + 8 (r >> 2) + 4 (l / 32) for its register r = 0 ... 15.
+// A result is thereby the second operand of the next product as it stands: the reduction over rows may run in any
+// order as long as the first operand is read in the same one, so probabilities never pass through LDS.
+#pragma once
+#include "common.h"
+
+namespace faith {
+namespace attn {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef short shortx8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+
+template <class T> struct Vec;
+template <> struct Vec<__bf16> { typedef bf16x8 x8; typedef bf16x4 x4; };
+template <> struct Vec<_Float16> { typedef halfx8 x8; typedef halfx4 x4; };
+
+__device__ __forceinline__ floatx16 mfma(bf16x8 a, bf16x8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mfma(halfx8 a, halfx8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mfma(float a, float b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+
+// the row that register r of a lane in half `half` of the wavefront holds of a 32 x 32 result
+__device__ __forceinline__ constexpr int row_of(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
+
+// One unit of work of one key head; eight ints, read as one scalar load.
+struct Item {
+    int q_start, q_len;          // the sequence's queries: first packed token and how many
+    int k_start, k_len;          // its keys
+    int row0;                    // first row (token * group + head of the group) or first key of the tile
+    int begin, end;              // keys (or tokens) that the tile goes over; end <= begin: none
+    int slot;                    // where its partial result goes; -1: it is the whole result
+};
+static_assert(sizeof(Item) == 32, "the host writes eight ints");
+
+// Workgroup -> (key head, item).  Workgroups are dealt to the eight XCDs round robin; a key head's items all run on one
+// XCD (or, with fewer than eight key heads, on 8 / gcd of them), whose L2 then holds that head's keys and values.
+struct Deal {
+    int heads_apart, stripes, items_per_stripe, n_items;
+};
+inline Deal deal(int n_items, int kv_heads, unsigned *grid) {
+    int e = 1;
+    while (e < 8 && kv_heads % (2 * e) == 0) e *= 2;
+    Deal d;
+    d.heads_apart = e;
+    d.stripes = 8 / e;
+    d.items_per_stripe = (n_items + d.stripes - 1) / d.stripes;
+    d.n_items = n_items;
+    *grid = 8u * (unsigned)(kv_heads / e) * (unsigned)d.items_per_stripe;
+    return d;
+}
+__device__ __forceinline__ bool dealt(const Deal &d, int *head, int *item) {
+    const int x = (int)(blockIdx.x & 7), l = (int)(blockIdx.x >> 3);
+    *head = x % d.heads_apart + d.heads_apart * (l / d.items_per_stripe);
+    *item = x / d.heads_apart + d.stripes * (l % d.items_per_stripe);
+    return *item < d.n_items;
+}
+
+// ------------------------------------------------------------------------------------------ a tile of rows in LDS
+// ROWS x DP elements, rows of RB bytes in chunks of 16 bytes; chunk c of row r stands at chunk c ^ swizzle(r).  Two reads
+// have to be free of bank conflicts (64 banks of 4 bytes): the same chunk of consecutive rows (16 bytes a lane), and 64
+// bytes of each of eight consecutive rows (the transposing read, 8 bytes a lane).
+template <class T, int DP> struct Tile {
+    static constexpr int RB = DP * (int)sizeof(T), CHUNKS = RB / 16, PER = 16 / (int)sizeof(T);
+    __device__ static __forceinline__ int swizzle(int r) {
+        if constexpr (CHUNKS == 4) return (r >> 2) & 3;
+        else if constexpr (CHUNKS == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        else return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+    // element offset of chunk c of row r
+    __device__ static __forceinline__ int at(int r, int c) { return r * DP + (c ^ swizzle(r)) * PER; }
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void *base, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, 0x00020000);
+}
+
+// The loads of one tile of ROWS rows by WAVES wavefronts: 1 KB an instruction, straight into LDS (lane i's 16 bytes land at
+// 16 i), so the swizzle is applied to the address that a lane reads.  Rows behind the sequence's last and chunks behind the
+// head's size lie outside the window and arrive as zeros.
+template <class T, int DP, int ROWS, int WAVES> struct Stager {
+    typedef Tile<T, DP> Tl;
+    static constexpr int ROWS_PER = 1024 / Tl::RB, LOADS = ROWS * Tl::RB / 1024 / WAVES;
+    static constexpr int PERIOD = ROWS_PER < 16 ? 16 / ROWS_PER : 1, PATTERNS = LOADS < PERIOD ? LOADS : PERIOD;   // the swizzle repeats every 16 rows
+    static_assert(LOADS * WAVES * 1024 == ROWS * Tl::RB && LOADS % PATTERNS == 0, "the wavefronts share the tile evenly");
+    unsigned off[PATTERNS];
+    unsigned stride;             // bytes from one row to the next
+
+    __device__ __forceinline__ void init(int lane, int wave, int size, long long row_stride) {
+        stride = (unsigned)(row_stride * (long long)sizeof(T));
+#pragma unroll
+        for (int i = 0; i < PATTERNS; ++i) {
+            const int r = (wave * LOADS + i) * ROWS_PER + lane / Tl::CHUNKS;
+            const int c = (lane % Tl::CHUNKS) ^ Tl::swizzle(r);
+            off[i] = c * Tl::PER < size ? (unsigned)r * stride + (unsigned)c * 16u : 0x7ffffff0u;
+        }
+    }
+    // base: the tile's first row; rows_left: rows from there to the sequence's end (may be <= 0)
+    __device__ __forceinline__ void load(T *lds, const T *base, int rows_left, int size, int wave) const {
+        // a window up to the last element of the last row; never so long that the offsets outside could fall into it
+        const long long n = rows_left > 0 ? (long long)((rows_left < ROWS ? rows_left : ROWS) - 1) * stride + (long long)size * (int)sizeof(T) : 0;
+        const __amdgpu_buffer_rsrc_t w = window(base, (unsigned)n);
+        char *dst = reinterpret_cast<char *>(lds) + wave * LOADS * 1024;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (lds_void *)(dst + i * 1024), 16, off[i % PATTERNS],
+                                                     (unsigned)((i / PATTERNS) * PATTERNS * ROWS_PER) * stride, 0, 0);
+    }
+};
+
+// first operand, 32 rows of a tile, 16 (T of 2 bytes) or 8 (float) of the reduction from chunk 2 u on
+template <class T, int DP> __device__ __forceinline__ typename Vec<T>::x8 row_fragment(const T *tile, int row, int u, int half) {
+    return *reinterpret_cast<const typename Vec<T>::x8 *>(tile + Tile<T, DP>::at(row, 2 * u + half));
+}
+template <int DP> __device__ __forceinline__ floatx4 row_fragment4(const float *tile, int row, int u, int half) {
+    return *reinterpret_cast<const floatx4 *>(tile + Tile<float, DP>::at(row, 2 * u + half));
+}
+// first operand transposed: columns col0 ... col0 + 31 of the tile against the 16 rows row0 + {0 ... 15} in the order in which
+// registers 0 ... 7 hold them: lane half h has rows 4h ... 4h + 3, then 8 + 4h ... 8 + 4h + 3
+template <class T, int DP> __device__ __forceinline__ typename Vec<T>::x8 column_fragment(const T *tile, int row0, int col0, int lane) {
+    const int i = lane & 15, r = row0 + 4 * (lane >> 5) + (i >> 2), c = col0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+    const T *lo = tile + Tile<T, DP>::at(r, c >> 3) + (c & 7);
+    const T *hi = tile + Tile<T, DP>::at(r + 8, c >> 3) + (c & 7);
+    const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4 *)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4 *)hi);
+    const shortx8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename Vec<T>::x8, v);
+}
+
+// acc[r] += sum_d tile[row_of(r)][d] * b[d]: the 32 rows from row0 on against this lane's column, whose values are in `b`
+template <class T, int DP> struct ColumnRegs { typename Vec<T>::x8 v[DP / 16]; };
+template <int DP> struct ColumnRegs<float, DP> { floatx4 v[DP / 8]; };
+
+template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(const T *tile, int row, int half, const ColumnRegs<T, DP> &b) {
+    floatx16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int u = 0; u < DP / 8; ++u) {
+            const floatx4 a = row_fragment4<DP>(tile, row, u, half);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = mfma(a[e], b.v[u][e], acc);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < DP / 16; ++u) acc = mfma(row_fragment<T, DP>(tile, row, u, half), b.v[u], acc);
+    }
+    return acc;
+}
+
+// the values of one row (DP of them, zero behind `size`) in the order in which rows_by_column takes them
+template <class T, int DP> __device__ __forceinline__ ColumnRegs<T, DP> column_regs(const T *row, int half, int size) {
+    ColumnRegs<T, DP> b;
+    constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int u = 0; u < DP / (2 * PER); ++u) {
+        const int d = (2 * u + half) * PER;
+        uintx4 z = {0u, 0u, 0u, 0u};
+        if (d < size) z = *reinterpret_cast<const uintx4 *>(row + d);
+        if constexpr (sizeof(T) == 4) b.v[u] = __builtin_bit_cast(floatx4, z);
+        else b.v[u] = __builtin_bit_cast(typename Vec<T>::x8, z);
+    }
+    return b;
+}
+
+// acc[m][r] += sum over the tile's 32 rows from row0 on of tile[row][32 m + row_of(r)] * p[row]: p is a result register set of
+// this lane's column.  Products of 2-byte elements round p to that type (half a step of it, against sums in 32 bits).
+template <class T, int DP> __device__ __forceinline__ void columns_by_result(floatx16 (&acc)[DP / 32], const T *tile, int row0, int lane, const floatx16 &p) {
+    if constexpr (sizeof(T) == 4) {
+        const int half = lane >> 5, col = lane & 31;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = row0 + row_of(r, half);
+#pragma unroll
+            for (int m = 0; m < DP / 32; ++m) {
+                const int c = 32 * m + col;
+                acc[m] = mfma(tile[Tile<T, DP>::at(row, c >> 2) + (c & 3)], p[r], acc[m]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            typename Vec<T>::x8 b;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b[e] = (T)p[8 * u + e];
+#pragma unroll
+            for (int m = 0; m < DP / 32; ++m) acc[m] = mfma(column_fragment<T, DP>(tile, row0 + 16 * u, 32 * m, lane), b, acc[m]);
+        }
+    }
+}
+
+// over the two lanes that share a column
+__device__ __forceinline__ float max_halves(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const unsigned a = s[0], b = s[1];
+    return __builtin_fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const unsigned a = s[0], b = s[1];
+    return __uint_as_float(a) + __uint_as_float(b);
+}
+
+// This wavefront's loads into LDS have landed and its reads are done; then the barrier.  (The compiler does not see
+// other wavefronts' loads.)
+__device__ __forceinline__ void landed_and_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Host checks that the three entry points share.
+inline int attention_shapes(const char *fn, int heads, int kv_heads, int size, int dtype, float scale) {
+    FAITH_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, FAITH_ERR_SHAPE, "%s: %d heads do not share %d key heads evenly", fn, heads, kv_heads);
+    FAITH_REQUIRE(dtype == FAITH_F32 || dtype == FAITH_BF16 || dtype == FAITH_F16, FAITH_ERR_UNSUPPORTED, "%s: element type %d", fn, dtype);
+    FAITH_REQUIRE(size > 0 && size <= 128 && size % (dtype == FAITH_F32 ? 4 : 8) == 0, FAITH_ERR_UNSUPPORTED,
+                  "%s: heads of %d elements (up to 128, whole groups of 16 bytes)", fn, size);
+    FAITH_REQUIRE(scale > 0.f && scale < 1e30f, FAITH_ERR_UNSUPPORTED, "%s: the scale must be positive and finite", fn);
+    return FAITH_OK;
+}
+// rows in whole 16-byte groups that neither overlap nor lie further apart than a 32-bit offset reaches over one tile
+inline bool attention_rows(const char *fn, const char *name, const void *p, long long token_stride, long long head_stride, int size, int es) {
+    const int per = 16 / es;
+    if (p && aligned(p, 16) && token_stride % per == 0 && head_stride % per == 0 && token_stride >= size && head_stride >= 0 &&
+        token_stride * es < (1LL << 24))
+        return true;
+    if (!p) set_error("%s: argument '%s' is NULL", fn, name);
+    else set_error("%s: %s must start on 16 bytes and have strides of whole 16-byte groups, the tokens' at least %d and under 2^24 bytes", fn, name, size);
+    return false;
+}
+
+}  // namespace attn
+}  // namespace faith

@@ -1,0 +1,478 @@
+// Attention of a network's concrete pass: out = softmax(scale q k^T) v over packed sequences of different lengths, with
+// groups of query heads that share a key head, causal or not; one query against a long cache is the same call.
+//
+// One pass over the keys with the running maximum and sum of the softmax.  A row is one (token, head of the group) pair,
+// row = token * group + head: all rows of a tile share the keys and values that it stages, so a group reads them once.
+// Two shapes of workgroup, four wavefronts each, 32 rows to a wavefront:
+//   rows    128 rows; every wavefront goes over every key tile (64 keys, 32 in fp32), staged once for the four
+//   keys    at most 32 rows (a single token's group, a short sentence); the wavefronts take turns at the key tiles of 32
+//           keys, each staged by its wavefront alone with no barrier, and join their results through LDS at the end
+// Few rows against many keys leave most of the device idle: the keys are then cut into several items, whose partial
+// results (maximum, sum, unnormalised output, all in fp32) a second small launch joins in a fixed order.
+#include "attention.h"
+
+#include <algorithm>
+#include <vector>
+
+namespace {
+
+using namespace faith;
+using namespace faith::attn;
+
+constexpr int KIND_ROWS = 0, KIND_KEYS = 1;
+constexpr float LOWEST = -3.0e38f;           // stands for "no key yet": finite, so that differences stay numbers
+constexpr float LAZY = 8.f;                  // powers of two by which a row's largest score may pass its reference
+
+struct FwdArgs {
+    const void *q, *k, *v;
+    void *out;
+    float *lse, *part;
+    const Item *items;
+    Deal deal;
+    long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, lse_hs;       // strides in elements
+    int group, kv_heads, size, causal;
+    float c;                                 // scale * log2(e)
+};
+
+// The softmax of one row over keys that this lane goes over by itself, in fp32 throughout: the way taken for the rows of a
+// wavefront whose result came out not finite.  The products above multiply masked values by zero, which a NaN or an
+// infinity in a place that the mask hides survives; this loop never touches what is masked.
+template <class T, int DP>
+__device__ void one_row(const FwdArgs &g, const Item &it, int hk, const T *qrow, int last, int half, float *ref, float *sum, floatx16 (&o)[DP / 32]) {
+    const T *k = reinterpret_cast<const T *>(g.k) + (long long)hk * g.k_hs, *v = reinterpret_cast<const T *>(g.v) + (long long)hk * g.v_hs;
+    const int end = it.end < last + 1 ? it.end : last + 1;
+    float top = LOWEST, l = 0.f;
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[m][r] = 0.f;
+    for (int pass = 0; pass < 2; ++pass)
+        for (int j = it.begin; j < end; ++j) {
+            const T *kr = k + (long long)(it.k_start + j) * g.k_ts;
+            float s = 0.f;
+            for (int d = 0; d < g.size; ++d) s = fmaf((float)qrow[d], (float)kr[d], s);
+            s *= g.c;
+            if (pass == 0) { top = s > top ? s : top; continue; }
+            const float p = __builtin_amdgcn_exp2f(s - top);
+            l += p;
+            const T *vr = v + (long long)(it.k_start + j) * g.v_ts;
+#pragma unroll
+            for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = 32 * m + row_of(r, half);
+                    if (d < g.size) o[m][r] = fmaf(p, (float)vr[d], o[m][r]);
+                }
+        }
+    *ref = top;
+    *sum = l;
+}
+
+// wavefronts of a workgroup that splits the keys: four, unless their four pairs of stages would not fit LDS (fp32, heads of 128)
+template <class T, int DP> constexpr int key_waves() { return 32 * DP * (int)sizeof(T) * 16 <= 128 * 1024 ? 4 : 2; }
+
+template <class T, int DP, int BN, bool KEYS, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, KEYS && DP * sizeof(T) >= 256 ? 1 : 2) attention_forward(const FwdArgs g) {
+    constexpr int TILE = BN * DP;
+    typedef Stager<T, DP, BN, KEYS ? 1 : 4> St;
+    // two stages in arrays of their own, so that the compiler sees that loads into one do not touch the other
+    __shared__ T k0[TILE * (KEYS ? WAVES : 1)], v0[TILE * (KEYS ? WAVES : 1)], k1[TILE * (KEYS ? WAVES : 1)], v1[TILE * (KEYS ? WAVES : 1)];
+
+    int hk, n;
+    if (!dealt(g.deal, &hk, &n)) return;
+    const Item it = g.items[n];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int half = lane >> 5, col = lane & 31;
+
+    // this lane's row
+    const int row = it.row0 + (KEYS ? 0 : wave * 32) + col, rows = it.q_len * g.group;
+    const int at = row < rows ? row : rows - 1;                    // a row behind the last repeats it and is not stored
+    const int token = at / g.group, head = hk * g.group + (at - token * g.group);
+    const T *qrow = reinterpret_cast<const T *>(g.q) + (long long)(it.q_start + token) * g.q_ts + (long long)head * g.q_hs;
+    const ColumnRegs<T, DP> q = column_regs<T, DP>(qrow, half, g.size);
+    // the last key that it may look at (the last query stands at the last key)
+    int last = it.k_len - 1;
+    if (g.causal) last = last < token + it.k_len - it.q_len ? last : token + it.k_len - it.q_len;
+    // first and last of the wavefront's rows: tiles that some row sees in part, tiles that no row sees
+    const int row_lo = it.row0 + (KEYS ? 0 : wave * 32), row_hi = row_lo + 31 < rows ? row_lo + 31 : rows - 1;
+    int all_see = it.k_len - 1, any_sees = it.k_len - 1;
+    if (g.causal) {
+        const int shift = it.k_len - it.q_len, a = row_lo / g.group + shift, b = row_hi / g.group + shift;
+        all_see = all_see < a ? all_see : a;
+        any_sees = any_sees < b ? any_sees : b;
+    }
+    if (row_lo >= rows) any_sees = -1;
+
+    floatx16 o[DP / 32];
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[m][r] = 0.f;
+    float ref = LOWEST, sum = 0.f;           // the row's reference (powers of two) and this lane's part of its sum
+
+    St ks, vs;
+    ks.init(lane, KEYS ? 0 : wave, g.size, g.k_ts);
+    vs.init(lane, KEYS ? 0 : wave, g.size, g.v_ts);
+    const T *kb = reinterpret_cast<const T *>(g.k) + (long long)it.k_start * g.k_ts + (long long)hk * g.k_hs;
+    const T *vb = reinterpret_cast<const T *>(g.v) + (long long)it.k_start * g.v_ts + (long long)hk * g.v_hs;
+    const int own = KEYS ? wave * TILE : 0;
+
+    auto stage = [&](T *kt, T *vt, int key0) {
+        ks.load(kt + own, kb + (long long)key0 * g.k_ts, it.k_len - key0, g.size, KEYS ? 0 : wave);
+        vs.load(vt + own, vb + (long long)key0 * g.v_ts, it.k_len - key0, g.size, KEYS ? 0 : wave);
+    };
+    auto tile = [&](const T *kt, const T *vt, int key0) {
+        if (key0 > any_sees) return;
+        floatx16 s[BN / 32];
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b) s[b] = rows_by_column<T, DP>(kt + own, 32 * b + col, half, q);
+        if (key0 + BN - 1 > all_see) {
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key0 + 32 * b + row_of(r, half) > last) s[b][r] = -__builtin_inff();
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[b][r]);
+        // The reference follows the maximum only when it has fallen LAZY powers of two behind: sums and outputs are then at
+        // most 2^LAZY times what they would be, which costs no precision, and most tiles rescale nothing.
+        if (__any(top * g.c > ref + LAZY)) {
+            const float now = __builtin_fmaxf(ref, max_halves(top) * g.c), f = __builtin_amdgcn_exp2f(ref - now);
+            ref = now;
+            sum *= f;
+#pragma unroll
+            for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[m][r] *= f;
+        }
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], g.c, -ref));
+                sum += s[b][r];
+            }
+            columns_by_result<T, DP>(o, vt + own, 32 * b, lane, s[b]);
+        }
+    };
+
+    if constexpr (!KEYS) {
+        if (it.begin < it.end) {
+            stage(k0, v0, it.begin);
+            for (int key0 = it.begin; key0 < it.end; key0 += 2 * BN) {
+                landed_and_barrier();
+                if (key0 + BN < it.end) stage(k1, v1, key0 + BN);
+                tile(k0, v0, key0);
+                if (key0 + BN >= it.end) break;
+                landed_and_barrier();
+                if (key0 + 2 * BN < it.end) stage(k0, v0, key0 + 2 * BN);
+                tile(k1, v1, key0 + BN);
+            }
+        }
+    } else {
+        const int first = it.begin + wave * BN;
+        if (first < it.end) {
+            // this wavefront's own tiles, no barrier: the younger stage's loads stay in flight while the older is used
+            constexpr int INFLIGHT = 2 * St::LOADS;
+            auto wait_for_older = [&](bool younger) {
+                if (younger) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(INFLIGHT) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            };
+            stage(k0, v0, first);
+            for (int key0 = first; key0 < it.end; key0 += 2 * WAVES * BN) {
+                const bool b = key0 + WAVES * BN < it.end;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (b) stage(k1, v1, key0 + WAVES * BN);
+                wait_for_older(b);
+                tile(k0, v0, key0);
+                if (!b) break;
+                const bool a = key0 + 2 * WAVES * BN < it.end;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (a) stage(k0, v0, key0 + 2 * WAVES * BN);
+                wait_for_older(a);
+                tile(k1, v1, key0 + WAVES * BN);
+            }
+        }
+        // the wavefronts' results meet in LDS: each leaves (reference, sum) and its output, the first joins them
+        __syncthreads();
+        constexpr int WIDTH = DP / 32 * 16;
+        static_assert((WAVES - 1) * 64 * WIDTH * 4 <= 2 * TILE * WAVES * (int)sizeof(T), "the results fit the two stages of keys");
+        float *lo = reinterpret_cast<float *>(k0), *hi = reinterpret_cast<float *>(k1), *ml = reinterpret_cast<float *>(v0);
+        auto cell = [&](int w, int e) -> float & {                 // result w, register e of this lane
+            const int x = (w * WIDTH + e) * 64 + lane;
+            constexpr int HALF = TILE * WAVES * (int)sizeof(T) / 4;
+            return x < HALF ? lo[x] : hi[x - HALF];
+        };
+        if (wave > 0) {
+            ml[(wave - 1) * 128 + lane] = ref;
+            ml[(wave - 1) * 128 + 64 + lane] = sum;
+#pragma unroll
+            for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) cell(wave - 1, 16 * m + r) = o[m][r];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+        float now = ref;
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; ++w) now = __builtin_fmaxf(now, ml[w * 128 + lane]);
+        const float f0 = __builtin_amdgcn_exp2f(ref - now);
+        sum *= f0;
+#pragma unroll
+        for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[m][r] *= f0;
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; ++w) {
+            const float f = __builtin_amdgcn_exp2f(ml[w * 128 + lane] - now);
+            sum = fmaf(ml[w * 128 + 64 + lane], f, sum);
+#pragma unroll
+            for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[m][r] = fmaf(cell(w, 16 * m + r), f, o[m][r]);
+        }
+        ref = now;
+    }
+
+    sum = sum_halves(sum);
+    if (g.causal) {
+        float bad = sum;
+#pragma unroll
+        for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bad = fmaf(0.f, o[m][r], bad);      // finite values leave it finite
+        if (__any(!(__builtin_fabsf(bad) < __builtin_inff()))) one_row<T, DP>(g, it, hk, qrow, last, half, &ref, &sum, o);
+    }
+    if (row >= rows) return;
+    if (it.slot >= 0) {
+        // a part: (reference, sum) and the unnormalised output, DP + 2 floats a row
+        constexpr int ROWS = KEYS ? 32 : 128;
+        float *p = g.part + ((long long)(it.slot * g.kv_heads + hk) * ROWS + (row - it.row0)) * (DP + 4);
+        if (half == 0) { p[0] = ref; p[1] = sum; }
+#pragma unroll
+        for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const floatx4 x = {o[m][r], o[m][r + 1], o[m][r + 2], o[m][r + 3]};
+                *reinterpret_cast<floatx4 *>(p + 4 + 32 * m + row_of(r, half)) = x;
+            }
+        return;
+    }
+    const float inverse = sum > 0.f || sum != sum ? 1.f / sum : 0.f;   // no key: zeros
+    T *dst = reinterpret_cast<T *>(g.out) + (long long)(it.q_start + token) * g.o_ts + (long long)head * g.o_hs;
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * m + row_of(r, half);
+            if (d >= g.size) continue;
+            if constexpr (sizeof(T) == 4) {
+                const floatx4 x = {o[m][r] * inverse, o[m][r + 1] * inverse, o[m][r + 2] * inverse, o[m][r + 3] * inverse};
+                *reinterpret_cast<floatx4 *>(dst + d) = x;
+            } else {
+                const typename Vec<T>::x4 x = {(T)(o[m][r] * inverse), (T)(o[m][r + 1] * inverse), (T)(o[m][r + 2] * inverse), (T)(o[m][r + 3] * inverse)};
+                *reinterpret_cast<typename Vec<T>::x4 *>(dst + d) = x;
+            }
+        }
+    if (g.lse && half == 0)
+        g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+}
+
+// Joins the parts of the rows of one item: {first token, tokens, -, -, first row, parts, rows of the item, first slot}; a
+// wavefront to a row, its lanes along the head.
+template <class T, int DP, int ROWS>
+__global__ void __launch_bounds__(256) attention_join(const FwdArgs g, const Item *joins) {
+    const Item it = joins[blockIdx.x];
+    const int hk = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int rows = it.q_len * g.group;
+    for (int i = blockIdx.z * 4 + wave; i < ROWS; i += 4 * gridDim.z) {
+        const int row = it.row0 + i;
+        if (row >= rows) return;
+        const long long step = (long long)g.kv_heads * ROWS * (DP + 4);
+        const float *p = g.part + ((long long)(it.slot * g.kv_heads + hk) * ROWS + i) * (DP + 4);
+        float ref = LOWEST;
+        for (int s = 0; s < it.begin; ++s) ref = __builtin_fmaxf(ref, p[s * step]);
+        float sum = 0.f, o[DP / 32] = {};
+        for (int s = 0; s < it.begin; ++s) {
+            const float f = __builtin_amdgcn_exp2f(p[s * step] - ref);
+            sum = fmaf(p[s * step + 1], f, sum);
+#pragma unroll
+            for (int e = 0; e < (DP + 63) / 64; ++e)
+                if (64 * e + lane < DP) o[e] = fmaf(p[s * step + 4 + 64 * e + lane], f, o[e]);
+        }
+        const float inverse = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        const int token = row / g.group, head = hk * g.group + (row - token * g.group);
+        T *dst = reinterpret_cast<T *>(g.out) + (long long)(it.q_start + token) * g.o_ts + (long long)head * g.o_hs;
+#pragma unroll
+        for (int e = 0; e < (DP + 63) / 64; ++e)
+            if (64 * e + lane < g.size) dst[64 * e + lane] = (T)(o[e] * inverse);
+        if (g.lse && lane == 0)
+            g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+    }
+}
+
+template <class T, int DP> int launch_forward(const FwdArgs &g, int kind, unsigned grid, const Item *joins, int n_joins, hipStream_t stream) {
+    constexpr int BN = sizeof(T) == 4 ? 32 : 64;
+    constexpr int WAVES = key_waves<T, DP>();
+    if (kind == KIND_KEYS) hipLaunchKernelGGL((attention_forward<T, DP, 32, true, WAVES>), dim3(grid), dim3(64 * WAVES), 0, stream, g);
+    else hipLaunchKernelGGL((attention_forward<T, DP, BN, false, 4>), dim3(grid), dim3(256), 0, stream, g);
+    if (n_joins > 0) {
+        if (kind == KIND_KEYS) hipLaunchKernelGGL((attention_join<T, DP, 32>), dim3(n_joins, g.kv_heads, 1), dim3(256), 0, stream, g, joins);
+        else hipLaunchKernelGGL((attention_join<T, DP, 128>), dim3(n_joins, g.kv_heads, 8), dim3(256), 0, stream, g, joins);
+    }
+    return check_launch("faith_attention");
+}
+template <class T> int launch_forward(const FwdArgs &g, int kind, unsigned grid, const Item *joins, int n_joins, hipStream_t stream) {
+    if (g.size <= 32) return launch_forward<T, 32>(g, kind, grid, joins, n_joins, stream);
+    if (g.size <= 64) return launch_forward<T, 64>(g, kind, grid, joins, n_joins, stream);
+    return launch_forward<T, 128>(g, kind, grid, joins, n_joins, stream);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------------ host
+namespace {
+
+struct Plan {
+    std::vector<Item> items, joins;
+    int kind = KIND_ROWS, slots = 0;
+};
+
+int tile_of(int pass, int kind, int element_size) {
+    if (pass == FAITH_ATTENTION_FORWARD) return kind == KIND_KEYS || element_size == 4 ? 32 : 64;
+    return 32;
+}
+
+// Items of one pass, longest first.  The forward pass cuts an item's keys where there are fewer items than the device holds
+// workgroups: into parts of equal length, as many as make up that number, none under 256 keys.
+Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int element_size, int causal, int pass) {
+    Plan p;
+    long long qs = 0, ks = 0;
+    int most = 0;
+    for (int b = 0; b < n; ++b) most = std::max(most, ql[b]);
+    if (pass == FAITH_ATTENTION_FORWARD && (long long)most * group <= 32) p.kind = KIND_KEYS;
+    const int rows_per = p.kind == KIND_KEYS ? 32 : 128, bn = tile_of(pass, p.kind, element_size);
+    for (int b = 0; b < n; ++b) {
+        const int shift = kl[b] - ql[b];
+        if (pass == FAITH_ATTENTION_GRAD_KEYS) {
+            for (int key0 = 0; key0 < kl[b]; key0 += 128) {
+                // the first token that sees a key of the tile
+                const int begin = causal ? std::min(ql[b], std::max(0, key0 - shift)) : 0;
+                p.items.push_back({(int)qs, ql[b], (int)ks, kl[b], key0, begin / 32 * 32, ql[b], -1});
+            }
+        } else {
+            const long long rows = (long long)ql[b] * group;
+            for (long long row0 = 0; row0 < rows; row0 += rows_per) {
+                const int token = (int)((std::min(rows, row0 + rows_per) - 1) / group);
+                const int end = causal ? std::max(0, std::min(kl[b], token + shift + 1)) : kl[b];
+                p.items.push_back({(int)qs, ql[b], (int)ks, kl[b], (int)row0, 0, end, -1});
+            }
+        }
+        qs += ql[b];
+        ks += kl[b];
+    }
+    const long long resident = 2LL * compute_units(), blocks = (long long)p.items.size() * kv_heads;
+    if (pass == FAITH_ATTENTION_FORWARD && blocks > 0 && blocks < (p.kind == KIND_KEYS ? 4 : 1) * resident) {
+        long long keys = 0;
+        for (const Item &it : p.items) keys += it.end;
+        const long long parts = (p.kind == KIND_KEYS ? 4 : 1) * resident;
+        long long chunk = (keys * kv_heads + parts - 1) / parts;
+        chunk = std::max<long long>((chunk + bn - 1) / bn * bn, 256);
+        std::vector<Item> cut;
+        for (const Item &it : p.items) {
+            const int n_parts = (int)((it.end + chunk - 1) / chunk);
+            if (n_parts <= 1) { cut.push_back(it); continue; }
+            Item j = it;
+            j.begin = n_parts;
+            j.end = 0;
+            j.slot = p.slots;
+            p.joins.push_back(j);
+            const int each = (int)(((it.end + n_parts - 1) / n_parts + bn - 1) / bn * bn);
+            for (int i = 0; i < n_parts; ++i) {
+                Item c = it;
+                c.begin = std::min(it.end, i * each);
+                c.end = std::min(it.end, (i + 1) * each);
+                c.slot = p.slots++;
+                cut.push_back(c);
+            }
+        }
+        p.items.swap(cut);
+    }
+    std::stable_sort(p.items.begin(), p.items.end(), [](const Item &a, const Item &b) { return a.end - a.begin > b.end - b.begin; });
+    return p;
+}
+
+}  // namespace
+
+extern "C" int faith_attention_plan(const int *query_lengths, const int *key_lengths, int sequences, int heads, int kv_heads,
+                                    int element_size, int causal, int pass, int *items, long long capacity, long long *counts) {
+    FAITH_NOT_NULL(query_lengths);
+    FAITH_NOT_NULL(key_lengths);
+    FAITH_NOT_NULL(counts);
+    FAITH_REQUIRE(sequences > 0, FAITH_ERR_SHAPE, "%s: %d sequences", __func__, sequences);
+    FAITH_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, FAITH_ERR_SHAPE, "%s: %d heads do not share %d key heads evenly", __func__, heads, kv_heads);
+    FAITH_REQUIRE(element_size == 2 || element_size == 4, FAITH_ERR_UNSUPPORTED, "%s: elements of %d bytes", __func__, element_size);
+    FAITH_REQUIRE(pass >= FAITH_ATTENTION_FORWARD && pass <= FAITH_ATTENTION_GRAD_KEYS, FAITH_ERR_UNSUPPORTED, "%s: pass %d", __func__, pass);
+    long long q = 0, k = 0;
+    for (int b = 0; b < sequences; ++b) {
+        FAITH_REQUIRE(query_lengths[b] >= 0 && key_lengths[b] >= 0, FAITH_ERR_SHAPE, "%s: sequence %d has a negative length", __func__, b);
+        q += query_lengths[b];
+        k += key_lengths[b];
+        FAITH_REQUIRE((long long)query_lengths[b] * (heads / kv_heads) < (1LL << 30) && key_lengths[b] < (1 << 30), FAITH_ERR_SHAPE,
+                      "%s: sequence %d is too long", __func__, b);
+    }
+    FAITH_REQUIRE(q < (1LL << 31) && k < (1LL << 31), FAITH_ERR_SHAPE, "%s: more than 2^31 tokens", __func__);
+    try {
+        const Plan p = make_plan(query_lengths, key_lengths, sequences, heads / kv_heads, kv_heads, element_size, causal, pass);
+        counts[0] = (long long)p.items.size();
+        counts[1] = (long long)p.joins.size();
+        counts[2] = p.slots;
+        counts[3] = p.kind;
+        if (items) {
+            FAITH_REQUIRE(capacity >= counts[0] + counts[1], FAITH_ERR_SHAPE, "%s: room for %lld items, %lld are needed", __func__, capacity, counts[0] + counts[1]);
+            std::copy(p.items.begin(), p.items.end(), reinterpret_cast<Item *>(items));
+            std::copy(p.joins.begin(), p.joins.end(), reinterpret_cast<Item *>(items) + p.items.size());
+        }
+    } catch (const std::exception &e) {
+        FAITH_REQUIRE(false, FAITH_ERR_UNSUPPORTED, "%s: %s", __func__, e.what());
+    }
+    return FAITH_OK;
+}
+
+extern "C" int faith_attention(const void *q, const void *k, const void *v, void *out, float *lse, float *parts, const int *items,
+                               int n_items, int n_joins, int kind, long long q_token_stride, long long q_head_stride,
+                               long long k_token_stride, long long k_head_stride, long long v_token_stride, long long v_head_stride,
+                               long long out_token_stride, long long out_head_stride, long long lse_head_stride, int heads, int kv_heads,
+                               int size, int dtype, int causal, float scale, void *stream) {
+    FAITH_REQUIRE(n_items >= 0 && n_joins >= 0, FAITH_ERR_SHAPE, "%s: %d items, %d joins", __func__, n_items, n_joins);
+    if (n_items == 0) return FAITH_OK;
+    FAITH_NOT_NULL(q);
+    FAITH_NOT_NULL(out);
+    FAITH_NOT_NULL(items);
+    FAITH_REQUIRE(n_joins == 0 || parts, FAITH_ERR_NULL, "%s: keys are cut into parts, and there is no room for their results", __func__);
+    FAITH_REQUIRE(kind == KIND_ROWS || kind == KIND_KEYS, FAITH_ERR_UNSUPPORTED, "%s: kind %d", __func__, kind);
+    const int rc = attention_shapes(__func__, heads, kv_heads, size, dtype, scale);
+    if (rc != FAITH_OK) return rc;
+    const int es = dtype == FAITH_F32 ? 4 : 2;
+    if (!attention_rows(__func__, "q", q, q_token_stride, q_head_stride, size, es) || !attention_rows(__func__, "k", k, k_token_stride, k_head_stride, size, es) ||
+        !attention_rows(__func__, "v", v, v_token_stride, v_head_stride, size, es) || !attention_rows(__func__, "out", out, out_token_stride, out_head_stride, size, es))
+        return FAITH_ERR_ALIGN;
+    FwdArgs g;
+    unsigned grid;
+    g.q = q; g.k = k; g.v = v; g.out = out; g.lse = lse; g.part = parts;
+    g.items = reinterpret_cast<const Item *>(items);
+    g.deal = deal(n_items, kv_heads, &grid);
+    g.q_ts = q_token_stride; g.q_hs = q_head_stride; g.k_ts = k_token_stride; g.k_hs = k_head_stride;
+    g.v_ts = v_token_stride; g.v_hs = v_head_stride; g.o_ts = out_token_stride; g.o_hs = out_head_stride; g.lse_hs = lse_head_stride;
+    g.group = heads / kv_heads; g.kv_heads = kv_heads; g.size = size; g.causal = causal;
+    g.c = scale * 1.4426950408889634f;
+    const Item *joins = g.items + n_items;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == FAITH_F32) return launch_forward<float>(g, kind, grid, joins, n_joins, s);
+    if (dtype == FAITH_BF16) return launch_forward<__bf16>(g, kind, grid, joins, n_joins, s);
+    return launch_forward<_Float16>(g, kind, grid, joins, n_joins, s);
+}

@@ -83,14 +83,14 @@ class Workspace:
     def reset(self):
         self.cursor = 0
 
-    def take(self, shape, device):
+    def take(self, shape, device, dtype=torch.float32):
         i = self.cursor
         self.cursor += 1
         if i < len(self.buffers):
             t = self.buffers[i]
-            if t.shape == shape and t.device == device:
+            if t.shape == shape and t.device == device and t.dtype == dtype:
                 return t
-        t = torch.empty(shape, device=device, dtype=torch.float32)
+        t = torch.empty(shape, device=device, dtype=dtype)
         self.allocations += 1
         if i < len(self.buffers):
             self.buffers[i] = t
@@ -99,7 +99,7 @@ class Workspace:
         return t
 
     def bytes(self):
-        return sum(t.numel() * 4 for t in self.buffers)
+        return sum(t.numel() * t.element_size() for t in self.buffers)
 
     def scope(self):
         """Context manager: the operator calls inside take their buffers from this workspace, from its start."""
@@ -129,15 +129,15 @@ class workspace:
         return False
 
 
-def _empty(*shape, device):
+def _empty(*shape, device, dtype=torch.float32):
     if _WORKSPACE is not None:
-        return _WORKSPACE.take(torch.Size(shape), device)
-    return torch.empty(shape, device=device, dtype=torch.float32)
+        return _WORKSPACE.take(torch.Size(shape), device, dtype)
+    return torch.empty(shape, device=device, dtype=dtype)
 
 
 def _empty_like(t):
     if _WORKSPACE is not None:
-        return _WORKSPACE.take(t.shape, t.device)
+        return _WORKSPACE.take(t.shape, t.device, t.dtype)
     return torch.empty_like(t)
 
 
@@ -1118,3 +1118,159 @@ def concretize_conv(lw, lb, uw, ub, p, eps):
     l, u = concretize(lw.view(1, 1, D, C * Hh * Ww), lb.view(1, 1, C * Hh * Ww),
                       uw.view(1, 1, D, C * Hh * Ww), ub.view(1, 1, C * Hh * Ww), p, eps, 1)
     return l.view(1, C, Hh, Ww), u.view(1, C, Hh, Ww)
+
+
+# ------------------------------------------------------------------------------------------
+# The concrete pass: what the network itself computes beside its dense layers.
+# ------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+class Packing:
+    """A batch of sequences of different lengths whose rows follow each other without padding.
+
+    lengths: how many rows (tokens) each sequence has, on the host (a list or a CPU tensor); key_lengths: the same for
+    keys and values where they differ from the queries' (one query against a long cache; default: equal).  Query i of a
+    sequence of n queries and m keys stands at key i + m - n, so the last query stands at the last key.
+
+    The lengths are checked and the attention kernels' work items laid down here, on the host; the first call with some
+    shape of heads uploads its items (a few kilobytes), later ones -- any stream, any contents -- reuse them.  A call that
+    is captured into a HIP graph has to have been made once before, and the packing must live as long as the graph."""
+
+    def __init__(self, lengths, key_lengths=None, device="cuda"):
+        self.lengths = self._checked("lengths", lengths)
+        self.key_lengths = self.lengths if key_lengths is None else self._checked("key_lengths", key_lengths)
+        if len(self.lengths) != len(self.key_lengths):
+            raise ValueError(f"{len(self.lengths)} sequences of queries, {len(self.key_lengths)} of keys")
+        self.tokens, self.keys = sum(self.lengths), sum(self.key_lengths)
+        if self.tokens >= 1 << 31 or self.keys >= 1 << 31:
+            raise ValueError("a packing holds fewer than 2^31 tokens")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"device: the work items live on the GPU (got {device}); there is no CPU path")
+        self.device = device
+        self._plans = {}
+
+    @staticmethod
+    def _checked(name, lengths):
+        out = []
+        for n in (lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths):
+            if isinstance(n, bool) or int(n) != n or not 0 <= n < 1 << 30:
+                raise ValueError(f"{name}: {n!r} is not a length")
+            out.append(int(n))
+        if not out:
+            raise ValueError(f"{name}: no sequences")
+        return tuple(out)
+
+    def starts(self):
+        """First packed row of every sequence, and the number of rows."""
+        at, out = 0, [0]
+        for n in self.lengths:
+            at += n
+            out.append(at)
+        return out
+
+    def plan(self, which, heads, kv_heads, element_size, causal):
+        """(items on the device, their address, how many, joins, parts, kind) of one pass; see faith_attention_plan."""
+        key = (which, heads // kv_heads, kv_heads, element_size, bool(causal))
+        found = self._plans.get(key)
+        if found is None:
+            found = self._plans[key] = self._make(which, heads, kv_heads, element_size, bool(causal))
+        stream = _stream(found[0])
+        if stream != found[6]:
+            # used on another stream than the one it was allocated on: its memory is not handed out again before this is done
+            found[0].record_stream(torch.cuda.current_stream(self.device))
+        return found
+
+    def _make(self, which, heads, kv_heads, element_size, causal):
+        import ctypes
+        n = len(self.lengths)
+        array = ctypes.c_int * n
+        ql, kl, counts = array(*self.lengths), array(*self.key_lengths), (ctypes.c_longlong * 4)()
+        args = (ctypes.addressof(ql), ctypes.addressof(kl), n, heads, kv_heads, element_size, int(causal), which)
+        with _on(self.device):
+            _lib.call("faith_attention_plan", *args, None, 0, ctypes.addressof(counts))
+            total = counts[0] + counts[1]
+            host = torch.empty((max(1, total), 8), dtype=torch.int32)
+            _lib.call("faith_attention_plan", *args, host.data_ptr(), total, ctypes.addressof(counts))
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call with this packing and these heads uploads its work items and cannot be captured: "
+                                   "make it once before the capture")
+            items = host.to(self.device)
+        return items, items.data_ptr(), counts[0], counts[1], counts[2], counts[3], _stream(items)
+
+
+def _rows(name, t, rows, heads, size, like=None):
+    """[rows or more, heads, size] of one of the concrete pass's types: strided as long as a head's elements are
+    contiguous and everything starts on 16 bytes."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must live on the GPU (got {t.device}); there is no CPU path")
+    if t.dtype not in _DTYPES or (like is not None and t.dtype != like.dtype):
+        raise TypeError(f"{name}: must be float32, bfloat16 or float16, alike for all operands, got {t.dtype}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name}: lives on {t.device}, the other operands on {like.device}")
+    if t.dim() != 3 or t.shape[0] < rows or (heads is not None and t.shape[1] != heads) or (size is not None and t.shape[2] != size):
+        raise ValueError(f"{name}: expected shape ({rows} or more, {heads or 'heads'}, {size or 'size'}), got {tuple(t.shape)}")
+    per = 16 // t.element_size()
+    ts, hs, es = t.stride()
+    if t.shape[0] == 1:
+        ts = t.shape[1] * t.shape[2]
+    if t.shape[1] == 1:
+        hs = t.shape[2]
+    if (es != 1 and t.shape[2] > 1) or ts % per or hs % per or t.data_ptr() % 16 or ts < t.shape[2] or hs < 0 or ts * t.element_size() >= 1 << 24:
+        raise ValueError(f"{name}: the elements of a head must be contiguous, rows must not overlap, and rows and heads must start on "
+                         f"16 bytes (strides {t.stride()})")
+    return ts, hs
+
+
+def _attention_operands(q, k, v, packing):
+    if not isinstance(packing, Packing):
+        raise TypeError(f"packing: expected a Packing, got {type(packing).__name__}")
+    qs = _rows("q", q, packing.tokens, None, None)
+    heads, size = q.shape[1], q.shape[2]
+    ks = _rows("k", k, packing.keys, None, size, q)
+    kv_heads = k.shape[1]
+    vs = _rows("v", v, packing.keys, kv_heads, size, q)
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"{heads} heads do not share {kv_heads} key heads evenly")
+    if size > 128 or size == 0 or size % (16 // q.element_size()):
+        raise ValueError(f"heads of {size} elements: up to 128 in whole groups of 16 bytes")
+    if q.device.index != (torch.cuda.current_device() if packing.device.index is None else packing.device.index):
+        raise ValueError(f"q lives on {q.device}, the packing on {packing.device}")
+    return heads, kv_heads, size, qs, ks, vs
+
+
+def _scale(scale, size):
+    if scale is None:
+        return 1.0 / math.sqrt(size)
+    scale = float(scale)
+    if not 0 < scale < 1e30:
+        raise ValueError(f"scale={scale}: must be positive and finite")
+    return scale
+
+
+def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=None):
+    """softmax(scale q k^T) v of every sequence of `packing`, for the network itself (not its bounds).
+
+    q [tokens, heads, size], k, v [keys, kv_heads, size], float32, bfloat16 or float16; heads that share a key head are
+    consecutive.  causal: a query sees the keys up to its own place.  scale: default 1 / sqrt(size).  Returns out like q
+    (and, with return_lse, the logarithm of every row's sum of exponentials, float32 [heads, tokens], which
+    attention_backward takes).  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, and
+    their places in `out` not written."""
+    heads, kv_heads, size, (qt, qh), (kt, kh), (vt, vh) = _attention_operands(q, k, v, packing)
+    scale = _scale(scale, size)
+    dev = q.device
+    if out is None:
+        out = _empty(q.shape[0], heads, size, device=dev, dtype=q.dtype)
+    ot, oh = _rows("out", out, packing.tokens, heads, size, q)
+    lse = _empty(heads, packing.tokens, device=dev) if return_lse else None
+    with _on(dev):
+        _, items, n, joins, parts, kind, _ = packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), causal)
+        scratch = None
+        if parts:
+            scratch = _empty(parts * kv_heads * (32 if kind else 128) * ((32 if size <= 32 else 64 if size <= 64 else 128) + 4), device=dev)
+        _lib.call("faith_attention", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(scratch), items, n, joins, kind,
+                  qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size, _DTYPES[q.dtype], int(causal), scale, _stream(q))
+    return (out, lse) if return_lse else out

@@ -638,6 +638,49 @@ int faith_convolution_verification(const float *x_lb, const float *x_ub,
                                    int K, int Stride, int padding_size, int dim_in,
                                    void *stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * The concrete pass: what the network itself computes beside its dense layers, and its gradient.  (No counterpart in
+ * the reference's kernels; its networks run as PyTorch modules, Transformer_Verification_Code/Models/.)  Arrays of
+ * these entry points hold `dtype` elements; sums, statistics and softmax values are held in 32 bits.
+ * --------------------------------------------------------------------------------------------------------------- */
+#define FAITH_F32   0
+#define FAITH_BF16  1
+#define FAITH_F16   2
+
+/*
+ * Work items of the attention entry points for a batch of packed sequences, laid down on the host (no GPU is touched):
+ * sequence b has query_lengths[b] queries and key_lengths[b] keys, >= 0 each; query i of a sequence of lengths (n, m)
+ * stands at key i + m - n, and with `causal` sees the keys up to there (none, if that is negative).
+ *   pass      FAITH_ATTENTION_FORWARD (faith_attention), _GRAD_QUERIES, _GRAD_KEYS (faith_attention_backward)
+ *   items     eight ints an item, or NULL: only the counts are wanted
+ *   capacity  items that fit
+ *   counts    [4]: items; joins (they follow the items in the array); parts of cut rows; kind
+ * The array, copied to the device, serves every call with these lengths, heads, element size and `causal`, from any
+ * stream, until the lengths change.  faith_attention needs parts * kv_heads * (kind ? 32 : 128) * (size rounded up to
+ * 32, 64 or 128, + 4) floats of scratch, which calls that may overlap must not share.
+ */
+#define FAITH_ATTENTION_FORWARD       0
+#define FAITH_ATTENTION_GRAD_QUERIES  1
+#define FAITH_ATTENTION_GRAD_KEYS     2
+int faith_attention_plan(const int *query_lengths, const int *key_lengths, int sequences, int heads, int kv_heads,
+                         int element_size, int causal, int pass, int *items, long long capacity, long long *counts);
+
+/*
+ * out = softmax(scale * q k^T) v over packed sequences; head h uses key head h / (heads / kv_heads).
+ *   q, out    [tokens, heads, size] by their strides (elements); k, v [keys, kv_heads, size] likewise.  16-byte aligned,
+ *             strides in whole 16-byte groups; size <= 128 in whole 16-byte groups.  Rows behind the last sequence are
+ *             neither read nor written.
+ *   lse       [heads, lse_head_stride] natural logarithm of each row's sum of exponentials, or NULL
+ *   parts     scratch (see faith_attention_plan), NULL if the plan has no joins
+ *   items ... kind: as the plan laid them down for FAITH_ATTENTION_FORWARD
+ * A row that sees no key is zero, its lse -inf.  What masked keys and values hold does not matter, NaN included.
+ */
+int faith_attention(const void *q, const void *k, const void *v, void *out, float *lse, float *parts, const int *items,
+                    int n_items, int n_joins, int kind, long long q_token_stride, long long q_head_stride,
+                    long long k_token_stride, long long k_head_stride, long long v_token_stride, long long v_head_stride,
+                    long long out_token_stride, long long out_head_stride, long long lse_head_stride, int heads, int kv_heads,
+                    int size, int dtype, int causal, float scale, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
