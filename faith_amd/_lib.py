@@ -16,6 +16,8 @@ ERR_NULL, ERR_SHAPE, ERR_UNSUPPORTED, ERR_ALIGN, ERR_LAUNCH = -1, -2, -3, -4, -5
 Q_1, Q_2, Q_INF = 1, 2, 0
 LAYOUT_NATURAL, LAYOUT_TRANSPOSED = 0, 1
 F32, BF16, F16 = 0, 1, 2
+NORM_KINDS = {"rms": 0, "standard": 1, "no_var": 2}
+BITS_INT8, BITS_E4M3 = 1, 2
 ATTENTION_FORWARD, ATTENTION_GRAD_QUERIES, ATTENTION_GRAD_KEYS = 0, 1, 2
 OP_RELU, OP_TANH, OP_EXP, OP_RECIPROCAL, OP_SQR, OP_SQRT = 1, 2, 3, 4, 5, 6
 
@@ -65,6 +67,9 @@ SIGNATURES = {
     "faith_attention_context_compact": [_P] * 17 + [_I] * 7 + [_F, _I, _I, _P],
     "faith_attention_context": [_P] * 16 + [_I] * 6 + [_F, _I, _I, _P],
     "faith_convolution_verification": [_P] * 10 + [_I] * 9 + [_P],
+    "faith_residual_norm": [_P] * 8 + [ctypes.c_longlong] + [_I] * 4 + [_F, _P],
+    "faith_residual_norm_blocks": [ctypes.c_longlong, _I, _I],          # answers a count: call it through `lib`
+    "faith_residual_norm_backward": [_P] * 9 + [ctypes.c_longlong] + [_I] * 3 + [_P],
     "faith_attention_plan": [_P, _P] + [_I] * 6 + [_P, ctypes.c_longlong, _P],
     "faith_attention": [_P] * 7 + [_I] * 3 + [ctypes.c_longlong] * 9 + [_I] * 5 + [_F, _P],
 }

@@ -1274,3 +1274,87 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
         _lib.call("faith_attention", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(scratch), items, n, joins, kind,
                   qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size, _DTYPES[q.dtype], int(causal), scale, _stream(q))
     return (out, lse) if return_lse else out
+
+
+def _row_tensor(name, t, like=None, shape=None, dtype=None):
+    """A contiguous GPU tensor of one of the concrete pass's types."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if not t.is_cuda or (like is not None and t.device != like.device):
+        raise ValueError(f"{name}: must live on the GPU, with the other operands (got {t.device}); there is no CPU path")
+    want = dtype or (like.dtype if like is not None else None)
+    if t.dtype not in _DTYPES or (want is not None and t.dtype != want):
+        raise TypeError(f"{name}: must be {want or 'float32, bfloat16 or float16'}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _norm_operands(x, others, vectors, kind):
+    _row_tensor("x", x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x: expected rows of at least one element, got {tuple(x.shape)}")
+    for name, t in others:
+        if t is not None:
+            _row_tensor(name, t, x, x.shape)
+    for name, t in vectors:
+        if t is not None:
+            _row_tensor(name, t, x, (x.shape[-1],))
+    if kind not in _lib.NORM_KINDS:
+        raise ValueError(f"unknown kind {kind!r}: one of {', '.join(_lib.NORM_KINDS)}")
+    return x.numel() // x.shape[-1], x.shape[-1], _lib.NORM_KINDS[kind]
+
+
+_BITS = {"int8": (_lib.BITS_INT8, torch.int8), "e4m3": (_lib.BITS_E4M3, torch.float8_e4m3fn)}
+
+
+def residual_norm(x, residual=None, weight=None, bias=None, kind="rms", eps=1e-6, quantize=None, return_stats=False):
+    """The residual connection and the normalisation behind it, for the network itself (Bounds.layer_norm is the same for
+    its bounds): h = x + residual and y = weight * z + bias, along the last axis, with
+        kind "rms"       z = h / sqrt(mean(h^2) + eps)
+        kind "standard"  z = (h - mean(h)) / sqrt(var(h) + eps)
+        kind "no_var"    z = h - mean(h)
+    float32, bfloat16 or float16, contiguous; weight and bias of x's type.  Returns (y, h); h is x itself without a residual.
+    quantize "int8" / "e4m3": returns (q, scales, h), 8-bit values with a float32 scale for every row, y ~ q * scale,
+    scale = max |y| / 127 or / 448.  return_stats: one more result, what residual_norm_backward takes as `stats`."""
+    rows, n, code = _norm_operands(x, (("residual", residual),), (("weight", weight), ("bias", bias)), kind)
+    eps = float(eps)
+    if not 0 <= eps < 1e30:
+        raise ValueError(f"eps={eps}: must be finite and not negative")
+    bits, scales = 0, None
+    if quantize is None:
+        y = _empty_like(x)
+    elif quantize in _BITS:
+        bits, dtype = _BITS[quantize]
+        y = _empty(*x.shape, device=x.device, dtype=dtype)
+        scales = _empty(*x.shape[:-1], device=x.device)
+    else:
+        raise ValueError(f"quantize={quantize!r}: one of {', '.join(_BITS)} or None")
+    h = x if residual is None else _empty_like(x)
+    stats = _empty(*x.shape[:-1], 2, device=x.device) if return_stats else None
+    with _on(x.device):
+        _lib.call("faith_residual_norm", _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y), None if residual is None else _ptr(h),
+                  _ptr(stats), _ptr(scales), rows, n, code, _DTYPES[x.dtype], bits, eps, _stream(x))
+    out = (y, h) if scales is None else (y, scales, h)
+    return out + (stats,) if return_stats else out
+
+
+def residual_norm_backward(dy, h, weight, stats, kind="rms", dsum=None, with_weight=True, with_bias=False):
+    """Gradients of residual_norm: dy of y, dsum of h (what reaches it past the normalisation, or None); h, stats as the
+    forward call returned them.  Returns (dx, dweight, dbias): dx is the gradient of x and of the residual alike, dweight and
+    dbias are None where they are not wanted.  The same bits on every call."""
+    rows, n, code = _norm_operands(h, (("dy", dy), ("dsum", dsum)), (("weight", weight),), kind)
+    _row_tensor("stats", stats, h, (*h.shape[:-1], 2), torch.float32)
+    dev = h.device
+    dx = _empty_like(h)
+    dweight = _empty(n, device=dev, dtype=h.dtype) if with_weight else None
+    dbias = _empty(n, device=dev, dtype=h.dtype) if with_bias else None
+    with _on(dev):
+        partial = None
+        if with_weight or with_bias:
+            partial = _empty(max(1, _lib.lib.faith_residual_norm_blocks(rows, n, _DTYPES[h.dtype])) * 2 * n, device=dev)
+        _lib.call("faith_residual_norm_backward", _ptr(dy), _ptr(dsum), _ptr(h), _ptr(weight), _ptr(stats), _ptr(dx), _ptr(dweight),
+                  _ptr(dbias), _ptr(partial), rows, n, code, _DTYPES[h.dtype], _stream(h))
+    return dx, dweight, dbias
