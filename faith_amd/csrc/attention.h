@@ -87,6 +87,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void *base, unsig
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, 0x00020000);
 }
 
+// 16 bytes a lane into LDS: lane i's land at dst + 16 i
+__device__ __forceinline__ void groups_to_lds(__amdgpu_buffer_rsrc_t w, char *dst, unsigned lane_off, unsigned uniform_off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (lds_void *)dst, 16, lane_off, uniform_off, 0, 0);
+}
+
 // The loads of one tile of ROWS rows by WAVES wavefronts: 1 KB an instruction, straight into LDS (lane i's 16 bytes land at
 // 16 i), so the swizzle is applied to the address that a lane reads.  Rows behind the sequence's last and chunks behind the
 // head's size lie outside the window and arrive as zeros.
@@ -115,10 +120,14 @@ template <class T, int DP, int ROWS, int WAVES> struct Stager {
         char *dst = reinterpret_cast<char *>(lds) + wave * LOADS * 1024;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (lds_void *)(dst + i * 1024), 16, off[i % PATTERNS],
-                                                     (unsigned)((i / PATTERNS) * PATTERNS * ROWS_PER) * stride, 0, 0);
+            groups_to_lds(w, dst + i * 1024, off[i % PATTERNS], (unsigned)((i / PATTERNS) * PATTERNS * ROWS_PER) * stride);
     }
 };
+
+// n <= 64 floats into LDS, one a lane; zeros behind them
+__device__ __forceinline__ void words_to_lds(float *lds, const float *src, int n, int lane) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(window(src, (unsigned)n * 4u), (lds_void *)lds, 4, (unsigned)lane * 4u, 0, 0, 0);
+}
 
 // first operand, 32 rows of a tile, 16 (T of 2 bytes) or 8 (float) of the reduction from chunk 2 u on
 template <class T, int DP> __device__ __forceinline__ typename Vec<T>::x8 row_fragment(const T *tile, int row, int u, int half) {

@@ -1,0 +1,328 @@
+// Gradients of the attention of a network's concrete pass (attention.hip), scores and probabilities computed again:
+//     p = exp(s - lse),  dp = do . v,  ds = p (dp - delta),  delta = do . out
+//     dq = scale sum_j ds k,   dk = scale sum_{i, heads of the group} ds q,   dv = sum_{i, heads of the group} p do
+// Two launches and no atomics, so that the same call gives the same bits: one goes over the keys for a tile of query rows (and
+// leaves delta and the logarithm of the row's sum, in powers of two, to the other), one over the queries of all heads of the
+// group for a tile of keys.  That computes s and dp twice -- seven products where five would do -- and needs neither an array
+// of sums in 32 bits that many workgroups add to nor a pass that rounds it.
+#include "attention.h"
+
+namespace {
+
+using namespace faith;
+using namespace faith::attn;
+
+struct GradArgs {
+    const void *dout, *q, *k, *v, *out;
+    const float *lse;
+    void *dq, *dk, *dv;
+    float *stat;                             // [2][heads][lse_hs]: lse in powers of two, delta
+    const Item *items;
+    Deal deal;
+    long long do_ts, do_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, dq_ts, dq_hs, dk_ts, dk_hs, dv_ts, dv_hs, lse_hs;
+    int group, kv_heads, size, causal;
+    float c, scale;                          // scale * log2(e); scale
+};
+
+template <class T> __device__ __forceinline__ const T *at(const void *base, long long row, long long ts, int head, long long hs) {
+    return reinterpret_cast<const T *>(base) + row * ts + (long long)head * hs;
+}
+
+template <class T> __device__ __forceinline__ float dot_rows(const T *a, const T *b, int n) {
+    float s = 0.f;
+    for (int d = 0; d < n; ++d) s = fmaf((float)a[d], (float)b[d], s);
+    return s;
+}
+
+// this lane's column of a result, `factor` times, to a row of T
+template <class T, int DP> __device__ __forceinline__ void store_column(T *dst, const floatx16 (&o)[DP / 32], float factor, int half, int size) {
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * m + row_of(r, half);
+            if (d >= size) continue;
+            if constexpr (sizeof(T) == 4) {
+                const floatx4 x = {o[m][r] * factor, o[m][r + 1] * factor, o[m][r + 2] * factor, o[m][r + 3] * factor};
+                *reinterpret_cast<floatx4 *>(dst + d) = x;
+            } else {
+                const typename Vec<T>::x4 x = {(T)(o[m][r] * factor), (T)(o[m][r + 1] * factor), (T)(o[m][r + 2] * factor), (T)(o[m][r + 3] * factor)};
+                *reinterpret_cast<typename Vec<T>::x4 *>(dst + d) = x;
+            }
+        }
+}
+template <int DP> __device__ __forceinline__ void clear(floatx16 (&o)[DP / 32]) {
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[m][r] = 0.f;
+}
+template <int DP> __device__ __forceinline__ bool any_not_finite(const floatx16 (&o)[DP / 32]) {
+    float bad = 0.f;
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad = fmaf(0.f, o[m][r], bad);
+    return __any(bad != 0.f);                // 0 * NaN, 0 * infinity
+}
+// o += f * row, for this lane's registers
+template <class T, int DP> __device__ __forceinline__ void add_row(floatx16 (&o)[DP / 32], const T *row, float f, int half, int size) {
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = 32 * m + row_of(r, half);
+            if (d < size) o[m][r] = fmaf(f, (float)row[d], o[m][r]);
+        }
+}
+
+template <class T, int DP, int BN>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) attention_grad_queries(const GradArgs g) {
+    constexpr int TILE = BN * DP;
+    typedef Stager<T, DP, BN, 4> St;
+    __shared__ T k0[TILE], v0[TILE], k1[TILE], v1[TILE];
+
+    int hk, n;
+    if (!dealt(g.deal, &hk, &n)) return;
+    const Item it = g.items[n];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int half = lane >> 5, col = lane & 31;
+    const int row_lo = it.row0 + wave * 32, row = row_lo + col, rows = it.q_len * g.group;
+    const int mine = row < rows ? row : rows - 1;
+    const int token = mine / g.group, head = hk * g.group + (mine - token * g.group);
+    const long long place = it.q_start + token;
+    const T *qrow = at<T>(g.q, place, g.q_ts, head, g.q_hs), *dorow = at<T>(g.dout, place, g.do_ts, head, g.do_hs);
+    const ColumnRegs<T, DP> q = column_regs<T, DP>(qrow, half, g.size), d_o = column_regs<T, DP>(dorow, half, g.size);
+    float delta = 0.f;
+    {
+        const ColumnRegs<T, DP> o = column_regs<T, DP>(at<T>(g.out, place, g.o_ts, head, g.o_hs), half, g.size);
+        constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int u = 0; u < DP / (2 * PER); ++u)
+#pragma unroll
+            for (int e = 0; e < PER; ++e) delta = fmaf((float)o.v[u][e], (float)d_o.v[u][e], delta);
+        delta = sum_halves(delta);
+    }
+    const float l = g.lse[(long long)head * g.lse_hs + place];
+    const float lse = l == -__builtin_inff() ? 0.f : l * 1.4426950408889634f;      // a row that sees no key: every p below is masked
+    if (row < rows && half == 0) {
+        float *s = g.stat + (long long)head * g.lse_hs + place;
+        s[0] = lse;
+        s[(long long)g.kv_heads * g.group * g.lse_hs] = delta;
+    }
+    int last = it.k_len - 1, all_see = it.k_len - 1, any_sees = it.k_len - 1;
+    if (g.causal) {
+        const int shift = it.k_len - it.q_len, row_hi = row_lo + 31 < rows ? row_lo + 31 : rows - 1;
+        const int a = row_lo / g.group + shift, b = row_hi / g.group + shift;
+        last = last < token + shift ? last : token + shift;
+        all_see = all_see < a ? all_see : a;
+        any_sees = any_sees < b ? any_sees : b;
+    }
+    if (row_lo >= rows) any_sees = -1;
+
+    floatx16 dq[DP / 32];
+    clear<DP>(dq);
+    St ks, vs;
+    ks.init(lane, wave, g.size, g.k_ts);
+    vs.init(lane, wave, g.size, g.v_ts);
+    const T *kb = at<T>(g.k, it.k_start, g.k_ts, hk, g.k_hs), *vb = at<T>(g.v, it.k_start, g.v_ts, hk, g.v_hs);
+    auto stage = [&](T *kt, T *vt, int key0) {
+        ks.load(kt, kb + (long long)key0 * g.k_ts, it.k_len - key0, g.size, wave);
+        vs.load(vt, vb + (long long)key0 * g.v_ts, it.k_len - key0, g.size, wave);
+    };
+    auto tile = [&](const T *kt, const T *vt, int key0) {
+        if (key0 > any_sees) return;
+        const bool part = key0 + BN - 1 > all_see;
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b) {
+            floatx16 s = rows_by_column<T, DP>(kt, 32 * b + col, half, q);
+            const floatx16 dp = rows_by_column<T, DP>(vt, 32 * b + col, half, d_o);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], g.c, -lse)) * (dp[r] - delta);
+            if (part) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key0 + 32 * b + row_of(r, half) > last) s[r] = 0.f;
+            }
+            columns_by_result<T, DP>(dq, kt, 32 * b, lane, s);
+        }
+    };
+    if (it.begin < it.end) {
+        stage(k0, v0, it.begin);
+        for (int key0 = it.begin; key0 < it.end; key0 += 2 * BN) {
+            landed_and_barrier();
+            if (key0 + BN < it.end) stage(k1, v1, key0 + BN);
+            tile(k0, v0, key0);
+            if (key0 + BN >= it.end) break;
+            landed_and_barrier();
+            if (key0 + 2 * BN < it.end) stage(k0, v0, key0 + 2 * BN);
+            tile(k1, v1, key0 + BN);
+        }
+    }
+    if (g.causal && any_not_finite<DP>(dq)) {
+        // see one_row in attention.hip: what the mask hides may have come in as 0 * NaN
+        clear<DP>(dq);
+        for (int j = 0; j <= last; ++j) {
+            const T *kr = kb + (long long)j * g.k_ts;
+            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qrow, kr, g.size), g.c, -lse));
+            add_row<T, DP>(dq, kr, p * (dot_rows(dorow, vb + (long long)j * g.v_ts, g.size) - delta), half, g.size);
+        }
+    }
+    if (row >= rows) return;
+    store_column<T, DP>(const_cast<T *>(at<T>(g.dq, place, g.dq_ts, head, g.dq_hs)), dq, g.scale, half, g.size);
+}
+
+template <class T, int DP, int BQ>
+__global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(const GradArgs g) {
+    constexpr int TILE = BQ * DP;
+    typedef Stager<T, DP, BQ, 4> St;
+    __shared__ T q0[TILE], d0[TILE], q1[TILE], d1[TILE];
+    __shared__ float l0[64], e0[64], l1[64], e1[64];           // lse, delta of the staged queries
+
+    int hk, n;
+    if (!dealt(g.deal, &hk, &n)) return;
+    const Item it = g.items[n];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int half = lane >> 5, col = lane & 31;
+    const int key_lo = it.row0 + wave * 32, key = key_lo + col, mine = key < it.k_len ? key : it.k_len - 1;
+    const T *krow = at<T>(g.k, it.k_start + mine, g.k_ts, hk, g.k_hs), *vrow = at<T>(g.v, it.k_start + mine, g.v_ts, hk, g.v_hs);
+    const ColumnRegs<T, DP> k = column_regs<T, DP>(krow, half, g.size), v = column_regs<T, DP>(vrow, half, g.size);
+    const int shift = it.k_len - it.q_len;
+    // the first token that sees this lane's key, all of the wavefront's, any of them
+    const int first = g.causal ? mine - shift : -1, all_see = g.causal ? key_lo + 31 - shift : -1, any_sees = key_lo >= it.k_len ? 0x7fffffff : g.causal ? key_lo - shift : -1;
+
+    floatx16 dk[DP / 32], dv[DP / 32];
+    clear<DP>(dk);
+    clear<DP>(dv);
+    St qs, ds;
+    qs.init(lane, wave, g.size, g.q_ts);
+    ds.init(lane, wave, g.size, g.do_ts);
+    const int span = it.end - it.begin, tiles = (span + BQ - 1) / BQ, total = span > 0 ? tiles * g.group : 0;
+    const long long stat_hs = (long long)g.kv_heads * g.group * g.lse_hs;
+
+    // step n: head n / tiles of the group, tokens from begin + (n % tiles) * BQ on
+    int next_h = 0, next_t = it.begin;
+    auto stage = [&](T *qt, T *dt, float *lt, float *et) {
+        const int h = hk * g.group + next_h, left = it.q_len - next_t;
+        qs.load(qt, at<T>(g.q, it.q_start + next_t, g.q_ts, h, g.q_hs), left, g.size, wave);
+        ds.load(dt, at<T>(g.dout, it.q_start + next_t, g.do_ts, h, g.do_hs), left, g.size, wave);
+        if (wave < 2) {
+            const float *s = g.stat + (wave ? stat_hs : 0) + (long long)h * g.lse_hs + it.q_start + next_t;
+            words_to_lds(wave ? et : lt, s, left < 64 ? left : 64, lane);
+        }
+        next_t += BQ;
+        if (next_t >= it.end) { next_t = it.begin; ++next_h; }
+    };
+    int tok0 = it.begin;
+    auto tile = [&](const T *qt, const T *dt, const float *lt, const float *et) {
+        const int t0 = tok0;
+        tok0 = tok0 + BQ >= it.end ? it.begin : tok0 + BQ;
+        if (t0 + BQ - 1 < any_sees) return;
+        const bool part = t0 < all_see;
+#pragma unroll
+        for (int b = 0; b < BQ / 32; ++b) {
+            floatx16 s = rows_by_column<T, DP>(qt, 32 * b + col, half, k);
+            floatx16 dp = rows_by_column<T, DP>(dt, 32 * b + col, half, v);
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const floatx4 l = *reinterpret_cast<const floatx4 *>(lt + 32 * b + row_of(r, half)), e = *reinterpret_cast<const floatx4 *>(et + 32 * b + row_of(r, half));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[r + i] = __builtin_amdgcn_exp2f(fmaf(s[r + i], g.c, -l[i]));
+                    dp[r + i] = s[r + i] * (dp[r + i] - e[i]);
+                }
+            }
+            if (part) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t0 + 32 * b + row_of(r, half) < first) s[r] = dp[r] = 0.f;
+            }
+            columns_by_result<T, DP>(dv, dt, 32 * b, lane, s);
+            columns_by_result<T, DP>(dk, qt, 32 * b, lane, dp);
+        }
+    };
+    if (total > 0) {
+        stage(q0, d0, l0, e0);
+        for (int i = 0; i < total; i += 2) {
+            landed_and_barrier();
+            if (i + 1 < total) stage(q1, d1, l1, e1);
+            tile(q0, d0, l0, e0);
+            if (i + 1 >= total) break;
+            landed_and_barrier();
+            if (i + 2 < total) stage(q0, d0, l0, e0);
+            tile(q1, d1, l1, e1);
+        }
+    }
+    if (g.causal && (any_not_finite<DP>(dk) || any_not_finite<DP>(dv))) {
+        clear<DP>(dk);
+        clear<DP>(dv);
+        for (int h = hk * g.group; h < (hk + 1) * g.group; ++h)
+            for (int i = first > 0 ? first : 0; i < it.q_len; ++i) {
+                const long long place = it.q_start + i;
+                const T *qr = at<T>(g.q, place, g.q_ts, h, g.q_hs), *dr = at<T>(g.dout, place, g.do_ts, h, g.do_hs);
+                const float *s = g.stat + (long long)h * g.lse_hs + place;
+                const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, krow, g.size), g.c, -s[0]));
+                add_row<T, DP>(dv, dr, p, half, g.size);
+                add_row<T, DP>(dk, qr, p * (dot_rows(dr, vrow, g.size) - s[stat_hs]), half, g.size);
+            }
+    }
+    if (key >= it.k_len) return;
+    store_column<T, DP>(const_cast<T *>(at<T>(g.dk, it.k_start + key, g.dk_ts, hk, g.dk_hs)), dk, g.scale, half, g.size);
+    store_column<T, DP>(const_cast<T *>(at<T>(g.dv, it.k_start + key, g.dv_ts, hk, g.dv_hs)), dv, 1.f, half, g.size);
+}
+
+template <class T, int DP> int launch_backward(GradArgs g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
+    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP == 32 ? 64 : 32;
+    unsigned grid;
+    if (n_q > 0) {
+        g.items = q_items;
+        g.deal = deal(n_q, g.kv_heads, &grid);
+        hipLaunchKernelGGL((attention_grad_queries<T, DP, BN>), dim3(grid), dim3(256), 0, stream, g);
+    }
+    if (n_k > 0) {
+        g.items = k_items;
+        g.deal = deal(n_k, g.kv_heads, &grid);
+        hipLaunchKernelGGL((attention_grad_keys<T, DP, BQ>), dim3(grid), dim3(256), 0, stream, g);
+    }
+    return check_launch("faith_attention_backward");
+}
+template <class T> int launch_backward(const GradArgs &g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
+    if (g.size <= 32) return launch_backward<T, 32>(g, q_items, n_q, k_items, n_k, stream);
+    if (g.size <= 64) return launch_backward<T, 64>(g, q_items, n_q, k_items, n_k, stream);
+    return launch_backward<T, 128>(g, q_items, n_q, k_items, n_k, stream);
+}
+
+}  // namespace
+
+extern "C" int faith_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
+                                        void *dq, void *dk, void *dv, float *stat, const int *query_items, int n_query_items,
+                                        const int *key_items, int n_key_items, const long long *strides, long long lse_head_stride,
+                                        int heads, int kv_heads, int size, int dtype, int causal, float scale, void *stream) {
+    FAITH_REQUIRE(n_query_items >= 0 && n_key_items >= 0, FAITH_ERR_SHAPE, "%s: %d and %d items", __func__, n_query_items, n_key_items);
+    if (n_query_items == 0 && n_key_items == 0) return FAITH_OK;
+    FAITH_NOT_NULL(strides);
+    const int rc = attention_shapes(__func__, heads, kv_heads, size, dtype, scale);
+    if (rc != FAITH_OK) return rc;
+    const int es = dtype == FAITH_F32 ? 4 : 2;
+    const struct { const char *name; const void *p; bool keys; } rows[8] = {{"dout", dout, false}, {"q", q, false}, {"k", k, true}, {"v", v, true},
+                                                                            {"out", out, false}, {"dq", dq, false}, {"dk", dk, true}, {"dv", dv, true}};
+    // a batch without queries or without keys may come without the tensors of that side
+    for (int i = 0; i < 8; ++i) {
+        if ((rows[i].keys ? n_key_items : n_query_items) == 0) continue;
+        if (!attention_rows(__func__, rows[i].name, rows[i].p, strides[2 * i], strides[2 * i + 1], size, es)) return rows[i].p ? FAITH_ERR_ALIGN : FAITH_ERR_NULL;
+    }
+    FAITH_REQUIRE(n_query_items == 0 || (lse && stat && query_items), FAITH_ERR_NULL, "%s: lse, stat or the query items are NULL", __func__);
+    FAITH_REQUIRE(n_key_items == 0 || key_items, FAITH_ERR_NULL, "%s: the key items are NULL", __func__);
+    GradArgs g;
+    g.dout = dout; g.q = q; g.k = k; g.v = v; g.out = out; g.lse = lse; g.dq = dq; g.dk = dk; g.dv = dv; g.stat = stat;
+    long long *to[16] = {&g.do_ts, &g.do_hs, &g.q_ts, &g.q_hs, &g.k_ts, &g.k_hs, &g.v_ts, &g.v_hs, &g.o_ts, &g.o_hs, &g.dq_ts, &g.dq_hs, &g.dk_ts, &g.dk_hs, &g.dv_ts, &g.dv_hs};
+    for (int i = 0; i < 16; ++i) *to[i] = strides[i];
+    g.lse_hs = lse_head_stride;
+    g.group = heads / kv_heads; g.kv_heads = kv_heads; g.size = size; g.causal = causal;
+    g.c = scale * 1.4426950408889634f; g.scale = scale;
+    const Item *qi = reinterpret_cast<const Item *>(query_items), *ki = reinterpret_cast<const Item *>(key_items);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == FAITH_F32) return launch_backward<float>(g, qi, n_query_items, ki, n_key_items, s);
+    if (dtype == FAITH_BF16) return launch_backward<__bf16>(g, qi, n_query_items, ki, n_key_items, s);
+    return launch_backward<_Float16>(g, qi, n_query_items, ki, n_key_items, s);
+}

@@ -1251,6 +1251,14 @@ def _scale(scale, size):
     return scale
 
 
+def _like_rows(t, rows):
+    """A contiguous result of t's shape; the places behind the packing's last row hold zeros."""
+    out = _empty(*t.shape, device=t.device, dtype=t.dtype)
+    if t.shape[0] > rows:
+        out[rows:].zero_()
+    return out
+
+
 def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=None):
     """softmax(scale q k^T) v of every sequence of `packing`, for the network itself (not its bounds).
 
@@ -1258,12 +1266,12 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
     consecutive.  causal: a query sees the keys up to its own place.  scale: default 1 / sqrt(size).  Returns out like q
     (and, with return_lse, the logarithm of every row's sum of exponentials, float32 [heads, tokens], which
     attention_backward takes).  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, and
-    their places in `out` not written."""
+    their places in an `out` that the caller brings not written."""
     heads, kv_heads, size, (qt, qh), (kt, kh), (vt, vh) = _attention_operands(q, k, v, packing)
     scale = _scale(scale, size)
     dev = q.device
     if out is None:
-        out = _empty(q.shape[0], heads, size, device=dev, dtype=q.dtype)
+        out = _like_rows(q, packing.tokens)
     ot, oh = _rows("out", out, packing.tokens, heads, size, q)
     lse = _empty(heads, packing.tokens, device=dev) if return_lse else None
     with _on(dev):
@@ -1274,6 +1282,31 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
         _lib.call("faith_attention", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(scratch), items, n, joins, kind,
                   qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size, _DTYPES[q.dtype], int(causal), scale, _stream(q))
     return (out, lse) if return_lse else out
+
+
+def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=None):
+    """Gradients of attention(): (dq, dk, dv), each of its operand's shape and type, from dout, the gradient of its result.
+    out, lse: what the forward call returned (return_lse=True); the other arguments as in that call.  Sums in float32;
+    the gradients of a key head add up those of the heads that share it.  The same bits on every call."""
+    import ctypes
+    heads, kv_heads, size, qs, ks, vs = _attention_operands(q, k, v, packing)
+    scale = _scale(scale, size)
+    dev = q.device
+    ds = _rows("dout", dout, packing.tokens, heads, size, q)
+    os_ = _rows("out", out, packing.tokens, heads, size, q)
+    _check("lse", lse, (heads, packing.tokens))
+    dq, dk, dv = _like_rows(q, packing.tokens), _like_rows(k, packing.keys), _like_rows(v, packing.keys)
+    row, kv_row = (heads * size, size), (kv_heads * size, size)
+    strides = (ctypes.c_longlong * 16)(*ds, *qs, *ks, *vs, *os_, *row, *kv_row, *kv_row)
+    with _on(dev):
+        es = q.element_size()
+        q_plan = packing.plan(_lib.ATTENTION_GRAD_QUERIES, heads, kv_heads, es, causal)
+        k_plan = packing.plan(_lib.ATTENTION_GRAD_KEYS, heads, kv_heads, es, causal)
+        stat = _empty(2, heads, packing.tokens, device=dev)
+        _lib.call("faith_attention_backward", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
+                  _ptr(stat), q_plan[1], q_plan[2], k_plan[1], k_plan[2], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
+                  size, _DTYPES[q.dtype], int(causal), scale, _stream(q))
+    return dq, dk, dv
 
 
 def _row_tensor(name, t, like=None, shape=None, dtype=None):

@@ -682,6 +682,18 @@ int faith_attention(const void *q, const void *k, const void *v, void *out, floa
                     int size, int dtype, int causal, float scale, void *stream);
 
 /*
+ * Gradients of faith_attention.  lse: as the forward call wrote it; strides: [16] token and head strides (elements) of
+ * dout, q, k, v, out, dq, dk, dv in this order, under the conditions of faith_attention; stat: 2 * heads * lse_head_stride
+ * floats of scratch that calls which may overlap must not share; the items of the passes FAITH_ATTENTION_GRAD_QUERIES and
+ * _GRAD_KEYS.  Two launches, no atomics: the same bits on every call.  A row that sees no key has dq = 0, a key that no
+ * query sees dk = dv = 0; what masked places hold does not matter.
+ */
+int faith_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
+                             void *dq, void *dk, void *dv, float *stat, const int *query_items, int n_query_items,
+                             const int *key_items, int n_key_items, const long long *strides, long long lse_head_stride,
+                             int heads, int kv_heads, int size, int dtype, int causal, float scale, void *stream);
+
+/*
  * The residual connection and the normalisation behind it, along rows of n:
  *   h = x + residual;  c = h - mean(h)  (FAITH_NORM_RMS: c = h);  z = c / sqrt(mean(c^2) + eps)  (FAITH_NORM_NO_VAR: z = c);
  *   y = weight z + bias
