@@ -141,10 +141,7 @@ __global__ void __launch_bounds__(256) residual_norm(const NormArgs g) {
         }
         r = 1.f / sqrtf(fmaf(across<WAVES, false>(q, slot[1], wave), inv_n, g.eps));
     }
-    if (g.stats && t == 0) {
-        g.stats[2 * row] = mean;
-        g.stats[2 * row + 1] = r;
-    }
+    if (g.stats && t == 0) g.stats[row] = r;
     float top = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -207,10 +204,7 @@ template <class T> __global__ void __launch_bounds__(256) residual_norm_any(cons
         }
         r = 1.f / sqrtf(fmaf(across<4, false>(q, slot[1], wave), inv_n, g.eps));
     }
-    if (g.stats && threadIdx.x == 0) {
-        g.stats[2 * (long long)blockIdx.x] = mean;
-        g.stats[2 * (long long)blockIdx.x + 1] = r;
-    }
+    if (g.stats && threadIdx.x == 0) g.stats[blockIdx.x] = r;
     auto y_at = [&](int e, float h) {
         float y = (h - mean) * r;
         if (w) y *= (float)w[e];
@@ -237,18 +231,21 @@ struct NormGradArgs {
     const void *dy, *dsum, *h, *weight;
     const float *stats;
     void *dx, *dweight, *dbias;
-    float *partial;              // [blocks][2][n]: this workgroup's sums for the weight's and the bias's gradient
+    float *partial;              // [blocks][2][n]: a workgroup's sums for the weight's and the bias's gradient
+    float *means;                // [rows], for the kernels of any width
     long long rows;
     int n, kind, blocks;
 };
 
-// dh = r (g - z mean(g z) [with the variance] - mean(g) [with the mean]) + dsum, g = w dy.  A workgroup goes over rows
+// dh = r (g - z mean(g z) [with the variance] - mean(g) [with the mean]) + dsum, g = w dy.  z comes from h as it was stored,
+// and so does the mean: against that of the unrounded sum a row of almost equal values would come out off by its rounding
+// over its spread.  A workgroup goes over rows
 // blockIdx.x, + gridDim.x, ...; its columns' sums of dy z and dy stay in registers until the end and go to a row of
 // `partial` of its own, which a second launch adds up in a fixed order: no atomics, the same bits every time.
 template <class T, int WAVES, int CH>
 __global__ void __launch_bounds__(256) residual_norm_grad(const NormGradArgs g) {
     constexpr int N = Group<T>::N, LANES = 64 * WAVES;
-    __shared__ float slot[2][2][4];
+    __shared__ float slot[2][2][4], mean_slot[2][4];
     const int wave = threadIdx.x >> 6, t = (int)threadIdx.x % LANES;
     const float inv_n = 1.f / (float)g.n;
     float dw[CH][N], db[CH][N];
@@ -261,16 +258,23 @@ __global__ void __launch_bounds__(256) residual_norm_grad(const NormGradArgs g) 
     for (long long row = (long long)blockIdx.x * (4 / WAVES) + wave / WAVES; row < g.rows; row += step, parity ^= 1) {
         const long long at = row * g.n;
         const T *dy = reinterpret_cast<const T *>(g.dy) + at, *hh = reinterpret_cast<const T *>(g.h) + at;
-        const float mean = g.kind == RMS ? 0.f : g.stats[2 * row], r = g.kind == NO_VAR ? 1.f : g.stats[2 * row + 1];
+        const float r = g.kind == NO_VAR ? 1.f : g.stats[row];
         float z[CH][N], d[CH][N];
-        float s0 = 0.f, s1 = 0.f;
+        float s0 = 0.f, s1 = 0.f, mean = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int e0 = (c * LANES + t) * N;
             if (e0 < g.n) { unpack(dy + e0, d[c]); unpack(hh + e0, z[c]); }
             else
 #pragma unroll
-                for (int e = 0; e < N; ++e) { d[c][e] = 0.f; z[c][e] = mean; }
+                for (int e = 0; e < N; ++e) d[c][e] = z[c][e] = 0.f;
+        }
+        if (g.kind != RMS) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < N; ++e) mean += z[c][e];
+            mean = across<WAVES, false>(mean, mean_slot[parity], wave) * inv_n;
         }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(256) residual_norm_grad(const NormGradArgs g) 
             if (g.weight && e0 < g.n) unpack(reinterpret_cast<const T *>(g.weight) + e0, w);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                z[c][e] = (z[c][e] - mean) * r;
+                z[c][e] = e0 < g.n ? (z[c][e] - mean) * r : 0.f;
                 dw[c][e] = fmaf(d[c][e], z[c][e], dw[c][e]);
                 db[c][e] += d[c][e];
                 if (g.weight && e0 < g.n) d[c][e] *= w[e];
@@ -335,11 +339,17 @@ __global__ void __launch_bounds__(256) residual_norm_grad(const NormGradArgs g) 
 
 // any width and alignment: dx, a workgroup to a row
 template <class T> __global__ void __launch_bounds__(256) residual_norm_grad_any(const NormGradArgs g) {
-    __shared__ float slot[2][4];
+    __shared__ float slot[3][4];
     const int wave = threadIdx.x >> 6;
     const long long row = blockIdx.x, at = row * g.n;
     const T *dy = reinterpret_cast<const T *>(g.dy) + at, *hh = reinterpret_cast<const T *>(g.h) + at, *w = reinterpret_cast<const T *>(g.weight);
-    const float mean = g.kind == RMS ? 0.f : g.stats[2 * row], r = g.kind == NO_VAR ? 1.f : g.stats[2 * row + 1], inv_n = 1.f / (float)g.n;
+    const float r = g.kind == NO_VAR ? 1.f : g.stats[row], inv_n = 1.f / (float)g.n;
+    float mean = 0.f;
+    if (g.kind != RMS) {
+        for (int e = threadIdx.x; e < g.n; e += 256) mean += (float)hh[e];
+        mean = across<4, false>(mean, slot[2], wave) * inv_n;
+    }
+    if (g.means && threadIdx.x == 0) g.means[row] = mean;
     float s0 = 0.f, s1 = 0.f;
     for (int e = threadIdx.x; e < g.n; e += 256) {
         const float d = (float)dy[e] * (w ? (float)w[e] : 1.f);
@@ -361,7 +371,7 @@ template <class T> __global__ void __launch_bounds__(256) residual_norm_columns_
     if (e >= g.n) return;
     float dw = 0.f, db = 0.f;
     for (long long row = blockIdx.y; row < g.rows; row += gridDim.y) {
-        const float mean = g.kind == RMS ? 0.f : g.stats[2 * row], r = g.kind == NO_VAR ? 1.f : g.stats[2 * row + 1];
+        const float mean = g.means[row], r = g.kind == NO_VAR ? 1.f : g.stats[row];
         const float d = (float)reinterpret_cast<const T *>(g.dy)[row * g.n + e];
         dw = fmaf(d, ((float)reinterpret_cast<const T *>(g.h)[row * g.n + e] - mean) * r, dw);
         db += d;
@@ -487,7 +497,8 @@ extern "C" int faith_residual_norm_backward(const void *dy, const void *dsum, co
     const Shape s = shape_of(n, dtype, whole);
     // rows of `partial` by the aligned rule, which is what the caller made room for; the kernel for any width writes as many
     const int blocks = grad_blocks(rows, shape_of(n, dtype, true).waves);
-    const NormGradArgs g = {dy, dsum, sum, weight, stats, dx, dweight, dbias, dweight || dbias ? partial : nullptr, rows, n, kind, blocks};
+    if (!dweight && !dbias) partial = nullptr;
+    const NormGradArgs g = {dy, dsum, sum, weight, stats, dx, dweight, dbias, partial, partial ? partial + 2LL * n * blocks : nullptr, rows, n, kind, blocks};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == FAITH_F32) return launch_grad<float>(g, s, st);
     if (dtype == FAITH_BF16) return launch_grad<__bf16>(g, s, st);

@@ -315,9 +315,31 @@ def bound_inputs(make_bounds, embeddings, indices, radii, p=2.0, norm=None, laye
     return bounds
 
 
+def _label(network, embeddings, label):
+    """`label`, or where it is None what the network itself answers (faith_amd.concrete: the sentence must live on the GPU)."""
+    if label is not None:
+        return label
+    from . import concrete
+    (label,) = concrete.predict(network, embeddings)
+    return label
+
+
+def _bounded(network):
+    """Refuses what only the concrete pass knows: a bound propagated without it would be no bound of this network."""
+    if getattr(network, "causal", False):
+        raise ValueError("bounds are not propagated through causal attention")
+    if network.layer_norm == "rms":
+        raise ValueError('bounds are not propagated through layer_norm = "rms"')
+    for layer in network.layers:
+        att = layer.attention.self
+        if getattr(att, "num_key_value_heads", att.num_attention_heads) != att.num_attention_heads:
+            raise ValueError("bounds are not propagated through heads that share keys")
+
+
 def propagate(bounds, network):
     """Embedding bounds -> bounds of the pooled output: every encoder layer, then the pooler
     (the body of VerifierForward.verify_safety, :98-116)."""
+    _bounded(network)
     for layer in network.layers:
         _, _, bounds = bound_layer(bounds, layer, network.layer_norm, network.hidden_act)
     return bounds
@@ -326,7 +348,9 @@ def propagate(bounds, network):
 def verify_safety(make_bounds, network, embeddings, index, eps, label, p=2.0, perturbed_words=1, buffers=None):
     """VerifierForward.verify_safety (:93-125): True if the label provably survives every
     perturbation of norm <= eps of the embedding at `index`.  A failed precondition inside the
-    propagation (reciprocal or sqrt of a bound that reaches zero) counts as not verified, as there."""
+    propagation (reciprocal or sqrt of a bound that reaches zero) counts as not verified, as there.
+    label None (here and below): the class that the network answers for the unperturbed sentence."""
+    label = _label(network, embeddings, label)
     with _scope(buffers):
         return _verify_safety(make_bounds, network, embeddings, index, eps, label, p, perturbed_words)
 
@@ -358,6 +382,7 @@ def verify_safety_batch(make_bounds, network, embeddings, indices, radii, label,
     """verify_safety for several (position, radius) pairs of one sentence in one propagation.
     Returns a list of bools.  Needs a bound object that reports failed preconditions per batch
     element instead of raising (`collect_failures`, as faith_amd.Bounds has)."""
+    label = _label(network, embeddings, label)
     x = bound_inputs(make_bounds, embeddings, indices, radii, p)
     with _scope(buffers), type(x).collect_failures(len(indices), embeddings.device) as failed:
         if network.embedding_norm is not None:
@@ -374,7 +399,9 @@ def certified_radii(make_bounds, network, embeddings, positions, label, p=2.0, m
     max_eps; num_iters times { m = (l + r) / 2; verified at m ? l = m : r = m }; the answer is l.
     batched = True runs step j of all positions as one propagation; captured = True also replays
     that propagation from a HIP graph captured at the first step.  buffers: persistent result buffers shared
-    by all steps (see _scope); every step overwrites what the one before produced."""
+    by all steps (see _scope); every step overwrites what the one before produced.
+    faith_amd.concrete.adversarial_radii is the other side: radii at which the answer does break."""
+    label = _label(network, embeddings, label)
     lo = [0.0] * len(positions)
     hi = [float(max_eps)] * len(positions)
     if batched or captured:
@@ -412,6 +439,7 @@ class CapturedVerifier:
     def __init__(self, make_bounds, network, embeddings, batch, label, p=2.0):
         length, dim = embeddings.shape[1], embeddings.shape[2]
         dev = embeddings.device
+        label = _label(network, embeddings, label)
         self.batch, self.label, self.dim, self.length, self.make_bounds = batch, label, dim, length, make_bounds
         self.b = embeddings[0].unsqueeze(0).expand(batch, length, dim).contiguous()
         compact = _compact_maker(make_bounds, batch, length, dim, dim, captured=True)

@@ -1366,7 +1366,7 @@ def residual_norm(x, residual=None, weight=None, bias=None, kind="rms", eps=1e-6
     else:
         raise ValueError(f"quantize={quantize!r}: one of {', '.join(_BITS)} or None")
     h = x if residual is None else _empty_like(x)
-    stats = _empty(*x.shape[:-1], 2, device=x.device) if return_stats else None
+    stats = _empty(*x.shape[:-1], device=x.device) if return_stats else None
     with _on(x.device):
         _lib.call("faith_residual_norm", _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y), None if residual is None else _ptr(h),
                   _ptr(stats), _ptr(scales), rows, n, code, _DTYPES[x.dtype], bits, eps, _stream(x))
@@ -1379,7 +1379,7 @@ def residual_norm_backward(dy, h, weight, stats, kind="rms", dsum=None, with_wei
     forward call returned them.  Returns (dx, dweight, dbias): dx is the gradient of x and of the residual alike, dweight and
     dbias are None where they are not wanted.  The same bits on every call."""
     rows, n, code = _norm_operands(h, (("dy", dy), ("dsum", dsum)), (("weight", weight),), kind)
-    _row_tensor("stats", stats, h, (*h.shape[:-1], 2), torch.float32)
+    _row_tensor("stats", stats, h, h.shape[:-1], torch.float32)
     dev = h.device
     dx = _empty_like(h)
     dweight = _empty(n, device=dev, dtype=h.dtype) if with_weight else None
@@ -1387,7 +1387,7 @@ def residual_norm_backward(dy, h, weight, stats, kind="rms", dsum=None, with_wei
     with _on(dev):
         partial = None
         if with_weight or with_bias:
-            partial = _empty(max(1, _lib.lib.faith_residual_norm_blocks(rows, n, _DTYPES[h.dtype])) * 2 * n, device=dev)
+            partial = _empty(max(1, _lib.lib.faith_residual_norm_blocks(rows, n, _DTYPES[h.dtype])) * 2 * n + rows, device=dev)
         _lib.call("faith_residual_norm_backward", _ptr(dy), _ptr(dsum), _ptr(h), _ptr(weight), _ptr(stats), _ptr(dx), _ptr(dweight),
                   _ptr(dbias), _ptr(partial), rows, n, code, _DTYPES[h.dtype], _stream(h))
     return dx, dweight, dbias

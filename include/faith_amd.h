@@ -697,8 +697,8 @@ int faith_attention_backward(const void *dout, const void *q, const void *k, con
  * The residual connection and the normalisation behind it, along rows of n:
  *   h = x + residual;  c = h - mean(h)  (FAITH_NORM_RMS: c = h);  z = c / sqrt(mean(c^2) + eps)  (FAITH_NORM_NO_VAR: z = c);
  *   y = weight z + bias
- * residual, weight, bias may be NULL; sum (h, rounded to dtype; y is computed from the unrounded one), stats ([rows, 2]: mean
- * and 1 / sqrt(...), what the gradient needs) too.  bits != 0: y holds 8-bit values and scales [rows] their scales,
+ * residual, weight, bias may be NULL; sum (h, rounded to dtype; y is computed from the unrounded one), stats ([rows]: 1 / sqrt(...),
+ * 1 for FAITH_NORM_NO_VAR; what the gradient needs) too.  bits != 0: y holds 8-bit values and scales [rows] their scales,
  * y ~ q * scale, scale = max |y| / 127 (FAITH_BITS_INT8) or / 448 (FAITH_BITS_E4M3, the OCP format), q rounded to nearest
  * even; a row of zeros has scale 0.  A NaN in y becomes 0 in int8 and stays NaN in e4m3.
  */
@@ -713,7 +713,8 @@ int faith_residual_norm(const void *x, const void *residual, const void *weight,
 /*
  * Gradients of faith_residual_norm: dx (of x and of the residual alike) from dy and, if not NULL, the gradient dsum that
  * reaches h by other ways; dweight = sum over rows of dy z, dbias = sum of dy (NULL: not wanted).  sum, stats: as the forward
- * call left them.  partial: 2 * n * faith_residual_norm_blocks(rows, n, dtype) floats of scratch if dweight or dbias are wanted.
+ * call left them (z is that of the rounded sum).  partial: rows + 2 * n * faith_residual_norm_blocks(rows, n, dtype) floats of
+ * scratch if dweight or dbias are wanted.
  */
 int faith_residual_norm_blocks(long long rows, int n, int dtype);   /* answers a number of rows of scratch, not a status */
 int faith_residual_norm_backward(const void *dy, const void *dsum, const void *sum, const void *weight, const float *stats,

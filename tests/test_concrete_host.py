@@ -1,0 +1,224 @@
+"""The concrete pass on the host: work items, refusals, the C ABI's argument checks.  No GPU is needed."""
+import ctypes
+import math
+import random
+
+import pytest
+import torch
+
+from faith_amd import _lib, concrete, forward, ops
+
+
+def plan(lengths, key_lengths, heads, kv_heads, element_size, causal, which):
+    n = len(lengths)
+    ql, kl, counts = (ctypes.c_int * n)(*lengths), (ctypes.c_int * n)(*key_lengths), (ctypes.c_longlong * 4)()
+    args = (ctypes.addressof(ql), ctypes.addressof(kl), n, heads, kv_heads, element_size, int(causal), which)
+    _lib.call("faith_attention_plan", *args, None, 0, ctypes.addressof(counts))
+    total = counts[0] + counts[1]
+    out = torch.full((total + 1, 8), -7, dtype=torch.int32)
+    _lib.call("faith_attention_plan", *args, out.data_ptr(), total, ctypes.addressof(counts))
+    assert bool((out[total] == -7).all())
+    rows = out.tolist()
+    return rows[:counts[0]], rows[counts[0]:total], counts[2], counts[3]
+
+
+CASES = [([5], [5], 4, 4), ([1, 1, 1], [700, 3, 65], 8, 2), ([130, 0, 7], [300, 5, 0], 2, 1), ([40, 9], [10, 9], 3, 1),
+         ([1], [8192], 32, 8), ([1000, 33], [1000, 33], 12, 4), ([128], [16384], 8, 1), ([1] * 70, list(range(70)), 4, 4)]
+
+
+@pytest.mark.parametrize("lengths, key_lengths, heads, kv_heads", CASES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("element_size", [2, 4])
+def test_forward_items_cover_every_row_and_key_once(lengths, key_lengths, heads, kv_heads, causal, element_size):
+    items, joins, slots, kind = plan(lengths, key_lengths, heads, kv_heads, element_size, causal, _lib.ATTENTION_FORWARD)
+    group, rows_per = heads // kv_heads, 32 if kind else 128
+    assert kind == (max(lengths) * group <= 32)
+    spans, used = {}, []
+    for qs, ql, ks, kl, row0, begin, end, slot in items:
+        spans.setdefault((qs, ql, ks, kl, row0), []).append((begin, end, slot))
+        assert 0 <= begin <= max(end, 0) and end <= kl and row0 % rows_per == 0 and row0 < ql * group
+        if slot >= 0:
+            used.append(slot)
+    assert sorted(used) == list(range(slots))
+    joined = {tuple(j[:5]): (j[5], j[7]) for j in joins}
+    assert len(joined) == len(joins)
+    a = b = 0
+    for n, m in zip(lengths, key_lengths):
+        for row0 in range(0, n * group, rows_per):
+            parts = sorted(spans.pop((a, n, b, m, row0)))
+            last = (min(n * group, row0 + rows_per) - 1) // group
+            end = max(0, min(m, last + m - n + 1)) if causal else m
+            assert parts[0][0] == 0 and parts[-1][1] == end
+            assert all(x[1] == y[0] for x, y in zip(parts, parts[1:]))
+            if len(parts) == 1:
+                assert parts[0][2] == -1
+            else:
+                n_parts, first = joined[(a, n, b, m, row0)]
+                assert sorted(p[2] for p in parts) == list(range(first, first + n_parts))
+        a, b = a + n, b + m
+    assert not spans
+
+
+@pytest.mark.parametrize("lengths, key_lengths, heads, kv_heads", CASES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_key_items_cover_every_key_and_every_query_that_sees_it(lengths, key_lengths, heads, kv_heads, causal):
+    items, joins, slots, _ = plan(lengths, key_lengths, heads, kv_heads, 2, causal, _lib.ATTENTION_GRAD_KEYS)
+    assert not joins and not slots
+    seen = set()
+    for qs, ql, ks, kl, key0, begin, end, slot in items:
+        assert slot == -1 and end == ql and 0 <= begin
+        first = max(0, key0 - (kl - ql)) if causal else 0       # the first query that sees the tile's first key
+        assert begin <= first
+        seen.add((ks, kl, key0))
+    b = 0
+    want = set()
+    for m in key_lengths:
+        want |= {(b, m, key0) for key0 in range(0, m, 128)}
+        b += m
+    assert seen == want
+
+
+def test_items_are_laid_down_longest_first():
+    items, _, _, _ = plan([3000, 10, 500], [3000, 10, 500], 4, 4, 2, True, _lib.ATTENTION_GRAD_QUERIES)
+    spans = [i[6] - i[5] for i in items]
+    assert spans == sorted(spans, reverse=True)
+
+
+def test_plan_refuses_what_it_cannot_lay_down():
+    L = _lib.lib
+    one, counts = (ctypes.c_int * 1)(4), (ctypes.c_longlong * 4)()
+    p, c = ctypes.addressof(one), ctypes.addressof(counts)
+    ok = lambda *a: L.faith_attention_plan(*a)
+    assert ok(None, p, 1, 4, 4, 2, 0, 0, None, 0, c) == -1
+    assert ok(p, p, 0, 4, 4, 2, 0, 0, None, 0, c) == -2
+    assert ok(p, p, 1, 4, 3, 2, 0, 0, None, 0, c) == -2
+    assert ok(p, p, 1, 4, 4, 3, 0, 0, None, 0, c) == -3
+    assert ok(p, p, 1, 4, 4, 2, 0, 9, None, 0, c) == -3
+    one[0] = -1
+    assert ok(p, p, 1, 4, 4, 2, 0, 0, None, 0, c) == -2
+    one[0] = 400
+    room = (ctypes.c_int * 8)()
+    assert ok(p, p, 1, 4, 4, 2, 0, 0, ctypes.addressof(room), 1, c) == -2 and b"room" in L.faith_last_error()
+
+
+def test_entry_points_check_on_the_host():
+    """Misaligned, overlapping, missing: a status, before anything is launched."""
+    L = _lib.lib
+    buf = (ctypes.c_float * 256)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+
+    def forward_call(q=p, k=p, v=p, out=p, items=p, n=1, ts=64, hs=16, heads=4, kv_heads=4, size=16, dtype=0, scale=0.5, joins=0, kind=0):
+        return L.faith_attention(q, k, v, out, None, None, items, n, joins, kind, ts, hs, ts, hs, ts, hs, ts, hs, 4, heads, kv_heads, size,
+                                 dtype, 0, scale, None)
+    assert forward_call(n=0) == 0
+    assert forward_call(q=None) == -1 and forward_call(items=None) == -1 and forward_call(joins=1) == -1
+    assert forward_call(k=None) == -4 and forward_call(q=p + 4) == -4 and forward_call(ts=8) == -4 and forward_call(hs=2) == -4 and forward_call(ts=1 << 22) == -4
+    assert forward_call(size=18) == -3 and forward_call(size=132) == -3 and forward_call(size=4, dtype=1) == -3
+    assert forward_call(dtype=3) == -3 and forward_call(kind=2) == -3 and forward_call(scale=0.0) == -3 and forward_call(scale=math.nan) == -3
+    assert forward_call(kv_heads=3) == -2
+    strides = (ctypes.c_longlong * 16)(*[64, 16] * 8)
+
+    def backward_call(t=p, lse=p, stat=p, n=1, s=ctypes.addressof(strides), size=16, scale=0.5):
+        return L.faith_attention_backward(t, t, t, t, t, lse, t, t, t, stat, p, n, p, n, s, 4, 4, 4, size, 0, 0, scale, None)
+    assert backward_call(n=0) == 0
+    assert backward_call(t=None) == -1 and backward_call(lse=None) == -1 and backward_call(stat=None) == -1 and backward_call(s=None) == -1
+    assert backward_call(t=p + 4) == -4 and backward_call(size=130) == -3 and backward_call(scale=-1.0) == -3
+
+    def norm_call(x=p, y=p, rows=1, n=8, kind=0, dtype=0, bits=0, scales=p, eps=1e-6):
+        return L.faith_residual_norm(x, None, None, None, y, None, None, scales, rows, n, kind, dtype, bits, eps, None)
+    assert norm_call(rows=0) == 0
+    assert norm_call(x=None) == -1 and norm_call(y=None) == -1 and norm_call(bits=1, scales=None) == -1
+    assert norm_call(n=0) == -2 and norm_call(rows=-1) == -2
+    assert norm_call(kind=3) == -3 and norm_call(dtype=5) == -3 and norm_call(bits=3) == -3 and norm_call(eps=-1.0) == -3 and norm_call(eps=math.nan) == -3
+    assert L.faith_residual_norm_backward(p, None, p, None, p, p, p, None, None, 1, 8, 0, 0, None) == -1
+    assert L.faith_residual_norm_backward(p, None, p, None, None, p, None, None, None, 1, 8, 0, 0, None) == -1
+    assert L.faith_residual_norm_backward(p, None, p, None, p, p, None, None, None, 1, 8, 7, 0, None) == -3
+
+
+@pytest.mark.parametrize("lengths, keys, what", [([], None, "no sequences"), ([3, -1], None, "not a length"), ([2.5], None, "not a length"),
+                                                 ([True], None, "not a length"), ([3], [3, 3], "1 sequences of queries, 2 of keys"),
+                                                 ([1 << 30], None, "not a length"), ([(1 << 30) - 1] * 3, None, "2\\^31")])
+def test_packing_checks_lengths(lengths, keys, what):
+    with pytest.raises(ValueError, match=what):
+        ops.Packing(lengths, keys)
+
+
+def test_packing_lives_on_the_gpu():
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.Packing([3], device="cpu")
+    assert ops.Packing(torch.tensor([3, 0, 2])).starts() == [0, 3, 3, 5]
+
+
+def test_operators_refuse_cpu_tensors_and_other_types():
+    packing = ops.Packing([3])
+    q = torch.zeros(3, 2, 16)
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.attention(q, q, q, packing)
+    with pytest.raises(TypeError, match="Packing"):
+        ops.attention(q, q, q, [3])
+    with pytest.raises(TypeError, match="tensor"):
+        ops.attention(None, q, q, packing)
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.residual_norm(torch.zeros(3, 16))
+    with pytest.raises(TypeError, match="tensor"):
+        ops.residual_norm([1.0])
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.residual_norm_backward(torch.zeros(3, 16), torch.zeros(3, 16), None, torch.zeros(3))
+
+
+def test_concrete_checks_embeddings_and_positions():
+    with pytest.raises(ValueError, match="embeddings"):
+        concrete._rows_of(torch.zeros(3, 4), None)
+    with pytest.raises(ValueError, match="embeddings"):
+        concrete._rows_of(torch.zeros(2, 3, 4), [3, 3])
+    with pytest.raises(ValueError, match="2 positions, 1 radii"):
+        concrete.falsify(None, torch.zeros(1, 4, 8), [1, 2], [0.1], 0)
+    with pytest.raises(ValueError, match="outside"):
+        concrete.falsify(None, torch.zeros(1, 4, 8), [4], [0.1], 0)
+    assert concrete.falsify(None, torch.zeros(1, 4, 8), [], [], 0) == []
+
+
+@pytest.mark.parametrize("p", [1.0, 1.5, 2.0, 3.0, math.inf])
+def test_steps_of_the_search_stay_in_the_ball_and_ascend(p):
+    g = torch.Generator().manual_seed(5)
+    x, r = torch.randn(6, 9, generator=g), torch.tensor([0.1, 0.5, 1.0, 2.0, 0.0, 3.0])
+    d = concrete._steepest(x, p)
+    norm = lambda t: torch.linalg.vector_norm(t, ord=p, dim=1)
+    assert torch.allclose(norm(d), torch.ones(6), rtol=1e-5)
+    # no direction of unit norm grows a linear function faster than its dual norm says
+    q = math.inf if p == 1 else 1.0 if math.isinf(p) else p / (p - 1)
+    assert torch.allclose((x * d).sum(1), torch.linalg.vector_norm(x, ord=q, dim=1), rtol=1e-5)
+    inside = concrete._into_ball(x, p, r)
+    assert bool((norm(inside) <= r * (1 + 1e-5)).all())
+
+
+def test_bounds_of_what_only_the_concrete_pass_knows_are_refused():
+    from types import SimpleNamespace
+    from faith_amd.workloads import random_layer
+    g = torch.Generator().manual_seed(3)
+    net = SimpleNamespace(embedding_norm=None, layers=[random_layer(g, 16, 4, 32)], layer_norm="no_var", hidden_act="relu")
+    forward._bounded(net)
+    net.causal = True
+    with pytest.raises(ValueError, match="causal"):
+        forward.propagate(None, net)
+    net.causal, net.layer_norm = False, "rms"
+    with pytest.raises(ValueError, match="rms"):
+        forward.propagate(None, net)
+    net.layer_norm = "standard"
+    net.layers[0].attention.self.num_key_value_heads = 2
+    with pytest.raises(ValueError, match="share"):
+        forward.propagate(None, net)
+
+
+def test_random_lengths_give_items_within_the_sequences():
+    rng = random.Random(8)
+    for _ in range(60):
+        n = rng.randint(1, 9)
+        ql = [rng.choice([0, 1, rng.randint(0, 400)]) for _ in range(n)]
+        kl = [rng.choice([0, 1, rng.randint(0, 900)]) for _ in range(n)]
+        kv = rng.choice([1, 2, 8])
+        for which in range(3):
+            items, joins, slots, kind = plan(ql, kl, kv * rng.choice([1, 3, 4]), kv, rng.choice([2, 4]), rng.random() < 0.5, which)
+            for qs, a, ks, b, row0, begin, end, slot in items:
+                i = next(i for i in range(n) if sum(ql[:i]) == qs and sum(kl[:i]) == ks and (ql[i], kl[i]) == (a, b))
+                assert 0 <= begin and end <= (b if which < 2 else a) and slot < max(1, slots), i

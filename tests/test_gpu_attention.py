@@ -1,0 +1,314 @@
+"""Attention of the concrete pass and its gradients against the definition in float64 (tests/concrete_reference.py, which also
+derives how far roundings may carry a result)."""
+import math
+
+import pytest
+import torch
+
+from tests import concrete_reference as R
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+SHAPES = [  # lengths, key lengths (None: alike), heads, key heads, causal
+    ([5, 1, 33], None, 4, 2, True),
+    ([32] * 3, None, 4, 4, False),
+    ([128, 65, 200], None, 6, 2, True),
+    ([1, 1, 1], [700, 3, 65], 8, 2, True),
+    ([1, 4], [3000, 20], 4, 4, False),
+    ([130, 0, 7], [300, 5, 0], 2, 1, True),       # no queries; no keys
+    ([40, 9], [10, 9], 3, 1, True),               # the first 30 queries see nothing
+    ([70], [5000], 4, 2, False),
+    ([1], [1], 1, 1, True),
+    ([31, 64, 129], [63, 64, 127], 2, 2, False),
+]
+
+
+def tensors(lengths, keys, heads, kv_heads, size, dtype, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda t, h: (torch.randn(t, h, size, generator=g, device="cuda") * scale).to(dtype)
+    return rnd(sum(lengths), heads), rnd(sum(keys), kv_heads), rnd(sum(keys), kv_heads), rnd(sum(lengths), heads)
+
+
+@pytest.mark.parametrize("dtype, size", [(F32, 64), (F32, 4), (F32, 32), (F32, 100), (F32, 128), (BF16, 8), (BF16, 32), (BF16, 64), (BF16, 80),
+                                         (BF16, 128), (F16, 64), (F16, 96), (F16, 128)])
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_attention_and_gradients(case, dtype, size):
+    from faith_amd import ops
+    lengths, keys, heads, kv_heads, causal = SHAPES[case]
+    keys = keys or lengths
+    q, k, v, dout = tensors(lengths, keys, heads, kv_heads, size, dtype, seed=case)
+    packing = ops.Packing(lengths, keys)
+    out, lse = ops.attention(q, k, v, packing, causal=causal, return_lse=True)
+    grads = ops.attention_backward(dout, q, k, v, out, lse, packing, causal=causal)
+    r = R.attention(q, k, v, lengths, keys, causal, 1 / math.sqrt(size), dout)
+    R.check("out", out, r["out"], r["out_tol"])
+    assert bool((torch.isinf(lse) == torch.isinf(r["lse"])).all())
+    R.check("lse", lse, r["lse"], r["lse_tol"] + 1e-30)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        assert got.dtype == dtype
+        R.check(name, got, r[name], r[name + "_tol"])
+    # without the logarithms: the same result; the same call: the same bits
+    assert torch.equal(out, ops.attention(q, k, v, packing, causal=causal))
+    again = ops.attention_backward(dout, q, k, v, out, lse, packing, causal=causal)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale, spread", [(0.3, 1.0), (1.0, 6.0), (4.0, 0.01)])
+def test_scores_far_apart_and_other_scales(dtype, scale, spread):
+    """Large scores: the running reference moves many times.  (Scores of hundreds: a probability's error grows with them,
+    and the tolerance with it.)"""
+    from faith_amd import ops
+    lengths = [300, 77]
+    q, k, v, dout = tensors(lengths, lengths, 2, 1, 64, dtype, 3, 1.0)
+    q = (q.float() * spread).to(dtype)
+    k = (k.float() * torch.linspace(0.1, 1, k.shape[0], device="cuda")[:, None, None]).to(dtype)      # later keys larger: later maxima
+    packing = ops.Packing(lengths)
+    out, lse = ops.attention(q, k, v, packing, causal=True, scale=scale, return_lse=True)
+    grads = ops.attention_backward(dout, q, k, v, out, lse, packing, causal=True, scale=scale)
+    r = R.attention(q, k, v, lengths, lengths, True, scale, dout)
+    R.check("out", out, r["out"], r["out_tol"])
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        R.check(name, got, r[name], r[name + "_tol"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_views_of_one_projection_and_other_layouts(dtype):
+    """q, k, v as slices of one [tokens, (heads + 2 key heads) * size] array; heads in front; a result that the caller brings,
+    inside a larger array whose other places stay as they were."""
+    from faith_amd import ops
+    lengths, heads, kv_heads, size = [37, 90], 4, 2, 32
+    g = torch.Generator(device="cuda").manual_seed(1)
+    t = sum(lengths)
+    both = torch.randn(t + 3, (heads + 2 * kv_heads) * size, generator=g, device="cuda").to(dtype)
+    both[t:] = math.nan                                                    # rows behind the last sequence
+    q, k, v = both.view(t + 3, -1, size).split([heads, kv_heads, kv_heads], 1)
+    packing = ops.Packing(lengths)
+    want = ops.attention(q[:t].contiguous(), k[:t].contiguous(), v[:t].contiguous(), packing, causal=True)
+    got, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
+    assert torch.equal(got[:t], want) and bool((got[t:] == 0).all())
+    large = torch.full((t + 5, heads + 1, size), 7.0, device="cuda", dtype=dtype)
+    ops.attention(q, k, v, packing, causal=True, out=large[2:, 1:])
+    assert torch.equal(large[2:t + 2, 1:], want)
+    assert bool((large[:2] == 7).all()) and bool((large[t + 2:] == 7).all()) and bool((large[:, 0] == 7).all())
+    front = lambda x: x[:t].transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(ops.attention(front(q), front(k), front(v), packing, causal=True), want)
+    dout = torch.randn(t, heads, size, generator=g, device="cuda").to(dtype)
+    a = ops.attention_backward(front(dout), q, k, v, got, lse, packing, causal=True)
+    b = ops.attention_backward(dout, q[:t].contiguous(), k[:t].contiguous(), v[:t].contiguous(), want, lse, packing, causal=True)
+    assert all(torch.equal(x[:t], y) and bool((x[t:] == 0).all()) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("lengths, keys", [([50], [50]), ([3], [400]), ([200], [200]), ([2], [3000])])
+def test_masked_places_may_hold_anything(dtype, bad, lengths, keys):
+    """NaN or infinity in the last key and value: every query but the last is masked from it.  In the first query and its
+    gradient: every key behind the first that it sees is masked from it."""
+    from faith_amd import ops
+    q, k, v, dout = tensors(lengths, keys, 2, 1, 64, dtype, 9)
+    n, packing = lengths[0], ops.Packing(lengths, keys)
+    scale = 1 / math.sqrt(64)
+    k0, v0 = k.clone(), v.clone()
+    k0[-1], v0[-1] = 0, 0
+    k[-1, :, 5], v[-1, :, 7] = bad, bad
+    r = R.attention(q, k0, v0, lengths, keys, True, scale, dout)
+    out, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
+    R.check("out", out[:n - 1], r["out"][:n - 1], r["out_tol"][:n - 1])
+    dq, _, _ = ops.attention_backward(dout, q, k, v, out, lse, packing, causal=True)
+    R.check("dq", dq[:n - 1], r["dq"][:n - 1], r["dq_tol"][:n - 1])
+    # and the other way round
+    q, k, v, dout = tensors(lengths, keys, 2, 1, 64, dtype, 10)
+    q0, dout0 = q.clone(), dout.clone()
+    q0[0], dout0[0] = 0, 0
+    q[0, :, 3], dout[0, :, 2] = bad, bad
+    out, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
+    _, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing, causal=True)
+    r = R.attention(q0, k, v, lengths, keys, True, scale, dout0)
+    seen = keys[0] - n + 1                                                  # keys that the first query sees
+    R.check("dk", dk[seen:], r["dk"][seen:], r["dk_tol"][seen:])
+    R.check("dv", dv[seen:], r["dv"][seen:], r["dv_tol"][seen:])
+
+
+def test_not_a_number_where_it_is_seen_stays_one():
+    from faith_amd import ops
+    q, k, v, _ = tensors([40], [40], 1, 1, 32, BF16, 2)
+    v[17, 0, 3] = math.nan
+    out = ops.attention(q, k, v, ops.Packing([40]), causal=True)
+    assert bool(torch.isnan(out[17:, 0, 3]).all()) and not bool(torch.isnan(out[:17]).any())
+    assert not bool(torch.isnan(out[:, 0, :3]).any()) and not bool(torch.isnan(out[:, 0, 4:]).any())
+
+
+@pytest.mark.parametrize("kv_heads, heads, lengths, keys", [(8, 32, [1] * 5, [8192, 1, 513, 4000, 257]), (1, 1, [1], [20000]), (2, 16, [2, 1], [3000, 300]),
+                                                            (1, 1, [32], [7000]), (1, 4, [128], [9000])])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_rows_against_many_keys(kv_heads, heads, lengths, keys, dtype):
+    """Keys cut into parts and joined."""
+    from faith_amd import _lib, ops
+    q, k, v, _ = tensors(lengths, keys, heads, kv_heads, 128, dtype, 4)
+    packing = ops.Packing(lengths, keys)
+    assert packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), True)[3] > 0
+    out, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
+    r = R.attention(q, k, v, lengths, keys, True, 1 / math.sqrt(128))
+    R.check("out", out, r["out"], r["out_tol"])
+    R.check("lse", lse, r["lse"], r["lse_tol"])
+
+
+def test_offsets_past_32_bits():
+    """A cache whose last sequence starts 4.3 GB into the array."""
+    from faith_amd import ops
+    skip, heads, size = (1 << 32) // (8 * 128 * 2) + 1000, 8, 128
+    k = torch.empty(skip + 300, heads, size, device="cuda", dtype=BF16)
+    v = torch.empty_like(k)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k[skip:] = torch.randn(300, heads, size, generator=g, device="cuda").to(BF16)
+    v[skip:] = torch.randn(300, heads, size, generator=g, device="cuda").to(BF16)
+    q = torch.randn(200, heads, size, generator=g, device="cuda").to(BF16)
+    for n in (1, 200):
+        got = ops.attention(q[:n], k, v, ops.Packing([0, n], [skip, 300]), causal=True)
+        want = ops.attention(q[:n], k[skip:], v[skip:], ops.Packing([n], [300]), causal=True)
+        assert torch.equal(got, want)
+
+
+def test_gradients_against_differences():
+    """Along random directions, central differences of the definition in float64: the error of a difference of step h is
+    h^2 / 6 times a third derivative (of order one here) plus rounding of 1e-16 / h."""
+    from faith_amd import ops
+    lengths, heads, kv_heads, size = [13, 30], 4, 2, 16
+    q, k, v, dout = tensors(lengths, lengths, heads, kv_heads, size, F32, 6)
+    packing = ops.Packing(lengths)
+    out, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
+    grads = ops.attention_backward(dout, q, k, v, out, lse, packing, causal=True)
+
+    def loss(*x):
+        total, a = 0.0, 0
+        for n in lengths:
+            for h in range(heads):
+                qs, ks, vs = x[0][a:a + n, h], x[1][a:a + n, h // 2], x[2][a:a + n, h // 2]
+                s = (qs @ ks.t() / math.sqrt(size)).masked_fill(torch.ones(n, n, device="cuda").triu(1).bool(), -math.inf)
+                total = total + (torch.softmax(s, 1) @ vs * dout[a:a + n, h].double()).sum()
+            a += n
+        return total
+    g = torch.Generator(device="cuda").manual_seed(7)
+    base, h = [t.double() for t in (q, k, v)], 1e-4
+    for i in range(3):
+        d = torch.randn(base[i].shape, generator=g, device="cuda", dtype=torch.float64)
+        d /= d.norm()
+        up, down = list(base), list(base)
+        up[i], down[i] = base[i] + h * d, base[i] - h * d
+        want = float(loss(*up) - loss(*down)) / (2 * h)
+        # the gradient's own error: some 1e-6 of its norm, along a unit direction
+        assert abs(float((grads[i].double() * d).sum()) - want) <= 1e-5 * float(grads[i].norm()) + 1e-6
+
+
+def test_captured_and_replayed_between_eager_work():
+    from faith_amd import ops
+    lengths, keys = [60, 7, 200], [60, 900, 200]
+    q, k, v, dout = tensors(lengths, keys, 4, 2, 64, BF16, 8)
+    packing, one = ops.Packing(lengths, keys), ops.Packing([1] * 3, keys)
+
+    def body():
+        out, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
+        return (out, *ops.attention_backward(dout, q, k, v, out, lse, packing, causal=True), ops.attention(q[:3], k, v, one))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        body()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    results = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            results.append(body())
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, device="cuda").to(BF16))
+        want = body()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(want, result)), i
+
+
+def test_first_call_inside_a_capture_is_refused():
+    from faith_amd import ops
+    q, k, v, _ = tensors([8], [8], 2, 2, 32, F32)
+    packing = ops.Packing([8])
+    graph = torch.cuda.CUDAGraph()
+    x = torch.zeros(4, device="cuda")
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            ops.attention(q, k, v, packing)
+
+
+def test_on_another_stream_with_other_work_in_flight():
+    from faith_amd import ops
+    lengths = [500, 90]
+    q, k, v, _ = tensors(lengths, lengths, 8, 2, 128, BF16, 5)
+    packing = ops.Packing(lengths)
+    want = ops.attention(q, k, v, packing, causal=True)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got += [ops.attention(q, k, v, packing, causal=True) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, x) for x in got)
+
+
+def test_workspace_keeps_results_of_every_type():
+    from faith_amd import ops
+    lengths = [40, 3000]
+    q, k, v, _ = tensors([1, 1], lengths, 8, 2, 128, F16, 5)
+    packing, ws = ops.Packing([1, 1], lengths), ops.Workspace()
+    want = ops.attention(q, k, v, packing)
+    for _ in range(3):
+        with ops.workspace(ws):
+            got = ops.attention(q, k, v, packing)
+            assert torch.equal(got, want)
+    n = ws.allocations
+    with ops.workspace(ws):
+        ops.attention(q, k, v, packing)
+    assert ws.allocations == n
+
+
+def test_refusals():
+    from faith_amd import _lib, ops
+    lengths = [6, 10]
+    q, k, v, dout = tensors(lengths, lengths, 4, 2, 32, BF16)
+    packing = ops.Packing(lengths)
+    call = lambda q=q, k=k, v=v, p=packing, **kw: ops.attention(q, k, v, p, **kw)
+    for bad, kind, what in [(dict(k=k.float()), TypeError, "k:"), (dict(q=q.double()), TypeError, "q:"), (dict(q=q[:15]), ValueError, "q: expected shape"),
+                            (dict(k=k[:, :, :16]), ValueError, "k: expected shape"), (dict(v=v[:, :1]), ValueError, "v: expected shape"),
+                            (dict(q=q[:, :3]), ValueError, "share"), (dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)), ValueError, "contiguous"),
+                            (dict(q=q[0]), ValueError, "q: expected shape"), (dict(k=k[:1].expand(16, 2, 32)), ValueError, "overlap"),
+                            (dict(scale=0.0), ValueError, "scale"), (dict(scale=math.inf), ValueError, "scale"), (dict(scale=-1.0), ValueError, "scale"),
+                            (dict(q=torch.zeros(16 * 128 + 1, device="cuda", dtype=BF16)[1:].view(16, 4, 32)), ValueError, "16 bytes")]:
+        with pytest.raises(kind, match=what):
+            call(**bad)
+    wide = torch.zeros(16, 2, 136, device="cuda", dtype=BF16)
+    with pytest.raises(ValueError, match="up to 128"):
+        call(q=wide, k=wide, v=wide)
+    with pytest.raises(ValueError, match="up to 128"):
+        call(q=wide[:, :, :20], k=wide[:, :, :20], v=wide[:, :, :20])
+    out, lse = ops.attention(q, k, v, packing, return_lse=True)
+    with pytest.raises(ValueError, match="lse"):
+        ops.attention_backward(dout, q, k, v, out, lse[:, :5], packing)
+    with pytest.raises(ValueError, match="dout"):
+        ops.attention_backward(dout[:, :2], q, k, v, out, lse, packing)
+    with pytest.raises(ValueError, match="out: expected"):
+        ops.attention(q, k, v, packing, out=out[:9])
+    assert issubclass(_lib.FaithError, RuntimeError)
+
+
+def test_empty_batches():
+    from faith_amd import ops
+    q, k, v, dout = tensors([0, 0], [5, 0], 2, 2, 32, F32)
+    packing = ops.Packing([0, 0], [5, 0])
+    out, lse = ops.attention(q, k, v, packing, return_lse=True)
+    assert out.shape == (0, 2, 32) and lse.shape == (2, 0)
+    dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing)
+    assert dq.shape == (0, 2, 32) and bool((dk == 0).all()) and bool((dv == 0).all())
