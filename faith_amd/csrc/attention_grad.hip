@@ -219,26 +219,34 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(co
         tok0 = tok0 + BQ >= it.end ? it.begin : tok0 + BQ;
         if (t0 + BQ - 1 < any_sees) return;
         const bool part = t0 < all_see;
+        // all scores of the tile first, so that the exponentials of one block of 32 queries can run beside the products of
+        // another: where heads have 128 elements a wavefront has its SIMD to itself
+        floatx16 s[BQ / 32], dp[BQ / 32];
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
-            floatx16 s = rows_by_column<T, DP>(qt, 32 * b + col, half, k);
-            floatx16 dp = rows_by_column<T, DP>(dt, 32 * b + col, half, v);
+            s[b] = rows_by_column<T, DP>(qt, 32 * b + col, half, k);
+            dp[b] = rows_by_column<T, DP>(dt, 32 * b + col, half, v);
+        }
+        if (part) {
+#pragma unroll
+            for (int b = 0; b < BQ / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t0 + 32 * b + row_of(r, half) < first) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
+        }
+#pragma unroll
+        for (int b = 0; b < BQ / 32; ++b) {
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const floatx4 l = *reinterpret_cast<const floatx4 *>(lt + 32 * b + row_of(r, half)), e = *reinterpret_cast<const floatx4 *>(et + 32 * b + row_of(r, half));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[r + i] = __builtin_amdgcn_exp2f(fmaf(s[r + i], g.c, -l[i]));
-                    dp[r + i] = s[r + i] * (dp[r + i] - e[i]);
+                    s[b][r + i] = __builtin_amdgcn_exp2f(fmaf(s[b][r + i], g.c, -l[i]));
+                    dp[b][r + i] = s[b][r + i] * (dp[b][r + i] - e[i]);
                 }
             }
-            if (part) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (t0 + 32 * b + row_of(r, half) < first) s[r] = dp[r] = 0.f;
-            }
-            columns_by_result<T, DP>(dv, dt, 32 * b, lane, s);
-            columns_by_result<T, DP>(dk, qt, 32 * b, lane, dp);
+            columns_by_result<T, DP>(dv, dt, 32 * b, lane, s[b]);
+            columns_by_result<T, DP>(dk, qt, 32 * b, lane, dp[b]);
         }
     };
     if (total > 0) {
@@ -272,7 +280,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(co
 }
 
 template <class T, int DP> int launch_backward(GradArgs g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
-    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP == 32 ? 64 : 32;
+    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 ? 64 : 32;
     unsigned grid;
     if (n_q > 0) {
         g.items = q_items;
