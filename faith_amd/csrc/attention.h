@@ -70,12 +70,20 @@ __device__ __forceinline__ bool dealt(const Deal &d, int *head, int *item) {
 
 // ------------------------------------------------------------------------------------------ a tile of rows in LDS
 // ROWS x DP elements, rows of RB bytes in chunks of 16 bytes; chunk c of row r stands at chunk c ^ swizzle(r).  Two reads
-// have to be free of bank conflicts (64 banks of 4 bytes): the same chunk of consecutive rows (16 bytes a lane), and 64
-// bytes of each of eight consecutive rows (the transposing read, 8 bytes a lane).
-template <class T, int DP> struct Tile {
+// have to be free of bank conflicts (64 banks of 4 bytes): the same chunk of 16 consecutive rows (ROWS: 16 bytes a lane, 16
+// lanes a clock), and 64 bytes of each of four (COLUMNS: the transposing read, 8 bytes a lane, 32 lanes a clock).  A tile that is
+// read by columns only has the simpler swizzle, which repeats sooner: fewer addresses to hold.
+enum Reads { COLUMNS, ROWS_TOO };
+template <class T, int DP, Reads READS = ROWS_TOO> struct Tile {
     static constexpr int RB = DP * (int)sizeof(T), CHUNKS = RB / 16, PER = 16 / (int)sizeof(T);
+    static constexpr int PERIOD = READS == ROWS_TOO ? 16 : sizeof(T) == 4 || CHUNKS == 4 ? 1 : 4;      // rows until the swizzle repeats
     __device__ static __forceinline__ int swizzle(int r) {
-        if constexpr (CHUNKS == 4) return (r >> 2) & 3;
+        if constexpr (READS == COLUMNS) {
+            if constexpr (PERIOD == 1) return 0;
+            else if constexpr (CHUNKS == 8) return ((r >> 1) & 1) << 2;
+            else return (r & 3) << 2;
+        }
+        else if constexpr (CHUNKS == 4) return (r >> 2) & 3;
         else if constexpr (CHUNKS == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
         else return ((r & 3) << 2) | ((r >> 2) & 3);
     }
@@ -95,10 +103,10 @@ __device__ __forceinline__ void groups_to_lds(__amdgpu_buffer_rsrc_t w, char *ds
 // The loads of one tile of ROWS rows by WAVES wavefronts: 1 KB an instruction, straight into LDS (lane i's 16 bytes land at
 // 16 i), so the swizzle is applied to the address that a lane reads.  Rows behind the sequence's last and chunks behind the
 // head's size lie outside the window and arrive as zeros.
-template <class T, int DP, int ROWS, int WAVES> struct Stager {
-    typedef Tile<T, DP> Tl;
+template <class T, int DP, int ROWS, int WAVES, Reads READS = ROWS_TOO> struct Stager {
+    typedef Tile<T, DP, READS> Tl;
     static constexpr int ROWS_PER = 1024 / Tl::RB, LOADS = ROWS * Tl::RB / 1024 / WAVES;
-    static constexpr int PERIOD = ROWS_PER < 16 ? 16 / ROWS_PER : 1, PATTERNS = LOADS < PERIOD ? LOADS : PERIOD;   // the swizzle repeats every 16 rows
+    static constexpr int PERIOD = ROWS_PER < Tl::PERIOD ? Tl::PERIOD / ROWS_PER : 1, PATTERNS = LOADS < PERIOD ? LOADS : PERIOD;
     static_assert(LOADS * WAVES * 1024 == ROWS * Tl::RB && LOADS % PATTERNS == 0, "the wavefronts share the tile evenly");
     unsigned off[PATTERNS];
     unsigned stride;             // bytes from one row to the next
@@ -138,10 +146,10 @@ template <int DP> __device__ __forceinline__ floatx4 row_fragment4(const float *
 }
 // first operand transposed: columns col0 ... col0 + 31 of the tile against the 16 rows row0 + {0 ... 15} in the order in which
 // registers 0 ... 7 hold them: lane half h has rows 4h ... 4h + 3, then 8 + 4h ... 8 + 4h + 3
-template <class T, int DP> __device__ __forceinline__ typename Vec<T>::x8 column_fragment(const T *tile, int row0, int col0, int lane) {
+template <class T, int DP, Reads READS> __device__ __forceinline__ typename Vec<T>::x8 column_fragment(const T *tile, int row0, int col0, int lane) {
     const int i = lane & 15, r = row0 + 4 * (lane >> 5) + (i >> 2), c = col0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-    const T *lo = tile + Tile<T, DP>::at(r, c >> 3) + (c & 7);
-    const T *hi = tile + Tile<T, DP>::at(r + 8, c >> 3) + (c & 7);
+    const T *lo = tile + Tile<T, DP, READS>::at(r, c >> 3) + (c & 7);
+    const T *hi = tile + Tile<T, DP, READS>::at(r + 8, c >> 3) + (c & 7);
     const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4 *)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4 *)hi);
     const shortx8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(typename Vec<T>::x8, v);
@@ -186,7 +194,7 @@ template <class T, int DP> __device__ __forceinline__ ColumnRegs<T, DP> column_r
 
 // acc[m][r] += sum over the tile's 32 rows from row0 on of tile[row][32 m + row_of(r)] * p[row]: p is a result register set of
 // this lane's column.  Products of 2-byte elements round p to that type (half a step of it, against sums in 32 bits).
-template <class T, int DP> __device__ __forceinline__ void columns_by_result(floatx16 (&acc)[DP / 32], const T *tile, int row0, int lane, const floatx16 &p) {
+template <class T, int DP, Reads READS = ROWS_TOO> __device__ __forceinline__ void columns_by_result(floatx16 (&acc)[DP / 32], const T *tile, int row0, int lane, const floatx16 &p) {
     if constexpr (sizeof(T) == 4) {
         const int half = lane >> 5, col = lane & 31;
 #pragma unroll
@@ -195,7 +203,7 @@ template <class T, int DP> __device__ __forceinline__ void columns_by_result(flo
 #pragma unroll
             for (int m = 0; m < DP / 32; ++m) {
                 const int c = 32 * m + col;
-                acc[m] = mfma(tile[Tile<T, DP>::at(row, c >> 2) + (c & 3)], p[r], acc[m]);
+                acc[m] = mfma(tile[Tile<T, DP, READS>::at(row, c >> 2) + (c & 3)], p[r], acc[m]);
             }
         }
     } else {
@@ -205,7 +213,7 @@ template <class T, int DP> __device__ __forceinline__ void columns_by_result(flo
 #pragma unroll
             for (int e = 0; e < 8; ++e) b[e] = (T)p[8 * u + e];
 #pragma unroll
-            for (int m = 0; m < DP / 32; ++m) acc[m] = mfma(column_fragment<T, DP>(tile, row0 + 16 * u, 32 * m, lane), b, acc[m]);
+            for (int m = 0; m < DP / 32; ++m) acc[m] = mfma(column_fragment<T, DP, READS>(tile, row0 + 16 * u, 32 * m, lane), b, acc[m]);
         }
     }
 }

@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) atte
 }
 
 template <class T, int DP, int BQ>
-__global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(const GradArgs g) {
+__global__ void __launch_bounds__(256, 2) attention_grad_keys(const GradArgs g) {
     constexpr int TILE = BQ * DP;
     typedef Stager<T, DP, BQ, 4> St;
     __shared__ T q0[TILE], d0[TILE], q1[TILE], d1[TILE];
@@ -186,7 +186,18 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(co
     const int half = lane >> 5, col = lane & 31;
     const int key_lo = it.row0 + wave * 32, key = key_lo + col, mine = key < it.k_len ? key : it.k_len - 1;
     const T *krow = at<T>(g.k, it.k_start + mine, g.k_ts, hk, g.k_hs), *vrow = at<T>(g.v, it.k_start + mine, g.v_ts, hk, g.v_hs);
-    const ColumnRegs<T, DP> k = column_regs<T, DP>(krow, half, g.size), v = column_regs<T, DP>(vrow, half, g.size);
+    const ColumnRegs<T, DP> k = column_regs<T, DP>(krow, half, g.size);
+    // The values' rows stay in LDS where registers for them would halve the wavefronts on a SIMD
+    constexpr bool V_IN_LDS = sizeof(T) == 2 && DP == 128;
+    __shared__ T v_rows[V_IN_LDS ? 128 * DP : 1];
+    ColumnRegs<T, DP> v;
+    if constexpr (V_IN_LDS) {
+        Stager<T, DP, 128, 4> vs;
+        vs.init(lane, wave, g.size, g.v_ts);
+        vs.load(v_rows, at<T>(g.v, it.k_start + it.row0, g.v_ts, hk, g.v_hs), it.k_len - it.row0, g.size, wave);
+    } else {
+        v = column_regs<T, DP>(vrow, half, g.size);
+    }
     const int shift = it.k_len - it.q_len;
     // the first token that sees this lane's key, all of the wavefront's, any of them
     const int first = g.causal ? mine - shift : -1, all_see = g.causal ? key_lo + 31 - shift : -1, any_sees = key_lo >= it.k_len ? 0x7fffffff : g.causal ? key_lo - shift : -1;
@@ -218,6 +229,9 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(co
         const int t0 = tok0;
         tok0 = tok0 + BQ >= it.end ? it.begin : tok0 + BQ;
         if (t0 + BQ - 1 < any_sees) return;
+        int lane = (int)threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int half = lane >> 5, col = lane & 31;
         const bool part = t0 < all_see;
         // all scores of the tile first, so that the exponentials of one block of 32 queries can run beside the products of
         // another: where heads have 128 elements a wavefront has its SIMD to itself
@@ -225,6 +239,10 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(co
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
             s[b] = rows_by_column<T, DP>(qt, 32 * b + col, half, k);
+            if constexpr (V_IN_LDS) {
+#pragma unroll
+                for (int u = 0; u < DP / 16; ++u) v.v[u] = row_fragment<T, DP>(v_rows, wave * 32 + col, u, half);
+            }
             dp[b] = rows_by_column<T, DP>(dt, 32 * b + col, half, v);
         }
         if (part) {
@@ -280,7 +298,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) attention_grad_keys(co
 }
 
 template <class T, int DP> int launch_backward(GradArgs g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
-    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 ? 64 : 32;
+    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP < 128 ? 64 : 32;
     unsigned grid;
     if (n_q > 0) {
         g.items = q_items;
