@@ -3,7 +3,7 @@
 //     c = h - mean(h)  (root mean square: c = h),   z = c / sqrt(mean(c^2) + eps)  (without the variance: z = c),   y = w z + b
 // and the gradients.  Everything is bound by HBM: forward 4 n elements a row (x, residual in; h, y out), backward 4 n (dy, h,
 // dsum in; dx out).  A row is read once and stays in registers between the statistics and the result: a wavefront to a row
-// up to 64 lanes' worth of 16-byte groups twice over, a workgroup of four beyond that; rows that do not fall into 16-byte
+// up to 128 groups of 16 bytes, four or eight wavefronts beyond that; rows that do not fall into 16-byte
 // groups, and rows wider than the registers hold, take a kernel that goes over the row again (it comes from the L2).
 // Statistics are sums in 32 bits over at most a few dozen values a lane and a tree above; the variance is that of the
 // centred values, so nothing cancels.
@@ -84,13 +84,15 @@ __device__ __forceinline__ unsigned to_e4m3(float a, float b, float c, float d) 
 }
 __device__ __forceinline__ float steps_of(int bits) { return bits == FAITH_BITS_INT8 ? 127.f : 448.f; }
 
-// WAVES wavefronts to a row (4 / WAVES rows to a workgroup), CH groups of 16 bytes to a lane
+// WAVES wavefronts to a row (a workgroup of four such rows, where one is enough), CH groups of 16 bytes to a lane
+constexpr int rows_of(int waves) { return waves == 1 ? 4 : 1; }
+constexpr int threads_of(int waves) { return 64 * waves * rows_of(waves); }
 template <class T, int WAVES, int CH>
-__global__ void __launch_bounds__(256) residual_norm(const NormArgs g) {
+__global__ void __launch_bounds__(threads_of(WAVES)) residual_norm(const NormArgs g) {
     constexpr int N = Group<T>::N, LANES = 64 * WAVES;
-    __shared__ float slot[3][4];
+    __shared__ float slot[3][WAVES];
     const int wave = threadIdx.x >> 6, t = (int)threadIdx.x % LANES;
-    const long long row = (long long)blockIdx.x * (4 / WAVES) + wave / WAVES;
+    const long long row = (long long)blockIdx.x * rows_of(WAVES) + wave / WAVES;
     if (WAVES < 4 && row >= g.rows) return;                   // a whole wavefront; no barrier follows in this shape
     const long long at = row * g.n;
     const T *x = reinterpret_cast<const T *>(g.x) + at, *res = g.residual ? reinterpret_cast<const T *>(g.residual) + at : nullptr;
@@ -242,33 +244,56 @@ struct NormGradArgs {
 // over its spread.  A workgroup goes over rows
 // blockIdx.x, + gridDim.x, ...; its columns' sums of dy z and dy stay in registers until the end and go to a row of
 // `partial` of its own, which a second launch adds up in a fixed order: no atomics, the same bits every time.
-template <class T, int WAVES, int CH>
-__global__ void __launch_bounds__(256) residual_norm_grad(const NormGradArgs g) {
+//
+// The next row is on its way while this one is worked on: without that a row's loads wait for the sums of the row before
+// (8191 rows of 5120 bf16: 114 -> 84 us, 4.0 TB/s; sixteen wavefronts to a row instead
+// of four take 95).
+template <class T, int WAVES, int CH, bool BIAS>
+__global__ void __launch_bounds__(threads_of(WAVES)) residual_norm_grad(const NormGradArgs g) {
     constexpr int N = Group<T>::N, LANES = 64 * WAVES;
-    __shared__ float slot[2][2][4], mean_slot[2][4];
+    typedef typename Packed<T>::type Raw;
+    __shared__ float slot[2][2][WAVES], mean_slot[2][WAVES];
     const int wave = threadIdx.x >> 6, t = (int)threadIdx.x % LANES;
     const float inv_n = 1.f / (float)g.n;
-    float dw[CH][N], db[CH][N];
+    float dw[CH][N], db[BIAS ? CH : 1][N];
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int e = 0; e < N; ++e) dw[c][e] = db[c][e] = 0.f;
-    int parity = 0;
-    const long long step = (long long)gridDim.x * (4 / WAVES);
-    for (long long row = (long long)blockIdx.x * (4 / WAVES) + wave / WAVES; row < g.rows; row += step, parity ^= 1) {
+        for (int e = 0; e < N; ++e) { dw[c][e] = 0.f; if (BIAS) db[c][e] = 0.f; }
+    Raw raw_d[CH], raw_h[CH], raw_s[CH];
+    float raw_r = 1.f;
+    auto fetch = [&](long long row) {
         const long long at = row * g.n;
-        const T *dy = reinterpret_cast<const T *>(g.dy) + at, *hh = reinterpret_cast<const T *>(g.h) + at;
-        const float r = g.kind == NO_VAR ? 1.f : g.stats[row];
-        float z[CH][N], d[CH][N];
-        float s0 = 0.f, s1 = 0.f, mean = 0.f;
+        if (g.kind != NO_VAR) raw_r = g.stats[row];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int e0 = (c * LANES + t) * N;
-            if (e0 < g.n) { unpack(dy + e0, d[c]); unpack(hh + e0, z[c]); }
-            else
-#pragma unroll
-                for (int e = 0; e < N; ++e) d[c][e] = z[c][e] = 0.f;
+            if (e0 >= g.n) continue;
+            raw_d[c] = *reinterpret_cast<const Raw *>(reinterpret_cast<const T *>(g.dy) + at + e0);
+            raw_h[c] = *reinterpret_cast<const Raw *>(reinterpret_cast<const T *>(g.h) + at + e0);
+            if (g.dsum) raw_s[c] = *reinterpret_cast<const Raw *>(reinterpret_cast<const T *>(g.dsum) + at + e0);
         }
+    };
+    int parity = 0;
+    const long long step = (long long)gridDim.x * rows_of(WAVES);
+    long long row = (long long)blockIdx.x * rows_of(WAVES) + wave / WAVES;
+    if (row < g.rows) fetch(row);
+    for (; row < g.rows; row += step, parity ^= 1) {
+        const float r = raw_r;
+        float z[CH][N], d[CH][N];
+        Raw s[CH];
+        float s0 = 0.f, s1 = 0.f, mean = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const bool in = (c * LANES + t) * N < g.n;
+            s[c] = raw_s[c];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                d[c][e] = in ? (float)raw_d[c][e] : 0.f;
+                z[c][e] = in ? (float)raw_h[c][e] : 0.f;
+            }
+        }
+        if (row + step < g.rows) fetch(row + step);
         if (g.kind != RMS) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
@@ -285,7 +310,7 @@ __global__ void __launch_bounds__(256) residual_norm_grad(const NormGradArgs g) 
             for (int e = 0; e < N; ++e) {
                 z[c][e] = e0 < g.n ? (z[c][e] - mean) * r : 0.f;
                 dw[c][e] = fmaf(d[c][e], z[c][e], dw[c][e]);
-                db[c][e] += d[c][e];
+                if (BIAS) db[c][e] += d[c][e];
                 if (g.weight && e0 < g.n) d[c][e] *= w[e];
                 s0 += d[c][e];
                 s1 = fmaf(d[c][e], z[c][e], s1);
@@ -312,27 +337,25 @@ __global__ void __launch_bounds__(256) residual_norm_grad(const NormGradArgs g) 
             const int e0 = (c * LANES + t) * N;
             if (e0 >= g.n) continue;
             float v[N];
-            if (g.dsum) unpack(reinterpret_cast<const T *>(g.dsum) + at + e0, v);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const float dh = (d[c][e] - m0 - z[c][e] * m1) * r;
-                v[e] = g.dsum ? v[e] + dh : dh;
+                v[e] = g.dsum ? (float)s[c][e] + dh : dh;
             }
-            pack(reinterpret_cast<T *>(g.dx) + at + e0, v);
+            pack(reinterpret_cast<T *>(g.dx) + row * g.n + e0, v);
         }
     }
     if (!g.partial) return;
     // rows of `partial`: one to a wavefront group
-    float *p = g.partial + ((long long)blockIdx.x * (4 / WAVES) + wave / WAVES) * 2 * g.n;
+    float *p = g.partial + ((long long)blockIdx.x * rows_of(WAVES) + wave / WAVES) * 2 * g.n;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e0 = (c * LANES + t) * N;
         if (e0 >= g.n) continue;
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
-            const floatx4 a = {dw[c][e], dw[c][e + 1], dw[c][e + 2], dw[c][e + 3]}, b = {db[c][e], db[c][e + 1], db[c][e + 2], db[c][e + 3]};
-            if (g.dweight) *reinterpret_cast<floatx4 *>(p + e0 + e) = a;
-            if (g.dbias) *reinterpret_cast<floatx4 *>(p + g.n + e0 + e) = b;
+            if (g.dweight) *reinterpret_cast<floatx4 *>(p + e0 + e) = floatx4{dw[c][e], dw[c][e + 1], dw[c][e + 2], dw[c][e + 3]};
+            if constexpr (BIAS) *reinterpret_cast<floatx4 *>(p + g.n + e0 + e) = floatx4{db[c][e], db[c][e + 1], db[c][e + 2], db[c][e + 3]};
         }
     }
 }
@@ -408,25 +431,28 @@ Shape shape_of(int n, int dtype, bool aligned16) {
     if (groups <= 256) return {4, 1};
     if (groups <= 512) return {4, 2};
     if (groups <= 768) return {4, 3};
-    if (groups <= 1024) return {4, 4};
-    if (groups <= 2048) return {4, 8};
+    if (groups <= 1024) return {8, 2};
+    if (groups <= 2048) return {8, 4};
     return {0, 0};
 }
 
-#define FAITH_BY_SHAPE(KERNEL, GRID, ARGS)                                                                             \
-    do {                                                                                                               \
-        if (s.waves == 1 && s.groups == 1) hipLaunchKernelGGL((KERNEL<T, 1, 1>), GRID, dim3(256), 0, stream, ARGS);      \
-        else if (s.waves == 1) hipLaunchKernelGGL((KERNEL<T, 1, 2>), GRID, dim3(256), 0, stream, ARGS);                  \
-        else if (s.groups == 1) hipLaunchKernelGGL((KERNEL<T, 4, 1>), GRID, dim3(256), 0, stream, ARGS);                 \
-        else if (s.groups == 2) hipLaunchKernelGGL((KERNEL<T, 4, 2>), GRID, dim3(256), 0, stream, ARGS);                 \
-        else if (s.groups == 3) hipLaunchKernelGGL((KERNEL<T, 4, 3>), GRID, dim3(256), 0, stream, ARGS);                 \
-        else if (s.groups == 4) hipLaunchKernelGGL((KERNEL<T, 4, 4>), GRID, dim3(256), 0, stream, ARGS);                 \
-        else hipLaunchKernelGGL((KERNEL<T, 4, 8>), GRID, dim3(256), 0, stream, ARGS);                                    \
+#define FAITH_LAUNCH_SHAPE(KERNEL, WAVES, CH, GRID, ARGS, ...) \
+    hipLaunchKernelGGL((KERNEL<T, WAVES, CH __VA_ARGS__>), GRID, dim3(threads_of(WAVES)), 0, stream, ARGS)
+#define FAITH_BY_SHAPE(KERNEL, GRID, ARGS, ...)                                                              \
+    do {                                                                                                     \
+        if (s.waves == 1 && s.groups == 1) FAITH_LAUNCH_SHAPE(KERNEL, 1, 1, GRID, ARGS, __VA_ARGS__);          \
+        else if (s.waves == 1) FAITH_LAUNCH_SHAPE(KERNEL, 1, 2, GRID, ARGS, __VA_ARGS__);                      \
+        else if (s.waves == 4 && s.groups == 1) FAITH_LAUNCH_SHAPE(KERNEL, 4, 1, GRID, ARGS, __VA_ARGS__);     \
+        else if (s.waves == 4 && s.groups == 2) FAITH_LAUNCH_SHAPE(KERNEL, 4, 2, GRID, ARGS, __VA_ARGS__);     \
+        else if (s.waves == 4) FAITH_LAUNCH_SHAPE(KERNEL, 4, 3, GRID, ARGS, __VA_ARGS__);                      \
+        else if (s.groups == 2) FAITH_LAUNCH_SHAPE(KERNEL, 8, 2, GRID, ARGS, __VA_ARGS__);                     \
+        else FAITH_LAUNCH_SHAPE(KERNEL, 8, 4, GRID, ARGS, __VA_ARGS__);                                        \
     } while (0)
+#define FAITH_COMMA ,
 
 template <class T> int launch_norm(const NormArgs &g, const Shape &s, hipStream_t stream) {
     if (s.waves == 0) hipLaunchKernelGGL((residual_norm_any<T>), dim3((unsigned)g.rows), dim3(256), 0, stream, g);
-    else FAITH_BY_SHAPE(residual_norm, dim3((unsigned)((g.rows + 4 / s.waves - 1) / (4 / s.waves))), g);
+    else FAITH_BY_SHAPE(residual_norm, dim3((unsigned)((g.rows + rows_of(s.waves) - 1) / rows_of(s.waves))), g, );
     return check_launch("faith_residual_norm");
 }
 
@@ -436,7 +462,9 @@ template <class T> int launch_grad(const NormGradArgs &g, const Shape &s, hipStr
             hipLaunchKernelGGL((residual_norm_grad_any<T>), dim3((unsigned)g.rows), dim3(256), 0, stream, g);
             if (g.partial) hipLaunchKernelGGL((residual_norm_columns_any<T>), dim3((unsigned)ceil_div(g.n, 256), (unsigned)g.blocks), dim3(256), 0, stream, g);
         } else {
-            FAITH_BY_SHAPE(residual_norm_grad, dim3((unsigned)(g.blocks / (4 / s.waves))), g);
+            const dim3 grid((unsigned)(g.blocks / rows_of(s.waves)));
+            if (g.dbias) FAITH_BY_SHAPE(residual_norm_grad, grid, g, FAITH_COMMA true);
+            else FAITH_BY_SHAPE(residual_norm_grad, grid, g, FAITH_COMMA false);
         }
     }
     if (g.dweight || g.dbias)

@@ -173,7 +173,7 @@ class _Tuned:
 def _on(device, op=None, shape=None):
     """Device guard for the launch; free when the tensor already lives on the current device.
     With a tuning table in use (autotune.use) the entry for (op, shape) is applied around the launch."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == torch._C._cuda_getDevice():
         guard = _NO_GUARD
     else:
         guard = torch.cuda.device(device)
@@ -1148,8 +1148,11 @@ class Packing:
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError(f"device: the work items live on the GPU (got {device}); there is no CPU path")
+        if device.index is None and torch.cuda.is_available():
+            device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
         self._plans = {}
+        self._calls = {}         # what does not depend on the operands' addresses, by their shapes and types
 
     @staticmethod
     def _checked(name, lengths):
@@ -1176,11 +1179,13 @@ class Packing:
         found = self._plans.get(key)
         if found is None:
             found = self._plans[key] = self._make(which, heads, kv_heads, element_size, bool(causal))
-        stream = _stream(found[0])
-        if stream != found[6]:
-            # used on another stream than the one it was allocated on: its memory is not handed out again before this is done
-            found[0].record_stream(torch.cuda.current_stream(self.device))
+        self._used_on(found, _stream(found[0]))
         return found
+
+    def _used_on(self, plan, stream):
+        if stream != plan[6]:
+            # another stream than the one it was allocated on: its memory is not handed out again before this use is done
+            plan[0].record_stream(torch.cuda.current_stream(self.device))
 
     def _make(self, which, heads, kv_heads, element_size, causal):
         import ctypes
@@ -1237,9 +1242,27 @@ def _attention_operands(q, k, v, packing):
         raise ValueError(f"{heads} heads do not share {kv_heads} key heads evenly")
     if size > 128 or size == 0 or size % (16 // q.element_size()):
         raise ValueError(f"heads of {size} elements: up to 128 in whole groups of 16 bytes")
-    if q.device.index != (torch.cuda.current_device() if packing.device.index is None else packing.device.index):
+    if q.device != packing.device:
         raise ValueError(f"q lives on {q.device}, the packing on {packing.device}")
     return heads, kv_heads, size, qs, ks, vs
+
+
+def _known_call(packing, which, causal, scale, q, k, v, *more):
+    """The arguments of an earlier call with operands of these shapes and types, all contiguous, on the packing's device and
+    on 16 bytes: (key, what was kept or None).  A small call is bound by its host side, and most of that is checks whose
+    outcome depends on nothing else; whatever this does not recognise takes the long way."""
+    try:
+        index, dtype, address = packing.device.index, q.dtype, 0
+        for t in (q, k, v, *more):
+            if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+                return None, None
+            address |= t.data_ptr()
+        if address & 15:
+            return None, None
+        key = (which, causal, scale, dtype, q.shape, k.shape, v.shape)
+        return key, packing._calls.get(key)
+    except (AttributeError, TypeError):
+        return None, None
 
 
 def _scale(scale, size):
@@ -1253,7 +1276,7 @@ def _scale(scale, size):
 
 def _like_rows(t, rows):
     """A contiguous result of t's shape; the places behind the packing's last row hold zeros."""
-    out = _empty(*t.shape, device=t.device, dtype=t.dtype)
+    out = _empty_like(t) if t.is_contiguous() else _empty(*t.shape, device=t.device, dtype=t.dtype)
     if t.shape[0] > rows:
         out[rows:].zero_()
     return out
@@ -1267,20 +1290,32 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
     (and, with return_lse, the logarithm of every row's sum of exponentials, float32 [heads, tokens], which
     attention_backward takes).  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, and
     their places in an `out` that the caller brings not written."""
-    heads, kv_heads, size, (qt, qh), (kt, kh), (vt, vh) = _attention_operands(q, k, v, packing)
-    scale = _scale(scale, size)
-    dev = q.device
+    key, known = _known_call(packing, 0, causal, scale, q, k, v) if out is None else (None, None)
+    dev = packing.device if known is not None else None
+    if known is None:
+        heads, kv_heads, size, (qt, qh), (kt, kh), (vt, vh) = _attention_operands(q, k, v, packing)
+        dev = q.device
+        with _on(dev):
+            plan = packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), causal)
+        _, items, n, joins, parts, kind, _ = plan
+        floats = parts * kv_heads * (32 if kind else 128) * ((32 if size <= 32 else 64 if size <= 64 else 128) + 4)
+        if out is None:
+            ot, oh = heads * size, size
+        else:
+            ot, oh = _rows("out", out, packing.tokens, heads, size, q)
+        known = (plan, floats, heads, (items, n, joins, kind, qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size,
+                                       _DTYPES[q.dtype], int(causal), _scale(scale, size)))
+        if key is not None:
+            packing._calls[key] = known
+    plan, floats, heads, rest = known
     if out is None:
         out = _like_rows(q, packing.tokens)
-    ot, oh = _rows("out", out, packing.tokens, heads, size, q)
     lse = _empty(heads, packing.tokens, device=dev) if return_lse else None
+    scratch = _empty(floats, device=dev) if floats else None
+    stream = _stream(q)
+    packing._used_on(plan, stream)
     with _on(dev):
-        _, items, n, joins, parts, kind, _ = packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), causal)
-        scratch = None
-        if parts:
-            scratch = _empty(parts * kv_heads * (32 if kind else 128) * ((32 if size <= 32 else 64 if size <= 64 else 128) + 4), device=dev)
-        _lib.call("faith_attention", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(scratch), items, n, joins, kind,
-                  qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size, _DTYPES[q.dtype], int(causal), scale, _stream(q))
+        _lib.call("faith_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(scratch), *rest, stream)
     return (out, lse) if return_lse else out
 
 
@@ -1288,29 +1323,45 @@ def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=Non
     """Gradients of attention(): (dq, dk, dv), each of its operand's shape and type, from dout, the gradient of its result.
     out, lse: what the forward call returned (return_lse=True); the other arguments as in that call.  Sums in float32;
     the gradients of a key head add up those of the heads that share it.  The same bits on every call."""
-    import ctypes
-    heads, kv_heads, size, qs, ks, vs = _attention_operands(q, k, v, packing)
-    scale = _scale(scale, size)
-    dev = q.device
-    ds = _rows("dout", dout, packing.tokens, heads, size, q)
-    os_ = _rows("out", out, packing.tokens, heads, size, q)
+    key, known = _known_call(packing, 1, causal, scale, q, k, v, dout, out)
+    if known is None or dout.shape != q.shape or out.shape != q.shape:
+        import ctypes
+        heads, kv_heads, size, qs, ks, vs = _attention_operands(q, k, v, packing)
+        ds = _rows("dout", dout, packing.tokens, heads, size, q)
+        os_ = _rows("out", out, packing.tokens, heads, size, q)
+        row, kv_row = (heads * size, size), (kv_heads * size, size)
+        strides = (ctypes.c_longlong * 16)(*ds, *qs, *ks, *vs, *os_, *row, *kv_row, *kv_row)
+        with _on(q.device):
+            plans = [packing.plan(which, heads, kv_heads, q.element_size(), causal) for which in (_lib.ATTENTION_GRAD_QUERIES, _lib.ATTENTION_GRAD_KEYS)]
+        known = (plans, heads, (plans[0][1], plans[0][2], plans[1][1], plans[1][2], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
+                                size, _DTYPES[q.dtype], int(causal), _scale(scale, size)), strides)
+        if key is not None and dout.shape == q.shape and out.shape == q.shape:
+            packing._calls[key] = known
+    plans, heads, rest, _ = known
     _check("lse", lse, (heads, packing.tokens))
+    dev = packing.device
+    if lse.get_device() != dev.index:
+        raise ValueError(f"lse: lives on {lse.device}, the other operands on {dev}")
     dq, dk, dv = _like_rows(q, packing.tokens), _like_rows(k, packing.keys), _like_rows(v, packing.keys)
-    row, kv_row = (heads * size, size), (kv_heads * size, size)
-    strides = (ctypes.c_longlong * 16)(*ds, *qs, *ks, *vs, *os_, *row, *kv_row, *kv_row)
+    stat = _empty(2, heads, packing.tokens, device=dev)
+    stream = _stream(q)
+    packing._used_on(plans[0], stream)
+    packing._used_on(plans[1], stream)
     with _on(dev):
-        es = q.element_size()
-        q_plan = packing.plan(_lib.ATTENTION_GRAD_QUERIES, heads, kv_heads, es, causal)
-        k_plan = packing.plan(_lib.ATTENTION_GRAD_KEYS, heads, kv_heads, es, causal)
-        stat = _empty(2, heads, packing.tokens, device=dev)
-        _lib.call("faith_attention_backward", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
-                  _ptr(stat), q_plan[1], q_plan[2], k_plan[1], k_plan[2], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
-                  size, _DTYPES[q.dtype], int(causal), scale, _stream(q))
+        _lib.call("faith_attention_backward", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stat.data_ptr(), *rest, stream)
     return dq, dk, dv
 
 
 def _row_tensor(name, t, like=None, shape=None, dtype=None):
     """A contiguous GPU tensor of one of the concrete pass's types."""
+    # one expression for the tensor that is fine, as in _check
+    try:
+        if t.is_contiguous() and t.dtype in _DTYPES and t.is_cuda and (like is None or (t.dtype is (dtype or like.dtype) and t.get_device() == like.get_device())) \
+                and (shape is None or t.shape == shape):
+            return t
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
     if not t.is_cuda or (like is not None and t.device != like.device):
@@ -1334,10 +1385,28 @@ def _norm_operands(x, others, vectors, kind):
             _row_tensor(name, t, x, x.shape)
     for name, t in vectors:
         if t is not None:
-            _row_tensor(name, t, x, (x.shape[-1],))
+            _row_tensor(name, t, x, x.shape[-1:])
     if kind not in _lib.NORM_KINDS:
         raise ValueError(f"unknown kind {kind!r}: one of {', '.join(_lib.NORM_KINDS)}")
-    return x.numel() // x.shape[-1], x.shape[-1], _lib.NORM_KINDS[kind]
+
+
+def _alike(x, rows, vectors):
+    """Whether every tensor given is contiguous and on the GPU of x, of x's type, and of its shape or of that of its last
+    axis: one pass over the operands that are fine, in front of the checks that name what is not."""
+    try:
+        shape, dtype, index = x.shape, x.dtype, x.get_device()
+        if index < 0 or dtype not in _DTYPES or not x.is_contiguous() or not shape or not shape[-1]:
+            return False
+        for t in rows:
+            if t is not None and (t.shape != shape or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous()):
+                return False
+        n = (shape[-1],)
+        for t in vectors:
+            if t is not None and (t.shape != n or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous()):
+                return False
+        return True
+    except AttributeError:
+        return False
 
 
 _BITS = {"int8": (_lib.BITS_INT8, torch.int8), "e4m3": (_lib.BITS_E4M3, torch.float8_e4m3fn)}
@@ -1352,7 +1421,10 @@ def residual_norm(x, residual=None, weight=None, bias=None, kind="rms", eps=1e-6
     float32, bfloat16 or float16, contiguous; weight and bias of x's type.  Returns (y, h); h is x itself without a residual.
     quantize "int8" / "e4m3": returns (q, scales, h), 8-bit values with a float32 scale for every row, y ~ q * scale,
     scale = max |y| / 127 or / 448.  return_stats: one more result, what residual_norm_backward takes as `stats`."""
-    rows, n, code = _norm_operands(x, (("residual", residual),), (("weight", weight), ("bias", bias)), kind)
+    if kind not in _lib.NORM_KINDS or not _alike(x, (residual,), (weight, bias)):
+        _norm_operands(x, (("residual", residual),), (("weight", weight), ("bias", bias)), kind)
+    n = x.shape[-1]
+    rows, code = x.numel() // n, _lib.NORM_KINDS[kind]
     eps = float(eps)
     if not 0 <= eps < 1e30:
         raise ValueError(f"eps={eps}: must be finite and not negative")
@@ -1378,7 +1450,11 @@ def residual_norm_backward(dy, h, weight, stats, kind="rms", dsum=None, with_wei
     """Gradients of residual_norm: dy of y, dsum of h (what reaches it past the normalisation, or None); h, stats as the
     forward call returned them.  Returns (dx, dweight, dbias): dx is the gradient of x and of the residual alike, dweight and
     dbias are None where they are not wanted.  The same bits on every call."""
-    rows, n, code = _norm_operands(h, (("dy", dy), ("dsum", dsum)), (("weight", weight),), kind)
+    if dy is None or kind not in _lib.NORM_KINDS or not _alike(h, (dy, dsum), (weight,)):
+        _row_tensor("dy", dy)
+        _norm_operands(h, (("dy", dy), ("dsum", dsum)), (("weight", weight),), kind)
+    n = h.shape[-1]
+    rows, code = h.numel() // n, _lib.NORM_KINDS[kind]
     _row_tensor("stats", stats, h, h.shape[:-1], torch.float32)
     dev = h.device
     dx = _empty_like(h)
