@@ -76,14 +76,16 @@ __device__ __forceinline__ bool dealt(const Deal &d, int *head, int *item) {
 enum Reads { COLUMNS, ROWS_TOO };
 template <class T, int DP, Reads READS = ROWS_TOO> struct Tile {
     static constexpr int RB = DP * (int)sizeof(T), CHUNKS = RB / 16, PER = 16 / (int)sizeof(T);
-    static constexpr int PERIOD = READS == ROWS_TOO ? 16 : sizeof(T) == 4 || CHUNKS == 4 ? 1 : 4;      // rows until the swizzle repeats
+    // rows until the swizzle repeats; rows of 12 chunks start at another quarter of the banks each by themselves
+    static constexpr int PERIOD = READS == ROWS_TOO ? 16 : sizeof(T) == 4 || CHUNKS == 4 || CHUNKS == 12 ? 1 : 4;
     __device__ static __forceinline__ int swizzle(int r) {
         if constexpr (READS == COLUMNS) {
             if constexpr (PERIOD == 1) return 0;
             else if constexpr (CHUNKS == 8) return ((r >> 1) & 1) << 2;
             else return (r & 3) << 2;
         }
-        else if constexpr (CHUNKS == 4) return (r >> 2) & 3;
+        else if constexpr (CHUNKS == 4 || CHUNKS == 12) return (r >> 2) & 3;
+        else if constexpr (CHUNKS == 24) return (r >> 1) & 7;
         else if constexpr (CHUNKS == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
         else return ((r & 3) << 2) | ((r >> 2) & 3);
     }
@@ -105,9 +107,11 @@ __device__ __forceinline__ void groups_to_lds(__amdgpu_buffer_rsrc_t w, char *ds
 // head's size lie outside the window and arrive as zeros.
 template <class T, int DP, int ROWS, int WAVES, Reads READS = ROWS_TOO> struct Stager {
     typedef Tile<T, DP, READS> Tl;
-    static constexpr int ROWS_PER = 1024 / Tl::RB, LOADS = ROWS * Tl::RB / 1024 / WAVES;
-    static constexpr int PERIOD = ROWS_PER < Tl::PERIOD ? Tl::PERIOD / ROWS_PER : 1, PATTERNS = LOADS < PERIOD ? LOADS : PERIOD;
-    static_assert(LOADS * WAVES * 1024 == ROWS * Tl::RB && LOADS % PATTERNS == 0, "the wavefronts share the tile evenly");
+    static constexpr int TOTAL = ROWS * Tl::RB / 1024, LOADS = (TOTAL + WAVES - 1) / WAVES;
+    // Where whole rows make up a load and the swizzle has repeated, a later load's offsets are an earlier one's further on.
+    static constexpr int ROWS_PER = 1024 / Tl::RB, PERIOD = ROWS_PER < Tl::PERIOD ? Tl::PERIOD / ROWS_PER : 1;
+    static constexpr int PATTERNS = 1024 % Tl::RB == 0 && PERIOD < LOADS ? PERIOD : LOADS;
+    static_assert(TOTAL * 1024 == ROWS * Tl::RB && LOADS % PATTERNS == 0, "whole loads");
     unsigned off[PATTERNS];
     unsigned stride;             // bytes from one row to the next
 
@@ -115,8 +119,7 @@ template <class T, int DP, int ROWS, int WAVES, Reads READS = ROWS_TOO> struct S
         stride = (unsigned)(row_stride * (long long)sizeof(T));
 #pragma unroll
         for (int i = 0; i < PATTERNS; ++i) {
-            const int r = (wave * LOADS + i) * ROWS_PER + lane / Tl::CHUNKS;
-            const int c = (lane % Tl::CHUNKS) ^ Tl::swizzle(r);
+            const int x = (wave * LOADS + i) * 64 + lane, r = x / Tl::CHUNKS, c = (x % Tl::CHUNKS) ^ Tl::swizzle(r);
             off[i] = c * Tl::PER < size ? (unsigned)r * stride + (unsigned)c * 16u : 0x7ffffff0u;
         }
     }
@@ -127,8 +130,10 @@ template <class T, int DP, int ROWS, int WAVES, Reads READS = ROWS_TOO> struct S
         const __amdgpu_buffer_rsrc_t w = window(base, (unsigned)n);
         char *dst = reinterpret_cast<char *>(lds) + wave * LOADS * 1024;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
+        for (int i = 0; i < LOADS; ++i) {
+            if (TOTAL % WAVES && wave * LOADS + i >= TOTAL) break;
             groups_to_lds(w, dst + i * 1024, off[i % PATTERNS], (unsigned)((i / PATTERNS) * PATTERNS * ROWS_PER) * stride);
+        }
     }
 };
 

@@ -73,7 +73,7 @@ __device__ void one_row(const FwdArgs &g, const Item &it, int hk, const T *qrow,
 template <class T, int DP> constexpr int key_waves() { return 32 * DP * (int)sizeof(T) * 16 <= 128 * 1024 ? 4 : 2; }
 
 template <class T, int DP, int BN, bool KEYS, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, KEYS && DP * sizeof(T) >= 256 ? 1 : 2) attention_forward(const FwdArgs g) {
+__global__ void __launch_bounds__(64 * WAVES, KEYS && DP * sizeof(T) >= 192 ? 1 : 2) attention_forward(const FwdArgs g) {
     constexpr int TILE = BN * DP;
     typedef Stager<T, DP, BN, KEYS ? 1 : 4> St;                     // keys: read by rows
     typedef Stager<T, DP, BN, KEYS ? 1 : 4, COLUMNS> Sv;            // values: by columns only
@@ -389,6 +389,7 @@ template <class T, int DP> int launch_forward(const FwdArgs &g, int kind, unsign
 template <class T> int launch_forward(const FwdArgs &g, int kind, unsigned grid, const Item *joins, int n_joins, hipStream_t stream) {
     if (g.size <= 32) return launch_forward<T, 32>(g, kind, grid, joins, n_joins, stream);
     if (g.size <= 64) return launch_forward<T, 64>(g, kind, grid, joins, n_joins, stream);
+    if (g.size <= 96) return launch_forward<T, 96>(g, kind, grid, joins, n_joins, stream);
     return launch_forward<T, 128>(g, kind, grid, joins, n_joins, stream);
 }
 

@@ -77,7 +77,7 @@ template <class T, int DP> __device__ __forceinline__ void add_row(floatx16 (&o)
 }
 
 template <class T, int DP, int BN>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) attention_grad_queries(const GradArgs g) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_grad_queries(const GradArgs g) {
     constexpr int TILE = BN * DP;
     typedef Stager<T, DP, BN, 4> St;
     __shared__ T k0[TILE], v0[TILE], k1[TILE], v1[TILE];
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2) atte
 }
 
 template <class T, int DP, int BQ>
-__global__ void __launch_bounds__(256, 2) attention_grad_keys(const GradArgs g) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_grad_keys(const GradArgs g) {
     constexpr int TILE = BQ * DP;
     typedef Stager<T, DP, BQ, 4> St;
     __shared__ T q0[TILE], d0[TILE], q1[TILE], d1[TILE];
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(256, 2) attention_grad_keys(const GradArgs g) 
 }
 
 template <class T, int DP> int launch_backward(GradArgs g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
-    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP < 128 ? 64 : 32;
+    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     unsigned grid;
     if (n_q > 0) {
         g.items = q_items;
@@ -315,6 +315,7 @@ template <class T, int DP> int launch_backward(GradArgs g, const Item *q_items, 
 template <class T> int launch_backward(const GradArgs &g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
     if (g.size <= 32) return launch_backward<T, 32>(g, q_items, n_q, k_items, n_k, stream);
     if (g.size <= 64) return launch_backward<T, 64>(g, q_items, n_q, k_items, n_k, stream);
+    if (g.size <= 96) return launch_backward<T, 96>(g, q_items, n_q, k_items, n_k, stream);
     return launch_backward<T, 128>(g, q_items, n_q, k_items, n_k, stream);
 }
 

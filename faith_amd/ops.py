@@ -1298,7 +1298,7 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
         with _on(dev):
             plan = packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), causal)
         _, items, n, joins, parts, kind, _ = plan
-        floats = parts * kv_heads * (32 if kind else 128) * ((32 if size <= 32 else 64 if size <= 64 else 128) + 4)
+        floats = parts * kv_heads * (32 if kind else 128) * ((size + 31) // 32 * 32 + 4)
         if out is None:
             ot, oh = heads * size, size
         else:

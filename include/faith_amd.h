@@ -657,7 +657,7 @@ int faith_convolution_verification(const float *x_lb, const float *x_ub,
  *   counts    [4]: items; joins (they follow the items in the array); parts of cut rows; kind
  * The array, copied to the device, serves every call with these lengths, heads, element size and `causal`, from any
  * stream, until the lengths change.  faith_attention needs parts * kv_heads * (kind ? 32 : 128) * (size rounded up to
- * 32, 64 or 128, + 4) floats of scratch, which calls that may overlap must not share.
+ * a multiple of 32, + 4) floats of scratch, which calls that may overlap must not share.
  */
 #define FAITH_ATTENTION_FORWARD       0
 #define FAITH_ATTENTION_GRAD_QUERIES  1
