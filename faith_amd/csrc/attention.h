@@ -9,6 +9,8 @@
 #pragma once
 #include "common.h"
 
+#include <type_traits>
+
 namespace faith {
 namespace attn {
 
@@ -34,6 +36,10 @@ __device__ __forceinline__ floatx16 mfma(float a, float b, floatx16 c) { return 
 
 // the row that register r of a lane in half `half` of the wavefront holds of a 32 x 32 result
 __device__ __forceinline__ constexpr int row_of(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
+
+// How a workgroup's wavefronts share its work: each has 32 rows of its own, or all have the same 32 and take turns at the tiles
+// of the rest (KEYS; ONCE where none has a second turn: one stage, half the LDS, twice the workgroups on a compute unit)
+constexpr int KIND_ROWS = 0, KIND_KEYS = 1, KIND_ONCE = 2;
 
 // One unit of work of one key head; eight ints, read as one scalar load.
 struct Item {
@@ -182,19 +188,50 @@ template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(co
     return acc;
 }
 
-// the values of one row (DP of them, zero behind `size`) in the order in which rows_by_column takes them
+// the values of one row (DP of them, zero behind `size`) in the order in which rows_by_column takes them; all loads first, with
+// no branch between them
 template <class T, int DP> __device__ __forceinline__ ColumnRegs<T, DP> column_regs(const T *row, int half, int size) {
     ColumnRegs<T, DP> b;
-    constexpr int PER = 16 / (int)sizeof(T);
+    constexpr int PER = 16 / (int)sizeof(T), N = DP / (2 * PER);
+    uintx4 z[N];
 #pragma unroll
-    for (int u = 0; u < DP / (2 * PER); ++u) {
+    for (int u = 0; u < N; ++u) {
         const int d = (2 * u + half) * PER;
-        uintx4 z = {0u, 0u, 0u, 0u};
-        if (d < size) z = *reinterpret_cast<const uintx4 *>(row + d);
-        if constexpr (sizeof(T) == 4) b.v[u] = __builtin_bit_cast(floatx4, z);
-        else b.v[u] = __builtin_bit_cast(typename Vec<T>::x8, z);
+        z[u] = *reinterpret_cast<const uintx4 *>(row + (d < size ? d : 0));
+    }
+    if (size < DP) {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if ((2 * u + half) * PER >= size) z[u] = uintx4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        if constexpr (sizeof(T) == 4) b.v[u] = __builtin_bit_cast(floatx4, z[u]);
+        else b.v[u] = __builtin_bit_cast(typename Vec<T>::x8, z[u]);
     }
     return b;
+}
+
+// this lane's column of a result, `factor` times, to a row of T
+template <class T, int DP> __device__ __forceinline__ void store_column(T *dst, const floatx16 (&o)[DP / 32], float factor, int half, int size) {
+    auto all = [&](auto checked) {
+#pragma unroll
+        for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int d = 32 * m + row_of(r, half);
+                if (decltype(checked)::value && d >= size) continue;
+                if constexpr (sizeof(T) == 4) {
+                    const floatx4 x = {o[m][r] * factor, o[m][r + 1] * factor, o[m][r + 2] * factor, o[m][r + 3] * factor};
+                    *reinterpret_cast<floatx4 *>(dst + d) = x;
+                } else {
+                    const typename Vec<T>::x4 x = {(T)(o[m][r] * factor), (T)(o[m][r + 1] * factor), (T)(o[m][r + 2] * factor), (T)(o[m][r + 3] * factor)};
+                    *reinterpret_cast<typename Vec<T>::x4 *>(dst + d) = x;
+                }
+            }
+    };
+    if (size == DP) all(std::false_type{});
+    else all(std::true_type{});
 }
 
 // acc[m][r] += sum over the tile's 32 rows from row0 on of tile[row][32 m + row_of(r)] * p[row]: p is a result register set of
@@ -233,6 +270,64 @@ __device__ __forceinline__ float sum_halves(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     const unsigned a = s[0], b = s[1];
     return __uint_as_float(a) + __uint_as_float(b);
+}
+
+// Wavefronts of a workgroup that share their columns and divide the reduction, each with tiles of its own: four, unless their
+// four pairs of stages would not fit LDS (fp32, heads of more than 64).
+constexpr int split_waves(int element_size, int padded) { return 32 * padded * element_size * 16 <= 128 * 1024 ? 4 : 2; }
+template <class T, int DP> constexpr int split_waves() { return split_waves((int)sizeof(T), DP); }
+
+// The reduction of such a wavefront: its tiles first, first + step, ... < end, no barrier; `stage(n, i)` issues LOADS loads for
+// tile i into stage n (the caller has done so for the first), `use(n, i)` works on it while the younger stage's loads stay in
+// flight.
+template <int LOADS, bool ONCE, class Stage, class Use> __device__ __forceinline__ void alone(int first, int step, int end, Stage stage, Use use) {
+    if constexpr (ONCE) {
+        if (first >= end) return;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        use(0, first);
+        return;
+    }
+    for (int i = first; i < end; i += 2 * step) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + step < end) {
+            stage(1, i + step);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        }
+        use(0, i);
+        if (i + step >= end) break;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + 2 * step < end) {
+            stage(0, i + 2 * step);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        }
+        use(1, i + step);
+    }
+}
+
+// Adds the wavefronts' results up in the first one, in order; lo and hi: room for them (HALF floats each).
+template <int WAVES, int DP, int HALF> __device__ __forceinline__ void add_waves(floatx16 (&o)[DP / 32], float *lo, float *hi, int wave, int lane) {
+    constexpr int WIDTH = DP / 32 * 16;
+    static_assert((WAVES - 1) * 64 * WIDTH <= 2 * HALF, "the results fit");
+    __syncthreads();
+    if (wave > 0)
+#pragma unroll
+        for (int e = 0; e < WIDTH; ++e) {
+            const int x = ((wave - 1) * WIDTH + e) * 64 + lane;
+            (x < HALF ? lo[x] : hi[x - HALF]) = o[e / 16][e % 16];
+        }
+    __syncthreads();
+    if (wave == 0)
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; ++w)
+#pragma unroll
+            for (int e = 0; e < WIDTH; ++e) {
+                const int x = (w * WIDTH + e) * 64 + lane;
+                o[e / 16][e % 16] += x < HALF ? lo[x] : hi[x - HALF];
+            }
 }
 
 // This wavefront's loads into LDS have landed and its reads are done; then the barrier.  (The compiler does not see

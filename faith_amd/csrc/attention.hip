@@ -19,7 +19,6 @@ namespace {
 using namespace faith;
 using namespace faith::attn;
 
-constexpr int KIND_ROWS = 0, KIND_KEYS = 1;
 constexpr int MFMA = 0x8, VALU = 0x2, DS_READ = 0x100;      // classes of __builtin_amdgcn_sched_group_barrier
 constexpr float LOWEST = -3.0e38f;           // stands for "no key yet": finite, so that differences stay numbers
 constexpr float LAZY = 8.f;                  // powers of two by which a row's largest score may pass its reference
@@ -69,16 +68,14 @@ __device__ void one_row(const FwdArgs &g, const Item &it, int hk, const T *qrow,
     *sum = l;
 }
 
-// wavefronts of a workgroup that splits the keys: four, unless their four pairs of stages would not fit LDS (fp32, heads of 128)
-template <class T, int DP> constexpr int key_waves() { return 32 * DP * (int)sizeof(T) * 16 <= 128 * 1024 ? 4 : 2; }
-
-template <class T, int DP, int BN, bool KEYS, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, KEYS && DP * sizeof(T) >= 192 ? 1 : 2) attention_forward(const FwdArgs g) {
-    constexpr int TILE = BN * DP;
+template <class T, int DP, int BN, int KIND, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS && DP * sizeof(T) >= 192 ? 1 : 2) attention_forward(const FwdArgs g) {
+    constexpr bool KEYS = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
+    constexpr int TILE = BN * DP, ALL = TILE * (KEYS ? WAVES : 1);
     typedef Stager<T, DP, BN, KEYS ? 1 : 4> St;                     // keys: read by rows
     typedef Stager<T, DP, BN, KEYS ? 1 : 4, COLUMNS> Sv;            // values: by columns only
     // two stages in arrays of their own, so that the compiler sees that loads into one do not touch the other
-    __shared__ T k0[TILE * (KEYS ? WAVES : 1)], v0[TILE * (KEYS ? WAVES : 1)], k1[TILE * (KEYS ? WAVES : 1)], v1[TILE * (KEYS ? WAVES : 1)];
+    __shared__ T k0[ALL], v0[ALL], k1[ONCE ? 1 : ALL], v1[ONCE ? 1 : ALL];
 
     int hk, n;
     if (!dealt(g.deal, &hk, &n)) return;
@@ -234,37 +231,18 @@ __global__ void __launch_bounds__(64 * WAVES, KEYS && DP * sizeof(T) >= 192 ? 1 
             }
         }
     } else {
-        const int first = it.begin + wave * BN;
-        if (first < it.end) {
-            // this wavefront's own tiles, no barrier: the younger stage's loads stay in flight while the older is used
-            constexpr int INFLIGHT = 2 * St::LOADS;
-            auto wait_for_older = [&](bool younger) {
-                if (younger) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(INFLIGHT) : "memory");
-                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            };
-            stage(k0, v0, first);
-            for (int key0 = first; key0 < it.end; key0 += 2 * WAVES * BN) {
-                const bool b = key0 + WAVES * BN < it.end;
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (b) stage(k1, v1, key0 + WAVES * BN);
-                wait_for_older(b);
-                tile(k0, v0, key0);
-                if (!b) break;
-                const bool a = key0 + 2 * WAVES * BN < it.end;
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (a) stage(k0, v0, key0 + 2 * WAVES * BN);
-                wait_for_older(a);
-                tile(k1, v1, key0 + WAVES * BN);
-            }
-        }
+        if (it.begin + wave * BN < it.end) stage(k0, v0, it.begin + wave * BN);
+        alone<2 * St::LOADS, ONCE>(it.begin + wave * BN, WAVES * BN, it.end,
+                             [&](int n, int key0) { n ? stage(k1, v1, key0) : stage(k0, v0, key0); },
+                             [&](int n, int key0) { n ? tile(k1, v1, key0) : tile(k0, v0, key0); });
         // the wavefronts' results meet in LDS: each leaves (reference, sum) and its output, the first joins them
         __syncthreads();
-        constexpr int WIDTH = DP / 32 * 16;
-        static_assert((WAVES - 1) * 64 * WIDTH * 4 <= 2 * TILE * WAVES * (int)sizeof(T), "the results fit the two stages of keys");
-        float *lo = reinterpret_cast<float *>(k0), *hi = reinterpret_cast<float *>(k1), *ml = reinterpret_cast<float *>(v0);
+        constexpr int WIDTH = DP / 32 * 16, HALF = ALL * (int)sizeof(T) / 4;
+        static_assert((WAVES - 1) * 64 * WIDTH <= 2 * HALF, "the results fit a stage");
+        __shared__ float ml[(WAVES - 1) * 128];
+        float *lo = reinterpret_cast<float *>(k0), *hi = reinterpret_cast<float *>(v0);
         auto cell = [&](int w, int e) -> float & {                 // result w, register e of this lane
             const int x = (w * WIDTH + e) * 64 + lane;
-            constexpr int HALF = TILE * WAVES * (int)sizeof(T) / 4;
             return x < HALF ? lo[x] : hi[x - HALF];
         };
         if (wave > 0) {
@@ -324,20 +302,7 @@ __global__ void __launch_bounds__(64 * WAVES, KEYS && DP * sizeof(T) >= 192 ? 1 
     }
     const float inverse = sum > 0.f || sum != sum ? 1.f / sum : 0.f;   // no key: zeros
     T *dst = reinterpret_cast<T *>(g.out) + (long long)(it.q_start + token) * g.o_ts + (long long)head * g.o_hs;
-#pragma unroll
-    for (int m = 0; m < DP / 32; ++m)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * m + row_of(r, half);
-            if (d >= g.size) continue;
-            if constexpr (sizeof(T) == 4) {
-                const floatx4 x = {o[m][r] * inverse, o[m][r + 1] * inverse, o[m][r + 2] * inverse, o[m][r + 3] * inverse};
-                *reinterpret_cast<floatx4 *>(dst + d) = x;
-            } else {
-                const typename Vec<T>::x4 x = {(T)(o[m][r] * inverse), (T)(o[m][r + 1] * inverse), (T)(o[m][r + 2] * inverse), (T)(o[m][r + 3] * inverse)};
-                *reinterpret_cast<typename Vec<T>::x4 *>(dst + d) = x;
-            }
-        }
+    store_column<T, DP>(dst, o, inverse, half, g.size);
     if (g.lse && half == 0)
         g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
 }
@@ -377,12 +342,13 @@ __global__ void __launch_bounds__(256) attention_join(const FwdArgs g, const Ite
 
 template <class T, int DP> int launch_forward(const FwdArgs &g, int kind, unsigned grid, const Item *joins, int n_joins, hipStream_t stream) {
     constexpr int BN = sizeof(T) == 4 ? 32 : 64;
-    constexpr int WAVES = key_waves<T, DP>();
-    if (kind == KIND_KEYS) hipLaunchKernelGGL((attention_forward<T, DP, 32, true, WAVES>), dim3(grid), dim3(64 * WAVES), 0, stream, g);
-    else hipLaunchKernelGGL((attention_forward<T, DP, BN, false, 4>), dim3(grid), dim3(256), 0, stream, g);
+    constexpr int WAVES = split_waves<T, DP>();
+    if (kind == KIND_ONCE) hipLaunchKernelGGL((attention_forward<T, DP, 32, KIND_ONCE, WAVES>), dim3(grid), dim3(64 * WAVES), 0, stream, g);
+    else if (kind == KIND_KEYS) hipLaunchKernelGGL((attention_forward<T, DP, 32, KIND_KEYS, WAVES>), dim3(grid), dim3(64 * WAVES), 0, stream, g);
+    else hipLaunchKernelGGL((attention_forward<T, DP, BN, KIND_ROWS, 4>), dim3(grid), dim3(256), 0, stream, g);
     if (n_joins > 0) {
-        if (kind == KIND_KEYS) hipLaunchKernelGGL((attention_join<T, DP, 32>), dim3(n_joins, g.kv_heads, 1), dim3(256), 0, stream, g, joins);
-        else hipLaunchKernelGGL((attention_join<T, DP, 128>), dim3(n_joins, g.kv_heads, 8), dim3(256), 0, stream, g, joins);
+        if (kind != KIND_ROWS) hipLaunchKernelGGL((attention_join<T, DP, 32>), dim3(n_joins, g.kv_heads, 8), dim3(256), 0, stream, g, joins);
+        else hipLaunchKernelGGL((attention_join<T, DP, 128>), dim3(n_joins, g.kv_heads, 32), dim3(256), 0, stream, g, joins);
     }
     return check_launch("faith_attention");
 }
@@ -403,24 +369,34 @@ struct Plan {
     int kind = KIND_ROWS, slots = 0;
 };
 
-int tile_of(int pass, int kind, int element_size) {
-    if (pass == FAITH_ATTENTION_FORWARD) return kind == KIND_KEYS || element_size == 4 ? 32 : 64;
-    return 32;
-}
-
-// Items of one pass, longest first.  The forward pass cuts an item's keys where there are fewer items than the device holds
-// workgroups: into parts of equal length, as many as make up that number, none under 256 keys.
-Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int element_size, int causal, int pass) {
+// Items of one pass, longest first.
+// Wavefronts share their rows and divide the rest (KEYS) for 32 rows or fewer, and
+//   backward  where workgroups of 128 rows would leave half of the compute units without one: 1000 tokens, 4 heads of 64, bf16
+//             26 us instead of 52; 2048 tokens, 8 / 2 heads of 128 152 instead of 467; 20 sequences of 256 with 4 heads (160
+//             workgroups) would take 33 instead of 21
+//   forward   there too, in fp32, if none has a second turn: 30 sequences of 128, 4 heads of 64 11.2 us instead of 13.4.  With
+//             more keys, or 2-byte elements, 128 rows and cut keys are faster (1000 tokens as above: 18 against 28).
+// The forward pass cuts an item's keys where there are fewer items than the device holds workgroups: into parts of equal
+// length, as many as make up that number, none under 256 keys.
+Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int element_size, int size, int causal, int pass) {
     Plan p;
     long long qs = 0, ks = 0;
-    int most = 0;
-    for (int b = 0; b < n; ++b) most = std::max(most, ql[b]);
-    if (pass == FAITH_ATTENTION_FORWARD && (long long)most * group <= 32) p.kind = KIND_KEYS;
-    const int rows_per = p.kind == KIND_KEYS ? 32 : 128, bn = tile_of(pass, p.kind, element_size);
+    const int cus = compute_units();
+    const int waves = split_waves(element_size, (size + 31) / 32 * 32);
+    long long most = 0, tall = 0;            // rows of a sequence; workgroups of 128 rows
+    int keys_most = 0;
+    for (int b = 0; b < n; ++b) {
+        const long long rows = pass == FAITH_ATTENTION_GRAD_KEYS ? kl[b] : (long long)ql[b] * group;
+        most = std::max(most, rows);
+        tall += (rows + 127) / 128 * kv_heads;
+        keys_most = std::max(keys_most, kl[b]);
+    }
+    if (most <= 32 || (2 * tall <= cus && (pass != FAITH_ATTENTION_FORWARD || (element_size == 4 && keys_most <= 32 * waves)))) p.kind = KIND_KEYS;
+    const int rows_per = p.kind == KIND_KEYS ? 32 : 128, bn = p.kind == KIND_KEYS || element_size == 4 ? 32 : 64;
     for (int b = 0; b < n; ++b) {
         const int shift = kl[b] - ql[b];
         if (pass == FAITH_ATTENTION_GRAD_KEYS) {
-            for (int key0 = 0; key0 < kl[b]; key0 += 128) {
+            for (int key0 = 0; key0 < kl[b]; key0 += rows_per) {
                 // the first token that sees a key of the tile
                 const int begin = causal ? std::min(ql[b], std::max(0, key0 - shift)) : 0;
                 p.items.push_back({(int)qs, ql[b], (int)ks, kl[b], key0, begin / 32 * 32, ql[b], -1});
@@ -436,7 +412,7 @@ Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int
         qs += ql[b];
         ks += kl[b];
     }
-    const long long resident = 2LL * compute_units(), blocks = (long long)p.items.size() * kv_heads;
+    const long long resident = 2LL * cus, blocks = (long long)p.items.size() * kv_heads;
     if (pass == FAITH_ATTENTION_FORWARD && blocks > 0 && blocks < (p.kind == KIND_KEYS ? 4 : 1) * resident) {
         long long keys = 0;
         for (const Item &it : p.items) keys += it.end;
@@ -463,6 +439,12 @@ Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int
         }
         p.items.swap(cut);
     }
+    if (p.kind == KIND_KEYS) {
+        // tiles of an item, as many of which as there are wavefronts are worked on at once
+        const int times = pass == FAITH_ATTENTION_GRAD_KEYS ? group : 1;
+        const bool once = std::all_of(p.items.begin(), p.items.end(), [&](const Item &it) { return (long long)((it.end - it.begin + 31) / 32) * times <= waves; });
+        if (once) p.kind = KIND_ONCE;
+    }
     std::stable_sort(p.items.begin(), p.items.end(), [](const Item &a, const Item &b) { return a.end - a.begin > b.end - b.begin; });
     return p;
 }
@@ -470,13 +452,14 @@ Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int
 }  // namespace
 
 extern "C" int faith_attention_plan(const int *query_lengths, const int *key_lengths, int sequences, int heads, int kv_heads,
-                                    int element_size, int causal, int pass, int *items, long long capacity, long long *counts) {
+                                    int element_size, int size, int causal, int pass, int *items, long long capacity, long long *counts) {
     FAITH_NOT_NULL(query_lengths);
     FAITH_NOT_NULL(key_lengths);
     FAITH_NOT_NULL(counts);
     FAITH_REQUIRE(sequences > 0, FAITH_ERR_SHAPE, "%s: %d sequences", __func__, sequences);
     FAITH_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, FAITH_ERR_SHAPE, "%s: %d heads do not share %d key heads evenly", __func__, heads, kv_heads);
     FAITH_REQUIRE(element_size == 2 || element_size == 4, FAITH_ERR_UNSUPPORTED, "%s: elements of %d bytes", __func__, element_size);
+    FAITH_REQUIRE(size > 0 && size <= 128, FAITH_ERR_UNSUPPORTED, "%s: heads of %d elements", __func__, size);
     FAITH_REQUIRE(pass >= FAITH_ATTENTION_FORWARD && pass <= FAITH_ATTENTION_GRAD_KEYS, FAITH_ERR_UNSUPPORTED, "%s: pass %d", __func__, pass);
     long long q = 0, k = 0;
     for (int b = 0; b < sequences; ++b) {
@@ -488,7 +471,7 @@ extern "C" int faith_attention_plan(const int *query_lengths, const int *key_len
     }
     FAITH_REQUIRE(q < (1LL << 31) && k < (1LL << 31), FAITH_ERR_SHAPE, "%s: more than 2^31 tokens", __func__);
     try {
-        const Plan p = make_plan(query_lengths, key_lengths, sequences, heads / kv_heads, kv_heads, element_size, causal, pass);
+        const Plan p = make_plan(query_lengths, key_lengths, sequences, heads / kv_heads, kv_heads, element_size, size, causal, pass);
         counts[0] = (long long)p.items.size();
         counts[1] = (long long)p.joins.size();
         counts[2] = p.slots;
@@ -515,7 +498,7 @@ extern "C" int faith_attention(const void *q, const void *k, const void *v, void
     FAITH_NOT_NULL(out);
     FAITH_NOT_NULL(items);
     FAITH_REQUIRE(n_joins == 0 || parts, FAITH_ERR_NULL, "%s: keys are cut into parts, and there is no room for their results", __func__);
-    FAITH_REQUIRE(kind == KIND_ROWS || kind == KIND_KEYS, FAITH_ERR_UNSUPPORTED, "%s: kind %d", __func__, kind);
+    FAITH_REQUIRE(kind >= KIND_ROWS && kind <= KIND_ONCE, FAITH_ERR_UNSUPPORTED, "%s: kind %d", __func__, kind);
     const int rc = attention_shapes(__func__, heads, kv_heads, size, dtype, scale);
     if (rc != FAITH_OK) return rc;
     const int es = dtype == FAITH_F32 ? 4 : 2;

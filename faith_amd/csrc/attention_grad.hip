@@ -34,23 +34,6 @@ template <class T> __device__ __forceinline__ float dot_rows(const T *a, const T
     return s;
 }
 
-// this lane's column of a result, `factor` times, to a row of T
-template <class T, int DP> __device__ __forceinline__ void store_column(T *dst, const floatx16 (&o)[DP / 32], float factor, int half, int size) {
-#pragma unroll
-    for (int m = 0; m < DP / 32; ++m)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * m + row_of(r, half);
-            if (d >= size) continue;
-            if constexpr (sizeof(T) == 4) {
-                const floatx4 x = {o[m][r] * factor, o[m][r + 1] * factor, o[m][r + 2] * factor, o[m][r + 3] * factor};
-                *reinterpret_cast<floatx4 *>(dst + d) = x;
-            } else {
-                const typename Vec<T>::x4 x = {(T)(o[m][r] * factor), (T)(o[m][r + 1] * factor), (T)(o[m][r + 2] * factor), (T)(o[m][r + 3] * factor)};
-                *reinterpret_cast<typename Vec<T>::x4 *>(dst + d) = x;
-            }
-        }
-}
 template <int DP> __device__ __forceinline__ void clear(floatx16 (&o)[DP / 32]) {
 #pragma unroll
     for (int m = 0; m < DP / 32; ++m)
@@ -76,40 +59,28 @@ template <class T, int DP> __device__ __forceinline__ void add_row(floatx16 (&o)
         }
 }
 
-template <class T, int DP, int BN>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_grad_queries(const GradArgs g) {
-    constexpr int TILE = BN * DP;
-    typedef Stager<T, DP, BN, 4> St;
-    __shared__ T k0[TILE], v0[TILE], k1[TILE], v1[TILE];
+// SPLIT: the wavefronts share 32 rows and divide the keys, as in attention.hip
+template <class T, int DP, int BN, int KIND, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_grad_queries(const GradArgs g) {
+    constexpr bool SPLIT = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
+    constexpr int TILE = BN * DP, ALL = TILE * (SPLIT ? WAVES : 1);
+    typedef Stager<T, DP, BN, SPLIT ? 1 : WAVES> St;
+    __shared__ T k0[ALL], v0[ALL], k1[ONCE ? 1 : ALL], v1[ONCE ? 1 : ALL];
 
     int hk, n;
     if (!dealt(g.deal, &hk, &n)) return;
     const Item it = g.items[n];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int half = lane >> 5, col = lane & 31;
-    const int row_lo = it.row0 + wave * 32, row = row_lo + col, rows = it.q_len * g.group;
+    const int staged = SPLIT ? 0 : wave, own = SPLIT ? wave * TILE : 0;
+    const int row_lo = it.row0 + (SPLIT ? 0 : wave * 32), row = row_lo + col, rows = it.q_len * g.group;
     const int mine = row < rows ? row : rows - 1;
     const int token = mine / g.group, head = hk * g.group + (mine - token * g.group);
     const long long place = it.q_start + token;
     const T *qrow = at<T>(g.q, place, g.q_ts, head, g.q_hs), *dorow = at<T>(g.dout, place, g.do_ts, head, g.do_hs);
     const ColumnRegs<T, DP> q = column_regs<T, DP>(qrow, half, g.size), d_o = column_regs<T, DP>(dorow, half, g.size);
-    float delta = 0.f;
-    {
-        const ColumnRegs<T, DP> o = column_regs<T, DP>(at<T>(g.out, place, g.o_ts, head, g.o_hs), half, g.size);
-        constexpr int PER = 16 / (int)sizeof(T);
-#pragma unroll
-        for (int u = 0; u < DP / (2 * PER); ++u)
-#pragma unroll
-            for (int e = 0; e < PER; ++e) delta = fmaf((float)o.v[u][e], (float)d_o.v[u][e], delta);
-        delta = sum_halves(delta);
-    }
+    const ColumnRegs<T, DP> o = column_regs<T, DP>(at<T>(g.out, place, g.o_ts, head, g.o_hs), half, g.size);
     const float l = g.lse[(long long)head * g.lse_hs + place];
-    const float lse = l == -__builtin_inff() ? 0.f : l * 1.4426950408889634f;      // a row that sees no key: every p below is masked
-    if (row < rows && half == 0) {
-        float *s = g.stat + (long long)head * g.lse_hs + place;
-        s[0] = lse;
-        s[(long long)g.kv_heads * g.group * g.lse_hs] = delta;
-    }
     int last = it.k_len - 1, all_see = it.k_len - 1, any_sees = it.k_len - 1;
     if (g.causal) {
         const int shift = it.k_len - it.q_len, row_hi = row_lo + 31 < rows ? row_lo + 31 : rows - 1;
@@ -123,20 +94,36 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     floatx16 dq[DP / 32];
     clear<DP>(dq);
     St ks, vs;
-    ks.init(lane, wave, g.size, g.k_ts);
-    vs.init(lane, wave, g.size, g.v_ts);
+    ks.init(lane, staged, g.size, g.k_ts);
+    vs.init(lane, staged, g.size, g.v_ts);
     const T *kb = at<T>(g.k, it.k_start, g.k_ts, hk, g.k_hs), *vb = at<T>(g.v, it.k_start, g.v_ts, hk, g.v_hs);
     auto stage = [&](T *kt, T *vt, int key0) {
-        ks.load(kt, kb + (long long)key0 * g.k_ts, it.k_len - key0, g.size, wave);
-        vs.load(vt, vb + (long long)key0 * g.v_ts, it.k_len - key0, g.size, wave);
+        ks.load(kt + own, kb + (long long)key0 * g.k_ts, it.k_len - key0, g.size, staged);
+        vs.load(vt + own, vb + (long long)key0 * g.v_ts, it.k_len - key0, g.size, staged);
     };
+    // the first tile is on its way before anything waits for this lane's row
+    const int first = it.begin + (SPLIT ? wave * BN : 0);
+    if (first < it.end) stage(k0, v0, first);
+    float delta = 0.f;
+    constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int u = 0; u < DP / (2 * PER); ++u)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) delta = fmaf((float)o.v[u][e], (float)d_o.v[u][e], delta);
+    delta = sum_halves(delta);
+    const float lse = l == -__builtin_inff() ? 0.f : l * 1.4426950408889634f;      // a row that sees no key: every p below is masked
+    if (row < rows && half == 0 && (!SPLIT || wave == 0)) {
+        float *s = g.stat + (long long)head * g.lse_hs + place;
+        s[0] = lse;
+        s[(long long)g.kv_heads * g.group * g.lse_hs] = delta;
+    }
     auto tile = [&](const T *kt, const T *vt, int key0) {
         if (key0 > any_sees) return;
         const bool part = key0 + BN - 1 > all_see;
 #pragma unroll
         for (int b = 0; b < BN / 32; ++b) {
-            floatx16 s = rows_by_column<T, DP>(kt, 32 * b + col, half, q);
-            const floatx16 dp = rows_by_column<T, DP>(vt, 32 * b + col, half, d_o);
+            floatx16 s = rows_by_column<T, DP>(kt + own, 32 * b + col, half, q);
+            const floatx16 dp = rows_by_column<T, DP>(vt + own, 32 * b + col, half, d_o);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], g.c, -lse)) * (dp[r] - delta);
             if (part) {
@@ -144,11 +131,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
                 for (int r = 0; r < 16; ++r)
                     if (key0 + 32 * b + row_of(r, half) > last) s[r] = 0.f;
             }
-            columns_by_result<T, DP>(dq, kt, 32 * b, lane, s);
+            columns_by_result<T, DP>(dq, kt + own, 32 * b, lane, s);
         }
     };
-    if (it.begin < it.end) {
-        stage(k0, v0, it.begin);
+    if constexpr (SPLIT) {
+        alone<2 * St::LOADS, ONCE>(first, WAVES * BN, it.end,
+                             [&](int n, int key0) { n ? stage(k1, v1, key0) : stage(k0, v0, key0); },
+                             [&](int n, int key0) { n ? tile(k1, v1, key0) : tile(k0, v0, key0); });
+        add_waves<WAVES, DP, ALL * (int)sizeof(T) / 4>(dq, reinterpret_cast<float *>(k0), reinterpret_cast<float *>(v0), wave, lane);
+        if (wave > 0) return;
+    } else if (it.begin < it.end) {
         for (int key0 = it.begin; key0 < it.end; key0 += 2 * BN) {
             landed_and_barrier();
             if (key0 + BN < it.end) stage(k1, v1, key0 + BN);
@@ -172,23 +164,25 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     store_column<T, DP>(const_cast<T *>(at<T>(g.dq, place, g.dq_ts, head, g.dq_hs)), dq, g.scale, half, g.size);
 }
 
-template <class T, int DP, int BQ>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_grad_keys(const GradArgs g) {
-    constexpr int TILE = BQ * DP;
-    typedef Stager<T, DP, BQ, 4> St;
-    __shared__ T q0[TILE], d0[TILE], q1[TILE], d1[TILE];
-    __shared__ float l0[64], e0[64], l1[64], e1[64];           // lse, delta of the staged queries
+template <class T, int DP, int BQ, int KIND, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_grad_keys(const GradArgs g) {
+    constexpr bool SPLIT = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
+    constexpr int TILE = BQ * DP, EACH = SPLIT ? WAVES : 1, ALL = TILE * EACH;
+    typedef Stager<T, DP, BQ, SPLIT ? 1 : WAVES> St;
+    __shared__ T q0[ALL], d0[ALL], q1[ONCE ? 1 : ALL], d1[ONCE ? 1 : ALL];
+    __shared__ float l0[64 * EACH], e0[64 * EACH], l1[ONCE ? 1 : 64 * EACH], e1[ONCE ? 1 : 64 * EACH];           // lse, delta of the staged queries
 
     int hk, n;
     if (!dealt(g.deal, &hk, &n)) return;
     const Item it = g.items[n];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int half = lane >> 5, col = lane & 31;
-    const int key_lo = it.row0 + wave * 32, key = key_lo + col, mine = key < it.k_len ? key : it.k_len - 1;
+    const int staged = SPLIT ? 0 : wave, own = SPLIT ? wave * TILE : 0, own64 = SPLIT ? wave * 64 : 0;
+    const int key_lo = it.row0 + (SPLIT ? 0 : wave * 32), key = key_lo + col, mine = key < it.k_len ? key : it.k_len - 1;
     const T *krow = at<T>(g.k, it.k_start + mine, g.k_ts, hk, g.k_hs), *vrow = at<T>(g.v, it.k_start + mine, g.v_ts, hk, g.v_hs);
     const ColumnRegs<T, DP> k = column_regs<T, DP>(krow, half, g.size);
     // The values' rows stay in LDS where registers for them would halve the wavefronts on a SIMD
-    constexpr bool V_IN_LDS = sizeof(T) == 2 && DP == 128;
+    constexpr bool V_IN_LDS = !SPLIT && sizeof(T) == 2 && DP == 128;
     __shared__ T v_rows[V_IN_LDS ? 128 * DP : 1];
     ColumnRegs<T, DP> v;
     if constexpr (V_IN_LDS) {
@@ -206,28 +200,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     clear<DP>(dk);
     clear<DP>(dv);
     St qs, ds;
-    qs.init(lane, wave, g.size, g.q_ts);
-    ds.init(lane, wave, g.size, g.do_ts);
+    qs.init(lane, staged, g.size, g.q_ts);
+    ds.init(lane, staged, g.size, g.do_ts);
     const int span = it.end - it.begin, tiles = (span + BQ - 1) / BQ, total = span > 0 ? tiles * g.group : 0;
     const long long stat_hs = (long long)g.kv_heads * g.group * g.lse_hs;
 
-    // step n: head n / tiles of the group, tokens from begin + (n % tiles) * BQ on
-    int next_h = 0, next_t = it.begin;
-    auto stage = [&](T *qt, T *dt, float *lt, float *et) {
-        const int h = hk * g.group + next_h, left = it.q_len - next_t;
-        qs.load(qt, at<T>(g.q, it.q_start + next_t, g.q_ts, h, g.q_hs), left, g.size, wave);
-        ds.load(dt, at<T>(g.dout, it.q_start + next_t, g.do_ts, h, g.do_hs), left, g.size, wave);
-        if (wave < 2) {
-            const float *s = g.stat + (wave ? stat_hs : 0) + (long long)h * g.lse_hs + it.q_start + next_t;
-            words_to_lds(wave ? et : lt, s, left < 64 ? left : 64, lane);
-        }
-        next_t += BQ;
-        if (next_t >= it.end) { next_t = it.begin; ++next_h; }
+    // the queries of head h of the group from token t on
+    auto stage_at = [&](T *qt, T *dt, float *lt, float *et, int h, int t) {
+        const int head = hk * g.group + h, left = it.q_len - t;
+        qs.load(qt + own, at<T>(g.q, it.q_start + t, g.q_ts, head, g.q_hs), left, g.size, staged);
+        ds.load(dt + own, at<T>(g.dout, it.q_start + t, g.do_ts, head, g.do_hs), left, g.size, staged);
+        const float *s = g.stat + (long long)head * g.lse_hs + it.q_start + t;
+        if (SPLIT || wave == 0) words_to_lds(lt + own64, s, left < 64 ? left : 64, lane);
+        if (SPLIT || wave == 1) words_to_lds(et + own64, s + stat_hs, left < 64 ? left : 64, lane);
     };
-    int tok0 = it.begin;
-    auto tile = [&](const T *qt, const T *dt, const float *lt, const float *et) {
-        const int t0 = tok0;
-        tok0 = tok0 + BQ >= it.end ? it.begin : tok0 + BQ;
+    auto tile_at = [&](const T *qt, const T *dt, const float *lt, const float *et, int t0) {
+        qt += own, dt += own, lt += own64, et += own64;
         if (t0 + BQ - 1 < any_sees) return;
         int lane = (int)threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
@@ -267,7 +255,28 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
             columns_by_result<T, DP>(dk, qt, 32 * b, lane, dp[b]);
         }
     };
-    if (total > 0) {
+    // step n: head n / tiles of the group, tokens from begin + (n % tiles) * BQ on
+    if constexpr (SPLIT) {
+        auto token = [&](int n) { return it.begin + n % tiles * BQ; };
+        if (wave < total) stage_at(q0, d0, l0, e0, wave / tiles, token(wave));
+        alone<2 * St::LOADS + 2, ONCE>(wave, WAVES, total,
+                                 [&](int n, int i) { n ? stage_at(q1, d1, l1, e1, i / tiles, token(i)) : stage_at(q0, d0, l0, e0, i / tiles, token(i)); },
+                                 [&](int n, int i) { n ? tile_at(q1, d1, l1, e1, token(i)) : tile_at(q0, d0, l0, e0, token(i)); });
+        constexpr int HALF = ALL * (int)sizeof(T) / 4;
+        add_waves<WAVES, DP, HALF>(dk, reinterpret_cast<float *>(q0), reinterpret_cast<float *>(d0), wave, lane);
+        add_waves<WAVES, DP, HALF>(dv, reinterpret_cast<float *>(q0), reinterpret_cast<float *>(d0), wave, lane);
+        if (wave > 0) return;
+    } else if (total > 0) {
+        int next_h = 0, next_t = it.begin, tok0 = it.begin;
+        auto stage = [&](T *qt, T *dt, float *lt, float *et) {
+            stage_at(qt, dt, lt, et, next_h, next_t);
+            next_t += BQ;
+            if (next_t >= it.end) { next_t = it.begin; ++next_h; }
+        };
+        auto tile = [&](const T *qt, const T *dt, const float *lt, const float *et) {
+            tile_at(qt, dt, lt, et, tok0);
+            tok0 = tok0 + BQ >= it.end ? it.begin : tok0 + BQ;
+        };
         stage(q0, d0, l0, e0);
         for (int i = 0; i < total; i += 2) {
             landed_and_barrier();
@@ -297,36 +306,44 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attent
     store_column<T, DP>(const_cast<T *>(at<T>(g.dv, it.k_start + key, g.dv_ts, hk, g.dv_hs)), dv, 1.f, half, g.size);
 }
 
-template <class T, int DP> int launch_backward(GradArgs g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
-    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
+struct Items { const Item *items; int n, kind; };
+
+template <class T, int DP> int launch_backward(GradArgs g, const Items &qi, const Items &ki, hipStream_t stream) {
+    constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32, W = split_waves<T, DP>();
     unsigned grid;
-    if (n_q > 0) {
-        g.items = q_items;
-        g.deal = deal(n_q, g.kv_heads, &grid);
-        hipLaunchKernelGGL((attention_grad_queries<T, DP, BN>), dim3(grid), dim3(256), 0, stream, g);
+    if (qi.n > 0) {
+        g.items = qi.items;
+        g.deal = deal(qi.n, g.kv_heads, &grid);
+        if (qi.kind == KIND_ONCE) hipLaunchKernelGGL((attention_grad_queries<T, DP, 32, KIND_ONCE, W>), dim3(grid), dim3(64 * W), 0, stream, g);
+        else if (qi.kind == KIND_KEYS) hipLaunchKernelGGL((attention_grad_queries<T, DP, 32, KIND_KEYS, W>), dim3(grid), dim3(64 * W), 0, stream, g);
+        else hipLaunchKernelGGL((attention_grad_queries<T, DP, BN, KIND_ROWS, 4>), dim3(grid), dim3(256), 0, stream, g);
     }
-    if (n_k > 0) {
-        g.items = k_items;
-        g.deal = deal(n_k, g.kv_heads, &grid);
-        hipLaunchKernelGGL((attention_grad_keys<T, DP, BQ>), dim3(grid), dim3(256), 0, stream, g);
+    if (ki.n > 0) {
+        g.items = ki.items;
+        g.deal = deal(ki.n, g.kv_heads, &grid);
+        if (ki.kind == KIND_ONCE) hipLaunchKernelGGL((attention_grad_keys<T, DP, 32, KIND_ONCE, W>), dim3(grid), dim3(64 * W), 0, stream, g);
+        else if (ki.kind == KIND_KEYS) hipLaunchKernelGGL((attention_grad_keys<T, DP, 32, KIND_KEYS, W>), dim3(grid), dim3(64 * W), 0, stream, g);
+        else hipLaunchKernelGGL((attention_grad_keys<T, DP, BQ, KIND_ROWS, 4>), dim3(grid), dim3(256), 0, stream, g);
     }
     return check_launch("faith_attention_backward");
 }
-template <class T> int launch_backward(const GradArgs &g, const Item *q_items, int n_q, const Item *k_items, int n_k, hipStream_t stream) {
-    if (g.size <= 32) return launch_backward<T, 32>(g, q_items, n_q, k_items, n_k, stream);
-    if (g.size <= 64) return launch_backward<T, 64>(g, q_items, n_q, k_items, n_k, stream);
-    if (g.size <= 96) return launch_backward<T, 96>(g, q_items, n_q, k_items, n_k, stream);
-    return launch_backward<T, 128>(g, q_items, n_q, k_items, n_k, stream);
+template <class T> int launch_backward(const GradArgs &g, const Items &qi, const Items &ki, hipStream_t stream) {
+    if (g.size <= 32) return launch_backward<T, 32>(g, qi, ki, stream);
+    if (g.size <= 64) return launch_backward<T, 64>(g, qi, ki, stream);
+    if (g.size <= 96) return launch_backward<T, 96>(g, qi, ki, stream);
+    return launch_backward<T, 128>(g, qi, ki, stream);
 }
 
 }  // namespace
 
 extern "C" int faith_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
                                         void *dq, void *dk, void *dv, float *stat, const int *query_items, int n_query_items,
-                                        const int *key_items, int n_key_items, const long long *strides, long long lse_head_stride,
+                                        int query_kind, const int *key_items, int n_key_items, int key_kind, const long long *strides, long long lse_head_stride,
                                         int heads, int kv_heads, int size, int dtype, int causal, float scale, void *stream) {
     FAITH_REQUIRE(n_query_items >= 0 && n_key_items >= 0, FAITH_ERR_SHAPE, "%s: %d and %d items", __func__, n_query_items, n_key_items);
     if (n_query_items == 0 && n_key_items == 0) return FAITH_OK;
+    FAITH_REQUIRE(query_kind >= KIND_ROWS && query_kind <= KIND_ONCE && key_kind >= KIND_ROWS && key_kind <= KIND_ONCE, FAITH_ERR_UNSUPPORTED,
+                  "%s: kinds %d and %d", __func__, query_kind, key_kind);
     FAITH_NOT_NULL(strides);
     const int rc = attention_shapes(__func__, heads, kv_heads, size, dtype, scale);
     if (rc != FAITH_OK) return rc;
@@ -347,9 +364,9 @@ extern "C" int faith_attention_backward(const void *dout, const void *q, const v
     g.lse_hs = lse_head_stride;
     g.group = heads / kv_heads; g.kv_heads = kv_heads; g.size = size; g.causal = causal;
     g.c = scale * 1.4426950408889634f; g.scale = scale;
-    const Item *qi = reinterpret_cast<const Item *>(query_items), *ki = reinterpret_cast<const Item *>(key_items);
+    const Items qi = {reinterpret_cast<const Item *>(query_items), n_query_items, query_kind}, ki = {reinterpret_cast<const Item *>(key_items), n_key_items, key_kind};
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == FAITH_F32) return launch_backward<float>(g, qi, n_query_items, ki, n_key_items, s);
-    if (dtype == FAITH_BF16) return launch_backward<__bf16>(g, qi, n_query_items, ki, n_key_items, s);
-    return launch_backward<_Float16>(g, qi, n_query_items, ki, n_key_items, s);
+    if (dtype == FAITH_F32) return launch_backward<float>(g, qi, ki, s);
+    if (dtype == FAITH_BF16) return launch_backward<__bf16>(g, qi, ki, s);
+    return launch_backward<_Float16>(g, qi, ki, s);
 }

@@ -1173,12 +1173,12 @@ class Packing:
             out.append(at)
         return out
 
-    def plan(self, which, heads, kv_heads, element_size, causal):
+    def plan(self, which, heads, kv_heads, element_size, size, causal):
         """(items on the device, their address, how many, joins, parts, kind) of one pass; see faith_attention_plan."""
-        key = (which, heads // kv_heads, kv_heads, element_size, bool(causal))
+        key = (which, heads // kv_heads, kv_heads, element_size, size, bool(causal))
         found = self._plans.get(key)
         if found is None:
-            found = self._plans[key] = self._make(which, heads, kv_heads, element_size, bool(causal))
+            found = self._plans[key] = self._make(which, heads, kv_heads, element_size, size, bool(causal))
         self._used_on(found, _stream(found[0]))
         return found
 
@@ -1187,12 +1187,12 @@ class Packing:
             # another stream than the one it was allocated on: its memory is not handed out again before this use is done
             plan[0].record_stream(torch.cuda.current_stream(self.device))
 
-    def _make(self, which, heads, kv_heads, element_size, causal):
+    def _make(self, which, heads, kv_heads, element_size, size, causal):
         import ctypes
         n = len(self.lengths)
         array = ctypes.c_int * n
         ql, kl, counts = array(*self.lengths), array(*self.key_lengths), (ctypes.c_longlong * 4)()
-        args = (ctypes.addressof(ql), ctypes.addressof(kl), n, heads, kv_heads, element_size, int(causal), which)
+        args = (ctypes.addressof(ql), ctypes.addressof(kl), n, heads, kv_heads, element_size, size, int(causal), which)
         with _on(self.device):
             _lib.call("faith_attention_plan", *args, None, 0, ctypes.addressof(counts))
             total = counts[0] + counts[1]
@@ -1296,7 +1296,7 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
         heads, kv_heads, size, (qt, qh), (kt, kh), (vt, vh) = _attention_operands(q, k, v, packing)
         dev = q.device
         with _on(dev):
-            plan = packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), causal)
+            plan = packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), size, causal)
         _, items, n, joins, parts, kind, _ = plan
         floats = parts * kv_heads * (32 if kind else 128) * ((size + 31) // 32 * 32 + 4)
         if out is None:
@@ -1332,8 +1332,8 @@ def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=Non
         row, kv_row = (heads * size, size), (kv_heads * size, size)
         strides = (ctypes.c_longlong * 16)(*ds, *qs, *ks, *vs, *os_, *row, *kv_row, *kv_row)
         with _on(q.device):
-            plans = [packing.plan(which, heads, kv_heads, q.element_size(), causal) for which in (_lib.ATTENTION_GRAD_QUERIES, _lib.ATTENTION_GRAD_KEYS)]
-        known = (plans, heads, (plans[0][1], plans[0][2], plans[1][1], plans[1][2], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
+            plans = [packing.plan(which, heads, kv_heads, q.element_size(), size, causal) for which in (_lib.ATTENTION_GRAD_QUERIES, _lib.ATTENTION_GRAD_KEYS)]
+        known = (plans, heads, (plans[0][1], plans[0][2], plans[0][5], plans[1][1], plans[1][2], plans[1][5], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
                                 size, _DTYPES[q.dtype], int(causal), _scale(scale, size)), strides)
         if key is not None and dout.shape == q.shape and out.shape == q.shape:
             packing._calls[key] = known

@@ -655,7 +655,7 @@ int faith_convolution_verification(const float *x_lb, const float *x_ub,
  *   items     eight ints an item, or NULL: only the counts are wanted
  *   capacity  items that fit
  *   counts    [4]: items; joins (they follow the items in the array); parts of cut rows; kind
- * The array, copied to the device, serves every call with these lengths, heads, element size and `causal`, from any
+ * The array, copied to the device, serves every call with these lengths, heads, element size, head size and `causal`, from any
  * stream, until the lengths change.  faith_attention needs parts * kv_heads * (kind ? 32 : 128) * (size rounded up to
  * a multiple of 32, + 4) floats of scratch, which calls that may overlap must not share.
  */
@@ -663,7 +663,7 @@ int faith_convolution_verification(const float *x_lb, const float *x_ub,
 #define FAITH_ATTENTION_GRAD_QUERIES  1
 #define FAITH_ATTENTION_GRAD_KEYS     2
 int faith_attention_plan(const int *query_lengths, const int *key_lengths, int sequences, int heads, int kv_heads,
-                         int element_size, int causal, int pass, int *items, long long capacity, long long *counts);
+                         int element_size, int size, int causal, int pass, int *items, long long capacity, long long *counts);
 
 /*
  * out = softmax(scale * q k^T) v over packed sequences; head h uses key head h / (heads / kv_heads).
@@ -684,13 +684,14 @@ int faith_attention(const void *q, const void *k, const void *v, void *out, floa
 /*
  * Gradients of faith_attention.  lse: as the forward call wrote it; strides: [16] token and head strides (elements) of
  * dout, q, k, v, out, dq, dk, dv in this order, under the conditions of faith_attention; stat: 2 * heads * lse_head_stride
- * floats of scratch that calls which may overlap must not share; the items of the passes FAITH_ATTENTION_GRAD_QUERIES and
- * _GRAD_KEYS.  Two launches, no atomics: the same bits on every call.  A row that sees no key has dq = 0, a key that no
+ * floats of scratch that calls which may overlap must not share; the items and kinds of the passes
+ * FAITH_ATTENTION_GRAD_QUERIES and _GRAD_KEYS.  Two launches, no atomics: the same bits on every call.  A row that sees no key has dq = 0, a key that no
  * query sees dk = dv = 0; what masked places hold does not matter.
  */
 int faith_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
                              void *dq, void *dk, void *dv, float *stat, const int *query_items, int n_query_items,
-                             const int *key_items, int n_key_items, const long long *strides, long long lse_head_stride,
+                             int query_kind, const int *key_items, int n_key_items, int key_kind, const long long *strides,
+                             long long lse_head_stride,
                              int heads, int kv_heads, int size, int dtype, int causal, float scale, void *stream);
 
 /*

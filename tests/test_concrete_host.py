@@ -9,10 +9,10 @@ import torch
 from faith_amd import _lib, concrete, forward, ops
 
 
-def plan(lengths, key_lengths, heads, kv_heads, element_size, causal, which):
+def plan(lengths, key_lengths, heads, kv_heads, element_size, causal, which, size=64):
     n = len(lengths)
     ql, kl, counts = (ctypes.c_int * n)(*lengths), (ctypes.c_int * n)(*key_lengths), (ctypes.c_longlong * 4)()
-    args = (ctypes.addressof(ql), ctypes.addressof(kl), n, heads, kv_heads, element_size, int(causal), which)
+    args = (ctypes.addressof(ql), ctypes.addressof(kl), n, heads, kv_heads, element_size, size, int(causal), which)
     _lib.call("faith_attention_plan", *args, None, 0, ctypes.addressof(counts))
     total = counts[0] + counts[1]
     out = torch.full((total + 1, 8), -7, dtype=torch.int32)
@@ -23,7 +23,7 @@ def plan(lengths, key_lengths, heads, kv_heads, element_size, causal, which):
 
 
 CASES = [([5], [5], 4, 4), ([1, 1, 1], [700, 3, 65], 8, 2), ([130, 0, 7], [300, 5, 0], 2, 1), ([40, 9], [10, 9], 3, 1),
-         ([1], [8192], 32, 8), ([1000, 33], [1000, 33], 12, 4), ([128], [16384], 8, 1), ([1] * 70, list(range(70)), 4, 4)]
+         ([1], [8192], 32, 8), ([4096] * 9, [4096] * 9, 8, 8), ([1000, 33], [1000, 33], 12, 4), ([128], [16384], 8, 1), ([1] * 70, list(range(70)), 4, 4)]
 
 
 @pytest.mark.parametrize("lengths, key_lengths, heads, kv_heads", CASES)
@@ -32,7 +32,9 @@ CASES = [([5], [5], 4, 4), ([1, 1, 1], [700, 3, 65], 8, 2), ([130, 0, 7], [300, 
 def test_forward_items_cover_every_row_and_key_once(lengths, key_lengths, heads, kv_heads, causal, element_size):
     items, joins, slots, kind = plan(lengths, key_lengths, heads, kv_heads, element_size, causal, _lib.ATTENTION_FORWARD)
     group, rows_per = heads // kv_heads, 32 if kind else 128
-    assert kind == (max(lengths) * group <= 32)
+    # 256 compute units without a GPU
+    tall = sum((n * group + 127) // 128 for n in lengths) * kv_heads
+    assert bool(kind) == (max(lengths) * group <= 32 or (tall <= 128 and element_size == 4 and max(key_lengths) <= 128))
     spans, used = {}, []
     for qs, ql, ks, kl, row0, begin, end, slot in items:
         spans.setdefault((qs, ql, ks, kl, row0), []).append((begin, end, slot))
@@ -57,12 +59,14 @@ def test_forward_items_cover_every_row_and_key_once(lengths, key_lengths, heads,
                 assert sorted(p[2] for p in parts) == list(range(first, first + n_parts))
         a, b = a + n, b + m
     assert not spans
+    if kind == 2:                       # one turn each: no item has more tiles of 32 keys than there are wavefronts
+        assert all(end - begin <= 4 * 32 for _, _, _, _, _, begin, end, _ in items)
 
 
 @pytest.mark.parametrize("lengths, key_lengths, heads, kv_heads", CASES)
 @pytest.mark.parametrize("causal", [False, True])
 def test_key_items_cover_every_key_and_every_query_that_sees_it(lengths, key_lengths, heads, kv_heads, causal):
-    items, joins, slots, _ = plan(lengths, key_lengths, heads, kv_heads, 2, causal, _lib.ATTENTION_GRAD_KEYS)
+    items, joins, slots, kind = plan(lengths, key_lengths, heads, kv_heads, 2, causal, _lib.ATTENTION_GRAD_KEYS)
     assert not joins and not slots
     seen = set()
     for qs, ql, ks, kl, key0, begin, end, slot in items:
@@ -73,7 +77,7 @@ def test_key_items_cover_every_key_and_every_query_that_sees_it(lengths, key_len
     b = 0
     want = set()
     for m in key_lengths:
-        want |= {(b, m, key0) for key0 in range(0, m, 128)}
+        want |= {(b, m, key0) for key0 in range(0, m, 32 if kind else 128)}
         b += m
     assert seen == want
 
@@ -89,16 +93,17 @@ def test_plan_refuses_what_it_cannot_lay_down():
     one, counts = (ctypes.c_int * 1)(4), (ctypes.c_longlong * 4)()
     p, c = ctypes.addressof(one), ctypes.addressof(counts)
     ok = lambda *a: L.faith_attention_plan(*a)
-    assert ok(None, p, 1, 4, 4, 2, 0, 0, None, 0, c) == -1
-    assert ok(p, p, 0, 4, 4, 2, 0, 0, None, 0, c) == -2
-    assert ok(p, p, 1, 4, 3, 2, 0, 0, None, 0, c) == -2
-    assert ok(p, p, 1, 4, 4, 3, 0, 0, None, 0, c) == -3
-    assert ok(p, p, 1, 4, 4, 2, 0, 9, None, 0, c) == -3
+    assert ok(None, p, 1, 4, 4, 2, 64, 0, 0, None, 0, c) == -1
+    assert ok(p, p, 0, 4, 4, 2, 64, 0, 0, None, 0, c) == -2
+    assert ok(p, p, 1, 4, 3, 2, 64, 0, 0, None, 0, c) == -2
+    assert ok(p, p, 1, 4, 4, 3, 64, 0, 0, None, 0, c) == -3
+    assert ok(p, p, 1, 4, 4, 2, 64, 0, 9, None, 0, c) == -3
+    assert ok(p, p, 1, 4, 4, 2, 129, 0, 0, None, 0, c) == -3
     one[0] = -1
-    assert ok(p, p, 1, 4, 4, 2, 0, 0, None, 0, c) == -2
+    assert ok(p, p, 1, 4, 4, 2, 64, 0, 0, None, 0, c) == -2
     one[0] = 400
-    room = (ctypes.c_int * 8)()
-    assert ok(p, p, 1, 4, 4, 2, 0, 0, ctypes.addressof(room), 1, c) == -2 and b"room" in L.faith_last_error()
+    room = (ctypes.c_int * 8)()          # one item; 400 rows of each of four heads are more
+    assert ok(p, p, 1, 4, 4, 2, 64, 0, 0, ctypes.addressof(room), 1, c) == -2 and b"room" in L.faith_last_error()
 
 
 def test_entry_points_check_on_the_host():
@@ -114,15 +119,15 @@ def test_entry_points_check_on_the_host():
     assert forward_call(q=None) == -1 and forward_call(items=None) == -1 and forward_call(joins=1) == -1
     assert forward_call(k=None) == -4 and forward_call(q=p + 4) == -4 and forward_call(ts=8) == -4 and forward_call(hs=2) == -4 and forward_call(ts=1 << 22) == -4
     assert forward_call(size=18) == -3 and forward_call(size=132) == -3 and forward_call(size=4, dtype=1) == -3
-    assert forward_call(dtype=3) == -3 and forward_call(kind=2) == -3 and forward_call(scale=0.0) == -3 and forward_call(scale=math.nan) == -3
+    assert forward_call(dtype=3) == -3 and forward_call(kind=3) == -3 and forward_call(scale=0.0) == -3 and forward_call(scale=math.nan) == -3
     assert forward_call(kv_heads=3) == -2
     strides = (ctypes.c_longlong * 16)(*[64, 16] * 8)
 
-    def backward_call(t=p, lse=p, stat=p, n=1, s=ctypes.addressof(strides), size=16, scale=0.5):
-        return L.faith_attention_backward(t, t, t, t, t, lse, t, t, t, stat, p, n, p, n, s, 4, 4, 4, size, 0, 0, scale, None)
+    def backward_call(t=p, lse=p, stat=p, n=1, s=ctypes.addressof(strides), size=16, scale=0.5, kind=1):
+        return L.faith_attention_backward(t, t, t, t, t, lse, t, t, t, stat, p, n, kind, p, n, 0, s, 4, 4, 4, size, 0, 0, scale, None)
     assert backward_call(n=0) == 0
     assert backward_call(t=None) == -1 and backward_call(lse=None) == -1 and backward_call(stat=None) == -1 and backward_call(s=None) == -1
-    assert backward_call(t=p + 4) == -4 and backward_call(size=130) == -3 and backward_call(scale=-1.0) == -3
+    assert backward_call(t=p + 4) == -4 and backward_call(size=130) == -3 and backward_call(scale=-1.0) == -3 and backward_call(kind=4) == -3
 
     def norm_call(x=p, y=p, rows=1, n=8, kind=0, dtype=0, bits=0, scales=p, eps=1e-6):
         return L.faith_residual_norm(x, None, None, None, y, None, None, scales, rows, n, kind, dtype, bits, eps, None)

@@ -148,7 +148,7 @@ def test_few_rows_against_many_keys(kv_heads, heads, lengths, keys, dtype):
     from faith_amd import _lib, ops
     q, k, v, _ = tensors(lengths, keys, heads, kv_heads, 128, dtype, 4)
     packing = ops.Packing(lengths, keys)
-    assert packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), True)[3] > 0
+    assert packing.plan(_lib.ATTENTION_FORWARD, heads, kv_heads, q.element_size(), 128, True)[3] > 0
     out, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
     r = R.attention(q, k, v, lengths, keys, True, 1 / math.sqrt(128))
     R.check("out", out, r["out"], r["out_tol"])
