@@ -72,7 +72,7 @@ SIGNATURES = {
     "faith_residual_norm_backward": [_P] * 9 + [ctypes.c_longlong] + [_I] * 3 + [_P],
     "faith_attention_plan": [_P, _P] + [_I] * 7 + [_P, ctypes.c_longlong, _P],
     "faith_attention": [_P] * 7 + [_I] * 3 + [ctypes.c_longlong] * 9 + [_I] * 5 + [_F, _P],
-    "faith_attention_backward": [_P] * 11 + [_I, _I, _P, _I, _I, _P, ctypes.c_longlong] + [_I] * 5 + [_F, _P],
+    "faith_attention_backward": [_P] * 12 + [_I, _I, _P] + [_I] * 4 + [_P, ctypes.c_longlong] + [_I] * 5 + [_F, _P],
 }
 
 

@@ -69,7 +69,7 @@ __device__ void one_row(const FwdArgs &g, const Item &it, int hk, const T *qrow,
 }
 
 template <class T, int DP, int BN, int KIND, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS && DP * sizeof(T) >= 192 ? 1 : 2) attention_forward(const FwdArgs g) {
+__global__ void __launch_bounds__(64 * WAVES, (KIND == KIND_KEYS && DP * sizeof(T) >= 192) || (KIND == KIND_ONCE && DP * sizeof(T) >= 512) ? 1 : 2) attention_forward(const FwdArgs g) {
     constexpr bool KEYS = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
     constexpr int TILE = BN * DP, ALL = TILE * (KEYS ? WAVES : 1);
     typedef Stager<T, DP, BN, KEYS ? 1 : 4> St;                     // keys: read by rows
@@ -376,6 +376,8 @@ struct Plan {
 //             workgroups) would take 33 instead of 21
 //   forward   there too, in fp32, if none has a second turn: 30 sequences of 128, 4 heads of 64 11.2 us instead of 13.4.  With
 //             more keys, or 2-byte elements, 128 rows and cut keys are faster (1000 tokens as above: 18 against 28).
+// The gradients of keys are cut by the heads of the group where there are fewer workgroups of 128 keys than the device holds:
+// 4096 tokens, 8 heads on one key head, 198 instead of 435 us.
 // The forward pass cuts an item's keys where there are fewer items than the device holds workgroups: into parts of equal
 // length, as many as make up that number, none under 256 keys.
 Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int element_size, int size, int causal, int pass) {
@@ -391,6 +393,11 @@ Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int
         tall += (rows + 127) / 128 * kv_heads;
         keys_most = std::max(keys_most, kl[b]);
     }
+    int by_heads = 1;                        // parts of the group
+    if (pass == FAITH_ATTENTION_GRAD_KEYS && tall > 0) {
+        by_heads = (int)std::max<long long>(1, std::min<long long>(group, 2LL * cus / tall));
+        tall *= by_heads;
+    }
     if (most <= 32 || (2 * tall <= cus && (pass != FAITH_ATTENTION_FORWARD || (element_size == 4 && keys_most <= 32 * waves)))) p.kind = KIND_KEYS;
     const int rows_per = p.kind == KIND_KEYS ? 32 : 128, bn = p.kind == KIND_KEYS || element_size == 4 ? 32 : 64;
     for (int b = 0; b < n; ++b) {
@@ -399,7 +406,17 @@ Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int
             for (int key0 = 0; key0 < kl[b]; key0 += rows_per) {
                 // the first token that sees a key of the tile
                 const int begin = causal ? std::min(ql[b], std::max(0, key0 - shift)) : 0;
-                p.items.push_back({(int)qs, ql[b], (int)ks, kl[b], key0, begin / 32 * 32, ql[b], -1});
+                const Item it = {(int)qs, ql[b], (int)ks, kl[b], key0, begin / 32 * 32, ql[b], -1};
+                if (by_heads == 1) { p.items.push_back(it); continue; }
+                Item j = it;
+                j.begin = by_heads;
+                j.end = 0;
+                j.slot = p.slots;
+                p.joins.push_back(j);
+                for (int i = 0; i < by_heads; ++i) {
+                    p.items.push_back(it);
+                    p.items.back().slot = p.slots++;
+                }
             }
         } else {
             const long long rows = (long long)ql[b] * group;
@@ -441,7 +458,7 @@ Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int
     }
     if (p.kind == KIND_KEYS) {
         // tiles of an item, as many of which as there are wavefronts are worked on at once
-        const int times = pass == FAITH_ATTENTION_GRAD_KEYS ? group : 1;
+        const int times = pass == FAITH_ATTENTION_GRAD_KEYS ? (group + by_heads - 1) / by_heads : 1;
         const bool once = std::all_of(p.items.begin(), p.items.end(), [&](const Item &it) { return (long long)((it.end - it.begin + 31) / 32) * times <= waves; });
         if (once) p.kind = KIND_ONCE;
     }

@@ -17,10 +17,11 @@ struct GradArgs {
     const float *lse;
     void *dq, *dk, *dv;
     float *stat;                             // [2][heads][lse_hs]: lse in powers of two, delta
+    float *part;                             // [slots][key heads][keys of an item][2 DP]: parts of dk and dv
     const Item *items;
     Deal deal;
     long long do_ts, do_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, dq_ts, dq_hs, dk_ts, dk_hs, dv_ts, dv_hs, lse_hs;
-    int group, kv_heads, size, causal;
+    int group, kv_heads, size, causal, parts;
     float c, scale;                          // scale * log2(e); scale
 };
 
@@ -202,12 +203,15 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
     St qs, ds;
     qs.init(lane, staged, g.size, g.q_ts);
     ds.init(lane, staged, g.size, g.do_ts);
-    const int span = it.end - it.begin, tiles = (span + BQ - 1) / BQ, total = span > 0 ? tiles * g.group : 0;
+    const int span = it.end - it.begin, tiles = (span + BQ - 1) / BQ;
+    // the heads of the group that this item takes: all of them, or those of one part
+    const int per_part = (g.group + g.parts - 1) / g.parts, h_first = it.slot < 0 ? 0 : it.slot % g.parts * per_part;
+    const int h_count = it.slot < 0 ? g.group : g.group - h_first < per_part ? g.group - h_first : per_part, total = span > 0 ? tiles * h_count : 0;
     const long long stat_hs = (long long)g.kv_heads * g.group * g.lse_hs;
 
-    // the queries of head h of the group from token t on
+    // the queries of the item's head h from token t on
     auto stage_at = [&](T *qt, T *dt, float *lt, float *et, int h, int t) {
-        const int head = hk * g.group + h, left = it.q_len - t;
+        const int head = hk * g.group + h_first + h, left = it.q_len - t;
         qs.load(qt + own, at<T>(g.q, it.q_start + t, g.q_ts, head, g.q_hs), left, g.size, staged);
         ds.load(dt + own, at<T>(g.dout, it.q_start + t, g.do_ts, head, g.do_hs), left, g.size, staged);
         const float *s = g.stat + (long long)head * g.lse_hs + it.q_start + t;
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
     if (g.causal && (any_not_finite<DP>(dk) || any_not_finite<DP>(dv))) {
         clear<DP>(dk);
         clear<DP>(dv);
-        for (int h = hk * g.group; h < (hk + 1) * g.group; ++h)
+        for (int h = hk * g.group + h_first; h < hk * g.group + h_first + h_count; ++h)
             for (int i = first > 0 ? first : 0; i < it.q_len; ++i) {
                 const long long place = it.q_start + i;
                 const T *qr = at<T>(g.q, place, g.q_ts, h, g.q_hs), *dr = at<T>(g.dout, place, g.do_ts, h, g.do_hs);
@@ -302,11 +306,39 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
             }
     }
     if (key >= it.k_len) return;
+    if (it.slot >= 0) {
+        constexpr int ROWS = SPLIT ? 32 : 128;
+        float *p = g.part + ((long long)(it.slot * g.kv_heads + hk) * ROWS + (key - it.row0)) * (2 * DP);
+        store_column<float, DP>(p, dk, 1.f, half, DP);
+        store_column<float, DP>(p + DP, dv, 1.f, half, DP);
+        return;
+    }
     store_column<T, DP>(const_cast<T *>(at<T>(g.dk, it.k_start + key, g.dk_ts, hk, g.dk_hs)), dk, g.scale, half, g.size);
     store_column<T, DP>(const_cast<T *>(at<T>(g.dv, it.k_start + key, g.dv_ts, hk, g.dv_hs)), dv, 1.f, half, g.size);
 }
 
-struct Items { const Item *items; int n, kind; };
+// Adds up the parts of an item's keys in their order; a wavefront to a key.  {-, -, first key of the sequence, its keys, first key
+// of the item, parts, -, first slot}
+template <class T, int DP, int ROWS>
+__global__ void __launch_bounds__(256) attention_grad_join(const GradArgs g, const Item *joins) {
+    const Item it = joins[blockIdx.x];
+    const int hk = blockIdx.y, lane = threadIdx.x & 63, i = blockIdx.z * 4 + (threadIdx.x >> 6), key = it.row0 + i;
+    if (key >= it.k_len) return;
+    const long long step = (long long)g.kv_heads * ROWS * (2 * DP);
+    const float *p = g.part + ((long long)(it.slot * g.kv_heads + hk) * ROWS + i) * (2 * DP);
+    T *dk = const_cast<T *>(at<T>(g.dk, it.k_start + key, g.dk_ts, hk, g.dk_hs)), *dv = const_cast<T *>(at<T>(g.dv, it.k_start + key, g.dv_ts, hk, g.dv_hs));
+    for (int d = lane; d < g.size; d += 64) {
+        float a = 0.f, b = 0.f;
+        for (int s = 0; s < it.begin; ++s) {
+            a += p[s * step + d];
+            b += p[s * step + DP + d];
+        }
+        dk[d] = (T)(a * g.scale);
+        dv[d] = (T)b;
+    }
+}
+
+struct Items { const Item *items; int n, kind, joins; };
 
 template <class T, int DP> int launch_backward(GradArgs g, const Items &qi, const Items &ki, hipStream_t stream) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32, BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32, W = split_waves<T, DP>();
@@ -324,6 +356,9 @@ template <class T, int DP> int launch_backward(GradArgs g, const Items &qi, cons
         if (ki.kind == KIND_ONCE) hipLaunchKernelGGL((attention_grad_keys<T, DP, 32, KIND_ONCE, W>), dim3(grid), dim3(64 * W), 0, stream, g);
         else if (ki.kind == KIND_KEYS) hipLaunchKernelGGL((attention_grad_keys<T, DP, 32, KIND_KEYS, W>), dim3(grid), dim3(64 * W), 0, stream, g);
         else hipLaunchKernelGGL((attention_grad_keys<T, DP, BQ, KIND_ROWS, 4>), dim3(grid), dim3(256), 0, stream, g);
+        const Item *joins = ki.items + ki.n;
+        if (ki.joins > 0 && ki.kind == KIND_ROWS) hipLaunchKernelGGL((attention_grad_join<T, DP, 128>), dim3(ki.joins, g.kv_heads, 32), dim3(256), 0, stream, g, joins);
+        else if (ki.joins > 0) hipLaunchKernelGGL((attention_grad_join<T, DP, 32>), dim3(ki.joins, g.kv_heads, 8), dim3(256), 0, stream, g, joins);
     }
     return check_launch("faith_attention_backward");
 }
@@ -337,14 +372,17 @@ template <class T> int launch_backward(const GradArgs &g, const Items &qi, const
 }  // namespace
 
 extern "C" int faith_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
-                                        void *dq, void *dk, void *dv, float *stat, const int *query_items, int n_query_items,
-                                        int query_kind, const int *key_items, int n_key_items, int key_kind, const long long *strides, long long lse_head_stride,
+                                        void *dq, void *dk, void *dv, float *stat, float *parts,
+                                        const int *query_items, int n_query_items, int query_kind, const int *key_items,
+                                        int n_key_items, int n_key_joins, int key_parts, int key_kind, const long long *strides, long long lse_head_stride,
                                         int heads, int kv_heads, int size, int dtype, int causal, float scale, void *stream) {
     FAITH_REQUIRE(n_query_items >= 0 && n_key_items >= 0, FAITH_ERR_SHAPE, "%s: %d and %d items", __func__, n_query_items, n_key_items);
     if (n_query_items == 0 && n_key_items == 0) return FAITH_OK;
     FAITH_REQUIRE(query_kind >= KIND_ROWS && query_kind <= KIND_ONCE && key_kind >= KIND_ROWS && key_kind <= KIND_ONCE, FAITH_ERR_UNSUPPORTED,
                   "%s: kinds %d and %d", __func__, query_kind, key_kind);
     FAITH_NOT_NULL(strides);
+    FAITH_REQUIRE(n_key_joins >= 0 && key_parts >= 0 && (n_key_joins == 0 || key_parts > 0), FAITH_ERR_SHAPE, "%s: %d joins of %d parts", __func__, n_key_joins, key_parts);
+    FAITH_REQUIRE(n_key_joins == 0 || parts, FAITH_ERR_NULL, "%s: keys are worked on in parts, and there is no room for their results", __func__);
     const int rc = attention_shapes(__func__, heads, kv_heads, size, dtype, scale);
     if (rc != FAITH_OK) return rc;
     const int es = dtype == FAITH_F32 ? 4 : 2;
@@ -358,13 +396,16 @@ extern "C" int faith_attention_backward(const void *dout, const void *q, const v
     FAITH_REQUIRE(n_query_items == 0 || (lse && stat && query_items), FAITH_ERR_NULL, "%s: lse, stat or the query items are NULL", __func__);
     FAITH_REQUIRE(n_key_items == 0 || key_items, FAITH_ERR_NULL, "%s: the key items are NULL", __func__);
     GradArgs g;
-    g.dout = dout; g.q = q; g.k = k; g.v = v; g.out = out; g.lse = lse; g.dq = dq; g.dk = dk; g.dv = dv; g.stat = stat;
+    g.dout = dout; g.q = q; g.k = k; g.v = v; g.out = out; g.lse = lse; g.dq = dq; g.dk = dk; g.dv = dv; g.stat = stat; g.part = parts;
     long long *to[16] = {&g.do_ts, &g.do_hs, &g.q_ts, &g.q_hs, &g.k_ts, &g.k_hs, &g.v_ts, &g.v_hs, &g.o_ts, &g.o_hs, &g.dq_ts, &g.dq_hs, &g.dk_ts, &g.dk_hs, &g.dv_ts, &g.dv_hs};
     for (int i = 0; i < 16; ++i) *to[i] = strides[i];
     g.lse_hs = lse_head_stride;
     g.group = heads / kv_heads; g.kv_heads = kv_heads; g.size = size; g.causal = causal;
     g.c = scale * 1.4426950408889634f; g.scale = scale;
-    const Items qi = {reinterpret_cast<const Item *>(query_items), n_query_items, query_kind}, ki = {reinterpret_cast<const Item *>(key_items), n_key_items, key_kind};
+    // every item is cut into as many parts
+    g.parts = n_key_joins > 0 ? key_parts / n_key_joins : 1;
+    const Items qi = {reinterpret_cast<const Item *>(query_items), n_query_items, query_kind, 0};
+    const Items ki = {reinterpret_cast<const Item *>(key_items), n_key_items, key_kind, n_key_joins};
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == FAITH_F32) return launch_backward<float>(g, qi, ki, s);
     if (dtype == FAITH_BF16) return launch_backward<__bf16>(g, qi, ki, s);

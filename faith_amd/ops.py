@@ -1333,23 +1333,25 @@ def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=Non
         strides = (ctypes.c_longlong * 16)(*ds, *qs, *ks, *vs, *os_, *row, *kv_row, *kv_row)
         with _on(q.device):
             plans = [packing.plan(which, heads, kv_heads, q.element_size(), size, causal) for which in (_lib.ATTENTION_GRAD_QUERIES, _lib.ATTENTION_GRAD_KEYS)]
-        known = (plans, heads, (plans[0][1], plans[0][2], plans[0][5], plans[1][1], plans[1][2], plans[1][5], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
+        floats = plans[1][4] * kv_heads * (32 if plans[1][5] else 128) * 2 * ((size + 31) // 32 * 32)
+        known = (plans, floats, heads, (plans[0][1], plans[0][2], plans[0][5], *plans[1][1:6], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
                                 size, _DTYPES[q.dtype], int(causal), _scale(scale, size)), strides)
         if key is not None and dout.shape == q.shape and out.shape == q.shape:
             packing._calls[key] = known
-    plans, heads, rest, _ = known
+    plans, floats, heads, rest, _ = known
     _check("lse", lse, (heads, packing.tokens))
     dev = packing.device
     if lse.get_device() != dev.index:
         raise ValueError(f"lse: lives on {lse.device}, the other operands on {dev}")
     dq, dk, dv = _like_rows(q, packing.tokens), _like_rows(k, packing.keys), _like_rows(v, packing.keys)
     stat = _empty(2, heads, packing.tokens, device=dev)
+    parts = _empty(floats, device=dev) if floats else None
     stream = _stream(q)
     packing._used_on(plans[0], stream)
     packing._used_on(plans[1], stream)
     with _on(dev):
         _lib.call("faith_attention_backward", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stat.data_ptr(), *rest, stream)
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stat.data_ptr(), _ptr(parts), *rest, stream)
     return dq, dk, dv
 
 

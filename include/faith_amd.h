@@ -684,14 +684,15 @@ int faith_attention(const void *q, const void *k, const void *v, void *out, floa
 /*
  * Gradients of faith_attention.  lse: as the forward call wrote it; strides: [16] token and head strides (elements) of
  * dout, q, k, v, out, dq, dk, dv in this order, under the conditions of faith_attention; stat: 2 * heads * lse_head_stride
- * floats of scratch that calls which may overlap must not share; the items and kinds of the passes
- * FAITH_ATTENTION_GRAD_QUERIES and _GRAD_KEYS.  Two launches, no atomics: the same bits on every call.  A row that sees no key has dq = 0, a key that no
+ * floats of scratch that calls which may overlap must not share; the items, kinds, joins and parts of the passes
+ * FAITH_ATTENTION_GRAD_QUERIES and _GRAD_KEYS; parts: key_parts * kv_heads * (key_kind ? 32 : 128) * 2 * (size rounded up to a
+ * multiple of 32) floats of scratch, NULL without joins.  Two launches (three with joins), no atomics: the same bits on every call.  A row that sees no key has dq = 0, a key that no
  * query sees dk = dv = 0; what masked places hold does not matter.
  */
 int faith_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
-                             void *dq, void *dk, void *dv, float *stat, const int *query_items, int n_query_items,
-                             int query_kind, const int *key_items, int n_key_items, int key_kind, const long long *strides,
-                             long long lse_head_stride,
+                             void *dq, void *dk, void *dv, float *stat, float *parts, const int *query_items,
+                             int n_query_items, int query_kind, const int *key_items, int n_key_items, int n_key_joins,
+                             int key_parts, int key_kind, const long long *strides, long long lse_head_stride,
                              int heads, int kv_heads, int size, int dtype, int causal, float scale, void *stream);
 
 /*

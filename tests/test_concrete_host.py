@@ -67,19 +67,25 @@ def test_forward_items_cover_every_row_and_key_once(lengths, key_lengths, heads,
 @pytest.mark.parametrize("causal", [False, True])
 def test_key_items_cover_every_key_and_every_query_that_sees_it(lengths, key_lengths, heads, kv_heads, causal):
     items, joins, slots, kind = plan(lengths, key_lengths, heads, kv_heads, 2, causal, _lib.ATTENTION_GRAD_KEYS)
-    assert not joins and not slots
-    seen = set()
+    group = heads // kv_heads
+    tall = sum((m + 127) // 128 for m in key_lengths) * kv_heads
+    parts = max(1, min(group, 512 // tall))                      # 256 compute units without a GPU
+    assert len(joins) == (len(items) // parts if parts > 1 else 0) and slots == (len(items) if parts > 1 else 0)
+    seen = {}
     for qs, ql, ks, kl, key0, begin, end, slot in items:
-        assert slot == -1 and end == ql and 0 <= begin
         first = max(0, key0 - (kl - ql)) if causal else 0       # the first query that sees the tile's first key
-        assert begin <= first
-        seen.add((ks, kl, key0))
+        assert begin <= first and 0 <= begin and end == ql
+        seen.setdefault((ks, kl, key0), []).append(slot)
+    for j in joins:
+        assert j[5] == parts and j[7] % parts == 0 and sorted(seen[j[2], j[3], j[4]]) == list(range(j[7], j[7] + parts))
+    if parts == 1:
+        assert all(v == [-1] for v in seen.values())
     b = 0
     want = set()
     for m in key_lengths:
         want |= {(b, m, key0) for key0 in range(0, m, 32 if kind else 128)}
         b += m
-    assert seen == want
+    assert set(seen) == want
 
 
 def test_items_are_laid_down_longest_first():
@@ -123,11 +129,12 @@ def test_entry_points_check_on_the_host():
     assert forward_call(kv_heads=3) == -2
     strides = (ctypes.c_longlong * 16)(*[64, 16] * 8)
 
-    def backward_call(t=p, lse=p, stat=p, n=1, s=ctypes.addressof(strides), size=16, scale=0.5, kind=1):
-        return L.faith_attention_backward(t, t, t, t, t, lse, t, t, t, stat, p, n, kind, p, n, 0, s, 4, 4, 4, size, 0, 0, scale, None)
+    def backward_call(t=p, lse=p, stat=p, n=1, s=ctypes.addressof(strides), size=16, scale=0.5, kind=1, joins=0):
+        return L.faith_attention_backward(t, t, t, t, t, lse, t, t, t, stat, None, p, n, kind, p, n, joins, 0, 0, s, 4, 4, 4, size, 0, 0, scale, None)
     assert backward_call(n=0) == 0
     assert backward_call(t=None) == -1 and backward_call(lse=None) == -1 and backward_call(stat=None) == -1 and backward_call(s=None) == -1
     assert backward_call(t=p + 4) == -4 and backward_call(size=130) == -3 and backward_call(scale=-1.0) == -3 and backward_call(kind=4) == -3
+    assert backward_call(joins=-1) == -2 and backward_call(joins=2) == -2
 
     def norm_call(x=p, y=p, rows=1, n=8, kind=0, dtype=0, bits=0, scales=p, eps=1e-6):
         return L.faith_residual_norm(x, None, None, None, y, None, None, scales, rows, n, kind, dtype, bits, eps, None)

@@ -21,6 +21,9 @@ SHAPES = [  # lengths, key lengths (None: alike), heads, key heads, causal
     ([70], [5000], 4, 2, False),
     ([1], [1], 1, 1, True),
     ([31, 64, 129], [63, 64, 127], 2, 2, False),
+    ([200, 33], None, 10, 2, True),               # gradients of keys in parts of the group
+    ([2100, 1500], None, 6, 3, True),
+    ([300] * 40, None, 4, 4, False),              # workgroups of 128 rows in every pass
 ]
 
 
