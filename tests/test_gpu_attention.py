@@ -134,6 +134,28 @@ def test_masked_places_may_hold_anything(dtype, bad, lengths, keys):
     R.check("dv", dv[seen:], r["dv"][seen:], r["dv_tol"][seen:])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("lengths, keys, causal", [([1] * 9, [1] * 9, False), ([1, 1], [1, 1], True), ([70, 300], [1, 1], False), ([40, 5], [40, 5], True), ([5], [3], True)])
+def test_a_query_that_sees_one_key_has_no_gradient_through_its_score(dtype, lengths, keys, causal):
+    """Its probability is 1 whatever the score: dq is zero, and it adds nothing to dk, not merely little."""
+    from faith_amd import ops
+    q, k, v, dout = tensors(lengths, keys, 4, 2, 64, dtype, 12)
+    packing = ops.Packing(lengths, keys)
+    out, lse = ops.attention(q, k, v, packing, causal=causal, return_lse=True)
+    dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing, causal=causal)
+    r = R.attention(q, k, v, lengths, keys, causal, 0.125, dout)
+    for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        R.check(name, got, r[name], r[name + "_tol"])
+    a = 0
+    for n, m in zip(lengths, keys):
+        i = m_only = max(0, n - m)                               # the first query that sees a key
+        alone = dq[a:a + n] if m == 1 else dq[a + i:a + i + 1] if causal else dq[:0]
+        assert bool((alone == 0).all()), m_only
+        a += n
+    if max(keys) == 1:
+        assert bool((dk == 0).all())
+
+
 def test_not_a_number_where_it_is_seen_stays_one():
     from faith_amd import ops
     q, k, v, _ = tensors([40], [40], 1, 1, 32, BF16, 2)
