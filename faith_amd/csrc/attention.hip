@@ -307,36 +307,75 @@ __global__ void __launch_bounds__(64 * WAVES, (KIND == KIND_KEYS && DP * sizeof(
         g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
 }
 
-// Joins the parts of the rows of one item: {first token, tokens, -, -, first row, parts, rows of the item, first slot}; a
-// wavefront to a row, its lanes along the head.
-template <class T, int DP, int ROWS>
+// Joins the parts of the rows of one item: {first token, tokens, -, -, first row, parts, -, first slot}; W wavefronts
+// to a row, taking turns at its parts, their lanes along the head: four for few rows in many parts, one for 128 rows in a few.
+// The order of the sums depends on the number of parts only.
+template <class T, int DP, int ROWS, int W>
 __global__ void __launch_bounds__(256) attention_join(const FwdArgs g, const Item *joins) {
+    constexpr int N = (DP + 63) / 64;
+    __shared__ float ml[4][2], os[3][64 * N];
     const Item it = joins[blockIdx.x];
     const int hk = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int rows = it.q_len * g.group;
-    for (int i = blockIdx.z * 4 + wave; i < ROWS; i += 4 * gridDim.z) {
-        const int row = it.row0 + i;
-        if (row >= rows) return;
-        const long long step = (long long)g.kv_heads * ROWS * (DP + 4);
+    const int rows = it.q_len * g.group, parts = it.begin;
+    const long long step = (long long)g.kv_heads * ROWS * (DP + 4);
+    const int turn = W == 1 ? 0 : wave;
+    for (int i = W == 1 ? blockIdx.z * 4 + wave : blockIdx.z; i < ROWS && it.row0 + i < rows; i += (W == 1 ? 4 : 1) * gridDim.z) {
         const float *p = g.part + ((long long)(it.slot * g.kv_heads + hk) * ROWS + i) * (DP + 4);
-        float ref = LOWEST;
-        for (int s = 0; s < it.begin; ++s) ref = __builtin_fmaxf(ref, p[s * step]);
-        float sum = 0.f, o[DP / 32] = {};
-        for (int s = 0; s < it.begin; ++s) {
-            const float f = __builtin_amdgcn_exp2f(p[s * step] - ref);
-            sum = fmaf(p[s * step + 1], f, sum);
+        float ref = LOWEST, sum = 0.f, o[N] = {};
+        // this wavefront's parts, 64 at a time: turn, turn + W, ...
+        for (int s0 = turn; s0 < parts; s0 += 64 * W) {
+            const int mine = s0 + W * lane, n = (parts - s0 + W - 1) / W < 64 ? (parts - s0 + W - 1) / W : 64;
+            const float r = mine < parts ? p[mine * step] : LOWEST, l = mine < parts ? p[mine * step + 1] : 0.f;
+            float now = __builtin_fmaxf(ref, r);
 #pragma unroll
-            for (int e = 0; e < (DP + 63) / 64; ++e)
-                if (64 * e + lane < DP) o[e] = fmaf(p[s * step + 4 + 64 * e + lane], f, o[e]);
+            for (int d = 32; d > 0; d >>= 1) now = __builtin_fmaxf(now, __shfl_xor(now, d));
+            const float old = __builtin_amdgcn_exp2f(ref - now), f = __builtin_amdgcn_exp2f(r - now);
+            float add = mine < parts ? l * f : 0.f;
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) add += __shfl_xor(add, d);
+            sum = fmaf(sum, old, add);
+            ref = now;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] *= old;
+            for (int k = 0; k < n; ++k) {
+                const float w = __shfl(f, k);
+                const float *q = p + (s0 + W * k) * step + 4;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (64 * e + lane < DP) o[e] = fmaf(q[64 * e + lane], w, o[e]);
+            }
         }
+        float now = ref;
+        if constexpr (W > 1) {
+            __syncthreads();                 // the row before has been read
+            if (lane == 0) { ml[wave][0] = ref; ml[wave][1] = sum; }
+            if (wave > 0)
+#pragma unroll
+                for (int e = 0; e < N; ++e) os[wave - 1][64 * e + lane] = o[e];
+            __syncthreads();
+            if (wave > 0) continue;
+#pragma unroll
+            for (int w = 1; w < W; ++w) now = __builtin_fmaxf(now, ml[w][0]);
+            float f = __builtin_amdgcn_exp2f(ref - now);
+            sum *= f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] *= f;
+#pragma unroll
+            for (int w = 1; w < W; ++w) {
+                f = __builtin_amdgcn_exp2f(ml[w][0] - now);
+                sum = fmaf(ml[w][1], f, sum);
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[e] = fmaf(os[w - 1][64 * e + lane], f, o[e]);
+            }
+        }
+        const int row = it.row0 + i, token = row / g.group, head = hk * g.group + (row - token * g.group);
         const float inverse = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        const int token = row / g.group, head = hk * g.group + (row - token * g.group);
         T *dst = reinterpret_cast<T *>(g.out) + (long long)(it.q_start + token) * g.o_ts + (long long)head * g.o_hs;
 #pragma unroll
-        for (int e = 0; e < (DP + 63) / 64; ++e)
+        for (int e = 0; e < N; ++e)
             if (64 * e + lane < g.size) dst[64 * e + lane] = (T)(o[e] * inverse);
         if (g.lse && lane == 0)
-            g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+            g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (now + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
     }
 }
 
@@ -347,8 +386,8 @@ template <class T, int DP> int launch_forward(const FwdArgs &g, int kind, unsign
     else if (kind == KIND_KEYS) hipLaunchKernelGGL((attention_forward<T, DP, 32, KIND_KEYS, WAVES>), dim3(grid), dim3(64 * WAVES), 0, stream, g);
     else hipLaunchKernelGGL((attention_forward<T, DP, BN, KIND_ROWS, 4>), dim3(grid), dim3(256), 0, stream, g);
     if (n_joins > 0) {
-        if (kind != KIND_ROWS) hipLaunchKernelGGL((attention_join<T, DP, 32>), dim3(n_joins, g.kv_heads, 8), dim3(256), 0, stream, g, joins);
-        else hipLaunchKernelGGL((attention_join<T, DP, 128>), dim3(n_joins, g.kv_heads, 32), dim3(256), 0, stream, g, joins);
+        if (kind != KIND_ROWS) hipLaunchKernelGGL((attention_join<T, DP, 32, 4>), dim3(n_joins, g.kv_heads, g.group < 8 ? g.group : 8), dim3(256), 0, stream, g, joins);
+        else hipLaunchKernelGGL((attention_join<T, DP, 128, 1>), dim3(n_joins, g.kv_heads, 32), dim3(256), 0, stream, g, joins);
     }
     return check_launch("faith_attention");
 }
@@ -378,8 +417,10 @@ struct Plan {
 //             more keys, or 2-byte elements, 128 rows and cut keys are faster (1000 tokens as above: 18 against 28).
 // The gradients of keys are cut by the heads of the group where there are fewer workgroups of 128 keys than the device holds:
 // 4096 tokens, 8 heads on one key head, 198 instead of 435 us.
-// The forward pass cuts an item's keys where there are fewer items than the device holds workgroups: into parts of equal
-// length, as many as make up that number, none under 256 keys.
+// The forward pass cuts an item's keys where there are fewer items than compute units: into parts of equal length, as many as
+// make up that number, none under 256 keys.  More parts pay for filling and draining the stages and for the join (4 queries
+// against 30000 keys each, 32 / 8 heads of 128: four times as many 161 us instead of 96), and 128 rows in two parts are slower
+// than whole (10 sequences of 300, 8 heads of 128: 28 against 12 us).
 Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int element_size, int size, int causal, int pass) {
     Plan p;
     long long qs = 0, ks = 0;
@@ -429,17 +470,16 @@ Plan make_plan(const int *ql, const int *kl, int n, int group, int kv_heads, int
         qs += ql[b];
         ks += kl[b];
     }
-    const long long resident = 2LL * cus, blocks = (long long)p.items.size() * kv_heads;
-    if (pass == FAITH_ATTENTION_FORWARD && blocks > 0 && blocks < (p.kind == KIND_KEYS ? 4 : 1) * resident) {
+    const long long blocks = (long long)p.items.size() * kv_heads;
+    if (pass == FAITH_ATTENTION_FORWARD && blocks > 0 && blocks < cus) {
         long long keys = 0;
         for (const Item &it : p.items) keys += it.end;
-        const long long parts = (p.kind == KIND_KEYS ? 4 : 1) * resident;
-        long long chunk = (keys * kv_heads + parts - 1) / parts;
+        long long chunk = (keys * kv_heads + cus - 1) / cus;
         chunk = std::max<long long>((chunk + bn - 1) / bn * bn, 256);
         std::vector<Item> cut;
         for (const Item &it : p.items) {
             const int n_parts = (int)((it.end + chunk - 1) / chunk);
-            if (n_parts <= 1) { cut.push_back(it); continue; }
+            if (n_parts <= (p.kind == KIND_ROWS ? 2 : 1)) { cut.push_back(it); continue; }
             Item j = it;
             j.begin = n_parts;
             j.end = 0;
