@@ -20,6 +20,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -36,6 +37,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         return (*ops.attention_backward(dout.contiguous(), q, k, v, out, lse, *ctx.rest), None, None, None)
@@ -66,6 +68,7 @@ class _ResidualNorm(torch.autograd.Function):
         return y, h if residual is not None else h.detach()
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dsum):
         h, weight, stats = ctx.saved_tensors
         _, with_residual, with_weight, with_bias = ctx.needs_input_grad[:4]
@@ -197,7 +200,7 @@ def _into_ball(d, p, radii):
 
 def falsify(network, embeddings, positions, radii, label, p=2.0, steps=10, batch=None):
     """Searches, for every (position, radius) pair at once, for a perturbation of the embedding at that position, of p-norm at
-    most the radius, with which the network no longer answers `label`: `steps` steps of projected steepest ascent from the
+    most the radius, with which the network no longer answers `label` with a positive margin: `steps` steps of projected steepest ascent from the
     sentence itself.  embeddings [1, L, hidden].  Returns a list of bools; True is a proof, False only that none was found.
 
     A step is one pass forward and backward over as many copies of the sentence as there are pairs.  batch: their Batch,
@@ -205,10 +208,21 @@ def falsify(network, embeddings, positions, radii, label, p=2.0, steps=10, batch
     from .forward import _checked_positions
     if len(radii) != len(positions):
         raise ValueError(f"{len(positions)} positions, {len(radii)} radii")
+    if not p >= 1:
+        raise ValueError(f"p={p}: the perturbation norm must be >= 1")
+    if steps < 0:
+        raise ValueError(f"{steps} steps")
+    for r in radii:
+        if not 0 <= r < math.inf:
+            raise ValueError(f"radius {r!r} is not a radius")
     if not positions:
         return []
     n, length = len(positions), embeddings.shape[1]
     at = [g[0] for g in _checked_positions([[i] for i in positions], length)]
+    classes = network.classifier.weight.shape[0]
+    if label != int(label) or not 0 <= label < classes:
+        raise ValueError(f"label {label!r}: the network answers with one of {classes} classes")
+    label = int(label)
     dev = embeddings.device
     batch = batch or Batch([length] * n, dev)
     if batch.packing.lengths != (length,) * n:

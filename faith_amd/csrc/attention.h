@@ -343,6 +343,14 @@ inline int attention_shapes(const char *fn, int heads, int kv_heads, int size, i
     FAITH_REQUIRE(scale > 0.f && scale < 1e30f, FAITH_ERR_UNSUPPORTED, "%s: the scale must be positive and finite", fn);
     return FAITH_OK;
 }
+// a launch holds fewer than 2^32 threads
+inline bool attention_grid(const char *fn, int n_items, int kv_heads) {
+    unsigned grid;
+    const Deal d = deal(n_items, kv_heads, &grid);
+    if (8LL * (kv_heads / d.heads_apart) * d.items_per_stripe < (1LL << 24)) return true;
+    set_error("%s: %d items of %d key heads are more than one launch holds", fn, n_items, kv_heads);
+    return false;
+}
 // rows in whole 16-byte groups that neither overlap nor lie further apart than a 32-bit offset reaches over one tile
 inline bool attention_rows(const char *fn, const char *name, const void *p, long long token_stride, long long head_stride, int size, int es) {
     const int per = 16 / es;

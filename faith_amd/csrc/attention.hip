@@ -562,6 +562,7 @@ extern "C" int faith_attention(const void *q, const void *k, const void *v, void
     if (!attention_rows(__func__, "q", q, q_token_stride, q_head_stride, size, es) || !attention_rows(__func__, "k", k, k_token_stride, k_head_stride, size, es) ||
         !attention_rows(__func__, "v", v, v_token_stride, v_head_stride, size, es) || !attention_rows(__func__, "out", out, out_token_stride, out_head_stride, size, es))
         return FAITH_ERR_ALIGN;
+    if (!attention_grid(__func__, n_items, kv_heads)) return FAITH_ERR_UNSUPPORTED;
     FwdArgs g;
     unsigned grid;
     g.q = q; g.k = k; g.v = v; g.out = out; g.lse = lse; g.part = parts;

@@ -406,6 +406,7 @@ extern "C" int faith_attention_backward(const void *dout, const void *q, const v
     }
     FAITH_REQUIRE(n_query_items == 0 || (lse && stat && query_items), FAITH_ERR_NULL, "%s: lse, stat or the query items are NULL", __func__);
     FAITH_REQUIRE(n_key_items == 0 || key_items, FAITH_ERR_NULL, "%s: the key items are NULL", __func__);
+    if (!attention_grid(__func__, n_query_items, kv_heads) || !attention_grid(__func__, n_key_items, kv_heads)) return FAITH_ERR_UNSUPPORTED;
     GradArgs g;
     g.dout = dout; g.q = q; g.k = k; g.v = v; g.out = out; g.lse = lse; g.dq = dq; g.dk = dk; g.dv = dv; g.stat = stat; g.part = parts;
     long long *to[16] = {&g.do_ts, &g.do_hs, &g.q_ts, &g.q_hs, &g.k_ts, &g.k_hs, &g.v_ts, &g.v_hs, &g.o_ts, &g.o_hs, &g.dq_ts, &g.dq_hs, &g.dk_ts, &g.dk_hs, &g.dv_ts, &g.dv_hs};

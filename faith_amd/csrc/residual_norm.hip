@@ -495,6 +495,7 @@ extern "C" int faith_residual_norm(const void *x, const void *residual, const vo
     FAITH_REQUIRE(bits == 0 || bits == FAITH_BITS_INT8 || bits == FAITH_BITS_E4M3, FAITH_ERR_UNSUPPORTED, "%s: output %d", __func__, bits);
     FAITH_REQUIRE(eps >= 0.f && eps < 1e30f, FAITH_ERR_UNSUPPORTED, "%s: eps must be finite and not negative", __func__);
     if (rows == 0) return FAITH_OK;
+    FAITH_REQUIRE(rows < (1LL << 24), FAITH_ERR_UNSUPPORTED, "%s: %lld rows are more than one launch holds", __func__, rows);
     FAITH_NOT_NULL(x);
     FAITH_NOT_NULL(y);
     FAITH_REQUIRE(!bits || scales, FAITH_ERR_NULL, "%s: an output in 8 bits has a scale for each row", __func__);
@@ -515,6 +516,7 @@ extern "C" int faith_residual_norm_backward(const void *dy, const void *dsum, co
     const int rc = norm_shapes(__func__, rows, n, kind, dtype);
     if (rc != FAITH_OK) return rc;
     FAITH_REQUIRE(!(dweight || dbias) || partial || rows == 0, FAITH_ERR_NULL, "%s: the parameters' gradients need scratch", __func__);
+    FAITH_REQUIRE(rows < (1LL << 24), FAITH_ERR_UNSUPPORTED, "%s: %lld rows are more than one launch holds", __func__, rows);
     if (rows > 0) {
         FAITH_NOT_NULL(dy);
         FAITH_NOT_NULL(sum);

@@ -320,6 +320,8 @@ def _label(network, embeddings, label):
     if label is not None:
         return label
     from . import concrete
+    if network.classifier.weight.shape[0] != 2:
+        raise ValueError("the propagated margin is that of two classes: with another number the label has to be given")
     (label,) = concrete.predict(network, embeddings)
     return label
 

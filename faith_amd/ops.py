@@ -1311,6 +1311,11 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
     if out is None:
         out = _like_rows(q, packing.tokens)
     lse = _empty(heads, packing.tokens, device=dev) if return_lse else None
+    if not packing.keys:
+        out[:packing.tokens].zero_()             # nothing to look at, and no address of keys to hand over
+        if return_lse:
+            lse.fill_(-math.inf)
+        return (out, lse) if return_lse else out
     scratch = _empty(floats, device=dev) if floats else None
     stream = _stream(q)
     packing._used_on(plan, stream)

@@ -127,6 +127,7 @@ def test_entry_points_check_on_the_host():
     assert forward_call(size=18) == -3 and forward_call(size=132) == -3 and forward_call(size=4, dtype=1) == -3
     assert forward_call(dtype=3) == -3 and forward_call(kind=3) == -3 and forward_call(scale=0.0) == -3 and forward_call(scale=math.nan) == -3
     assert forward_call(kv_heads=3) == -2
+    assert forward_call(n=1 << 27) == -3
     strides = (ctypes.c_longlong * 16)(*[64, 16] * 8)
 
     def backward_call(t=p, lse=p, stat=p, n=1, s=ctypes.addressof(strides), size=16, scale=0.5, kind=1, joins=0):
@@ -140,7 +141,7 @@ def test_entry_points_check_on_the_host():
         return L.faith_residual_norm(x, None, None, None, y, None, None, scales, rows, n, kind, dtype, bits, eps, None)
     assert norm_call(rows=0) == 0
     assert norm_call(x=None) == -1 and norm_call(y=None) == -1 and norm_call(bits=1, scales=None) == -1
-    assert norm_call(n=0) == -2 and norm_call(rows=-1) == -2
+    assert norm_call(n=0) == -2 and norm_call(rows=-1) == -2 and norm_call(rows=1 << 24) == -3
     assert norm_call(kind=3) == -3 and norm_call(dtype=5) == -3 and norm_call(bits=3) == -3 and norm_call(eps=-1.0) == -3 and norm_call(eps=math.nan) == -3
     assert L.faith_residual_norm_backward(p, None, p, None, p, p, p, None, None, 1, 8, 0, 0, None) == -1
     assert L.faith_residual_norm_backward(p, None, p, None, None, p, None, None, None, 1, 8, 0, 0, None) == -1
@@ -188,6 +189,18 @@ def test_concrete_checks_embeddings_and_positions():
     with pytest.raises(ValueError, match="outside"):
         concrete.falsify(None, torch.zeros(1, 4, 8), [4], [0.1], 0)
     assert concrete.falsify(None, torch.zeros(1, 4, 8), [], [], 0) == []
+    from types import SimpleNamespace
+    net = SimpleNamespace(classifier=SimpleNamespace(weight=torch.zeros(2, 8)))
+    emb = torch.zeros(1, 4, 8)
+    for bad, what in ((dict(label=2), "classes"), (dict(label=-1), "classes"), (dict(label=0.5), "classes"), (dict(p=0.5), "norm"), (dict(steps=-1), "steps"),
+                      (dict(radii=[-0.1]), "radius"), (dict(radii=[math.nan]), "radius"), (dict(radii=[math.inf]), "radius"), (dict(p=math.nan), "norm")):
+        args = dict(radii=[0.1], label=0)
+        args.update(bad)
+        with pytest.raises(ValueError, match=what):
+            concrete.falsify(net, emb, [1], **args)
+    net.classifier.weight = torch.zeros(3, 8)
+    with pytest.raises(ValueError, match="two classes"):
+        forward.verify_safety(None, net, emb, 1, 0.1, None)
 
 
 @pytest.mark.parametrize("p", [1.0, 1.5, 2.0, 3.0, math.inf])

@@ -337,3 +337,10 @@ def test_empty_batches():
     assert out.shape == (0, 2, 32) and lse.shape == (2, 0)
     dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing)
     assert dq.shape == (0, 2, 32) and bool((dk == 0).all()) and bool((dv == 0).all())
+    q, k, v, dout = tensors([4, 1], [0, 0], 2, 2, 32, F32)              # queries, and no keys at all
+    packing = ops.Packing([4, 1], [0, 0])
+    for causal in (False, True):
+        out, lse = ops.attention(q, k, v, packing, causal, return_lse=True)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+        dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing, causal)
+        assert bool((dq == 0).all()) and dk.shape == (0, 2, 32) and dv.shape == (0, 2, 32)

@@ -194,3 +194,37 @@ def test_parameters_collect_no_gradients_in_the_search():
     assert net.classifier.weight.grad is None and net.layers[0].output.LayerNorm.weight.grad is None
     with torch.no_grad():
         assert len(concrete.falsify(net, emb, [1], [1.0], 0)) == 1
+
+
+def test_second_derivatives_are_refused():
+    from faith_amd import concrete, ops
+    x = torch.randn(6, 2, 16, device="cuda", requires_grad=True)
+    out = concrete.attention(x, x, x, ops.Packing([6]))
+    (g,) = torch.autograd.grad(out.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+    y, _ = concrete.residual_norm(x.view(6, 32), None, None, None, "rms")
+    (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_sum_and_normalised_sum_both_carry_gradients():
+    """What a network with the norm in front of its blocks does: the sum goes on beside its normalisation."""
+    from faith_amd import concrete
+    g = torch.Generator(device="cuda").manual_seed(3)
+    t = [torch.randn(9, 64, generator=g, device="cuda", requires_grad=True) for _ in range(2)] + [torch.randn(64, generator=g, device="cuda", requires_grad=True) for _ in range(2)]
+    for kind in ("rms", "standard", "no_var"):
+        for given in ([0, 1, 2, 3], [0, 2, 3], [0]):
+            args = [t[i] if i in given else None for i in range(4)]
+            y, h = concrete.residual_norm(*args, kind, 1e-6)
+            got = torch.autograd.grad((y * y).sum() + (h * h * h).sum(), [t[i] for i in given])
+            a = [x.detach().double().requires_grad_(True) if x is not None else None for x in args]
+            s = a[0] if a[1] is None else a[0] + a[1]
+            c = s if kind == "rms" else s - s.mean(-1, keepdim=True)
+            z = c if kind == "no_var" else c / (c.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+            yy = z if a[2] is None else z * a[2] + a[3]
+            want = torch.autograd.grad((yy * yy).sum() + (s * s * s).sum(), [a[i] for i in given])
+            assert all(float((p.double() - q).norm()) <= 1e-5 * float(q.norm()) for p, q in zip(got, want)), (kind, given)
+            only = torch.autograd.grad(concrete.residual_norm(*args, kind, 1e-6)[1].square().sum(), t[0])[0]
+            assert float((only.double() - 2 * s.detach()).norm()) <= 1e-5 * float(s.detach().norm())
