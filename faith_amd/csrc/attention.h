@@ -148,42 +148,74 @@ __device__ __forceinline__ void words_to_lds(float *lds, const float *src, int n
     __builtin_amdgcn_raw_ptr_buffer_load_lds(window(src, (unsigned)n * 4u), (lds_void *)lds, 4, (unsigned)lane * 4u, 0, 0, 0);
 }
 
-// first operand, 32 rows of a tile, 16 (T of 2 bytes) or 8 (float) of the reduction from chunk 2 u on
-template <class T, int DP> __device__ __forceinline__ typename Vec<T>::x8 row_fragment(const T *tile, int row, int u, int half) {
-    return *reinterpret_cast<const typename Vec<T>::x8 *>(tile + Tile<T, DP>::at(row, 2 * u + half));
+// Addresses.  Where a row's bytes are a power of two, the place of a row's chunk is that of its first one with the chunk's number
+// exclusive-ored in: one instruction from one register, however many chunks, blocks and tiles are read (their starts are
+// constants of the instructions).  row0: a multiple of 32.
+
+// first operand, rows row0 ... row0 + 31 of a tile (this lane: row0 + col), 16 bytes of the reduction at its chunk 2 u + half
+template <class T, int DP> __device__ __forceinline__ const char *row_chunk(const T *tile, int row0, int col, int u, int half) {
+    typedef Tile<T, DP> Tl;
+    const int first = (half ^ Tl::swizzle(col)) * 16;
+    int off;
+    if constexpr ((Tl::RB & (Tl::RB - 1)) == 0) off = (col * Tl::RB + first) ^ (32 * u);
+    else off = col * Tl::RB + (first ^ (32 * u));
+    return reinterpret_cast<const char *>(tile) + row0 * Tl::RB + off;
 }
-template <int DP> __device__ __forceinline__ floatx4 row_fragment4(const float *tile, int row, int u, int half) {
-    return *reinterpret_cast<const floatx4 *>(tile + Tile<float, DP>::at(row, 2 * u + half));
+template <class T, int DP> __device__ __forceinline__ typename Vec<T>::x8 row_fragment(const T *tile, int row0, int col, int u, int half) {
+    return *reinterpret_cast<const typename Vec<T>::x8 *>(row_chunk<T, DP>(tile, row0, col, u, half));
 }
-// first operand transposed: columns col0 ... col0 + 31 of the tile against the 16 rows row0 + {0 ... 15} in the order in which
-// registers 0 ... 7 hold them: lane half h has rows 4h ... 4h + 3, then 8 + 4h ... 8 + 4h + 3
-template <class T, int DP, Reads READS> __device__ __forceinline__ typename Vec<T>::x8 column_fragment(const T *tile, int row0, int col0, int lane) {
-    const int i = lane & 15, r = row0 + 4 * (lane >> 5) + (i >> 2), c = col0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-    const T *lo = tile + Tile<T, DP, READS>::at(r, c >> 3) + (c & 7);
-    const T *hi = tile + Tile<T, DP, READS>::at(r + 8, c >> 3) + (c & 7);
-    const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4 *)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4 *)hi);
-    const shortx8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+template <int DP> __device__ __forceinline__ floatx4 row_fragment4(const float *tile, int row0, int col, int u, int half) {
+    return *reinterpret_cast<const floatx4 *>(row_chunk<float, DP>(tile, row0, col, u, half));
+}
+// first operand transposed: columns 32 m ... 32 m + 31 of the tile against the 16 rows row0 + 16 u + {0 ... 15} in the order in
+// which registers 0 ... 7 hold them: lane half h has rows 4h ... 4h + 3, then 8 + 4h ... 8 + 4h + 3
+template <class T, int DP, Reads READS> __device__ __forceinline__ typename Vec<T>::x8 column_fragment(const T *tile, int row0, int u, int m, int lane) {
+    typedef Tile<T, DP, READS> Tl;
+    const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2), c = 16 * ((lane >> 4) & 1) + 4 * (i & 3);       // within the block
+    shortx4 part[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int first = ((c >> 3) ^ Tl::swizzle(r)) * 16 + (c & 7) * 2, flip = (64 * m) ^ ((Tl::swizzle(8) ^ Tl::swizzle(0)) * 16 * h);
+        int off;
+        if constexpr ((Tl::RB & (Tl::RB - 1)) == 0) off = (r * Tl::RB + first) ^ flip;
+        else off = r * Tl::RB + (READS == COLUMNS ? first + flip : (first ^ ((Tl::swizzle(8) ^ Tl::swizzle(0)) * 16 * h)) + 64 * m);
+        part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4 *)(reinterpret_cast<const char *>(tile) + (row0 + 16 * u + 8 * h) * Tl::RB + off));
+    }
+    const shortx8 v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(typename Vec<T>::x8, v);
+}
+// one element, fp32: column 32 m + col of row row0 + row_of(r, half)
+template <int DP, Reads READS> __device__ __forceinline__ float column_element(const float *tile, int row0, int r, int half, int m, int col) {
+    typedef Tile<float, DP, READS> Tl;
+    if constexpr ((Tl::RB & (Tl::RB - 1)) == 0) {
+        // row_of(r, half) = row_of(r, 0) + 4 half, and the swizzles of the two parts have no bit in common
+        const int first = ((col >> 2) ^ Tl::swizzle(4 * half)) * 16 + (col & 3) * 4;
+        const int off = (half * 4 * Tl::RB + first) ^ (128 * m ^ Tl::swizzle(row_of(r, 0)) * 16);
+        return *reinterpret_cast<const float *>(reinterpret_cast<const char *>(tile) + (row0 + row_of(r, 0)) * Tl::RB + off);
+    } else {
+        const int row = row_of(r, half), c = 32 * m + col;
+        return tile[row0 * DP + Tl::at(row, c >> 2) + (c & 3)];
+    }
 }
 
 // acc[r] += sum_d tile[row_of(r)][d] * b[d]: the 32 rows from row0 on against this lane's column, whose values are in `b`
 template <class T, int DP> struct ColumnRegs { typename Vec<T>::x8 v[DP / 16]; };
 template <int DP> struct ColumnRegs<float, DP> { floatx4 v[DP / 8]; };
 
-template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(const T *tile, int row, int half, const ColumnRegs<T, DP> &b) {
+template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(const T *tile, int row0, int col, int half, const ColumnRegs<T, DP> &b) {
     floatx16 acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0.f;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int u = 0; u < DP / 8; ++u) {
-            const floatx4 a = row_fragment4<DP>(tile, row, u, half);
+            const floatx4 a = row_fragment4<DP>(tile, row0, col, u, half);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc = mfma(a[e], b.v[u][e], acc);
         }
     } else {
 #pragma unroll
-        for (int u = 0; u < DP / 16; ++u) acc = mfma(row_fragment<T, DP>(tile, row, u, half), b.v[u], acc);
+        for (int u = 0; u < DP / 16; ++u) acc = mfma(row_fragment<T, DP>(tile, row0, col, u, half), b.v[u], acc);
     }
     return acc;
 }
@@ -240,14 +272,9 @@ template <class T, int DP, Reads READS = ROWS_TOO> __device__ __forceinline__ vo
     if constexpr (sizeof(T) == 4) {
         const int half = lane >> 5, col = lane & 31;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int row = row0 + row_of(r, half);
+        for (int r = 0; r < 16; ++r)
 #pragma unroll
-            for (int m = 0; m < DP / 32; ++m) {
-                const int c = 32 * m + col;
-                acc[m] = mfma(tile[Tile<T, DP, READS>::at(row, c >> 2) + (c & 3)], p[r], acc[m]);
-            }
-        }
+            for (int m = 0; m < DP / 32; ++m) acc[m] = mfma(column_element<DP, READS>(tile, row0, r, half, m, col), p[r], acc[m]);
     } else {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -255,7 +282,7 @@ template <class T, int DP, Reads READS = ROWS_TOO> __device__ __forceinline__ vo
 #pragma unroll
             for (int e = 0; e < 8; ++e) b[e] = (T)p[8 * u + e];
 #pragma unroll
-            for (int m = 0; m < DP / 32; ++m) acc[m] = mfma(column_fragment<T, DP, READS>(tile, row0 + 16 * u, 32 * m, lane), b, acc[m]);
+            for (int m = 0; m < DP / 32; ++m) acc[m] = mfma(column_fragment<T, DP, READS>(tile, row0, u, m, lane), b, acc[m]);
         }
     }
 }

@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(64 * WAVES, (KIND == KIND_KEYS && DP * sizeof(
     typedef floatx16 Scores[BN / 32];
     auto scores = [&](const T *kt, Scores &s) {
 #pragma unroll
-        for (int b = 0; b < BN / 32; ++b) s[b] = rows_by_column<T, DP>(kt + own, 32 * b + col, half, q);
+        for (int b = 0; b < BN / 32; ++b) s[b] = rows_by_column<T, DP>(kt + own, 32 * b, col, half, q);
     };
     // what the mask hides of the tile, and the row's reference
     auto masked = [&](Scores &s, int key0) {

@@ -126,8 +126,8 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         const bool part = key0 + BN - 1 > all_see;
 #pragma unroll
         for (int b = 0; b < BN / 32; ++b) {
-            floatx16 s = rows_by_column<T, DP>(kt + own, 32 * b + col, half, q);
-            const floatx16 dp = rows_by_column<T, DP>(vt + own, 32 * b + col, half, d_o);
+            floatx16 s = rows_by_column<T, DP>(kt + own, 32 * b, col, half, q);
+            const floatx16 dp = rows_by_column<T, DP>(vt + own, 32 * b, col, half, d_o);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], g.c, -lse)) * (dp[r] - delta);
             if (part) {
@@ -236,12 +236,12 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         floatx16 s[BQ / 32], dp[BQ / 32];
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
-            s[b] = rows_by_column<T, DP>(qt, 32 * b + col, half, k);
+            s[b] = rows_by_column<T, DP>(qt, 32 * b, col, half, k);
             if constexpr (V_IN_LDS) {
 #pragma unroll
-                for (int u = 0; u < DP / 16; ++u) v.v[u] = row_fragment<T, DP>(v_rows, wave * 32 + col, u, half);
+                for (int u = 0; u < DP / 16; ++u) v.v[u] = row_fragment<T, DP>(v_rows + wave * 32 * DP, 0, col, u, half);
             }
-            dp[b] = rows_by_column<T, DP>(dt, 32 * b + col, half, v);
+            dp[b] = rows_by_column<T, DP>(dt, 32 * b, col, half, v);
         }
         if (part) {
 #pragma unroll
