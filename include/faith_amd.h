@@ -1,7 +1,8 @@
 /*
  * faith_amd.h -- C ABI of the MI355X (gfx950) forward bound-propagation kernels.
  *
- * Each entry point takes raw DEVICE pointers to contiguous fp32 arrays, plain
+ * Each entry point takes raw DEVICE pointers to contiguous fp32 arrays (those of the
+ * concrete pass, at the end, also 2-byte types and strides), plain
  * ints / floats, and a HIP stream handle passed as void* (NULL = the default
  * stream).  Launches are asynchronous on that stream.  Nothing is allocated or
  * freed; the caller owns every buffer, inputs and outputs alike (as in the
