@@ -1289,7 +1289,8 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
     consecutive.  causal: a query sees the keys up to its own place.  scale: default 1 / sqrt(size).  Returns out like q
     (and, with return_lse, the logarithm of every row's sum of exponentials, float32 [heads, tokens], which
     attention_backward takes).  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, and
-    their places in an `out` that the caller brings not written."""
+    their places in an `out` that the caller brings not written; such an `out` shares no
+    memory with q, k or v."""
     key, known = _known_call(packing, 0, causal, scale, q, k, v) if out is None else (None, None)
     dev = packing.device if known is not None else None
     if known is None:
@@ -1303,6 +1304,9 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
             ot, oh = heads * size, size
         else:
             ot, oh = _rows("out", out, packing.tokens, heads, size, q)
+            # token by token, or head by head; anything in between would be written twice
+            if heads > 1 and (oh < size or (ot < (heads - 1) * oh + size and oh < (packing.tokens - 1) * ot + size and packing.tokens > 1)):
+                raise ValueError(f"out: its rows and heads must not overlap (strides {out.stride()})")
         known = (plan, floats, heads, (items, n, joins, kind, qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size,
                                        _DTYPES[q.dtype], int(causal), _scale(scale, size)))
         if key is not None:

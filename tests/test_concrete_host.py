@@ -247,3 +247,22 @@ def test_random_lengths_give_items_within_the_sequences():
             for qs, a, ks, b, row0, begin, end, slot in items:
                 i = next(i for i in range(n) if sum(ql[:i]) == qs and sum(kl[:i]) == ks and (ql[i], kl[i]) == (a, b))
                 assert 0 <= begin and end <= (b if which < 2 else a) and slot < max(1, slots), i
+
+
+def test_results_whose_heads_share_memory_are_refused():
+    """Heads that lie on each other may be read (one key head seen as many); written, they would race."""
+    L = _lib.lib
+    buf = (ctypes.c_float * 256)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+
+    def forward_call(hs, heads=4):
+        return L.faith_attention(p, p, p, p, None, None, p, 1 << 27, 0, 0, 64, 0, 64, 0, 64, 0, 64, hs, 4, heads, heads, 16, 0, 0, 0.5, None)
+    assert forward_call(0) == -4 and forward_call(12) == -4
+    # past this check, and refused for its number of items: nothing is launched
+    assert forward_call(16) == -3 and forward_call(0, heads=1) == -3
+
+    def backward_call(which):
+        strides = (ctypes.c_longlong * 16)(*[64, 16] * 8)
+        strides[2 * which + 1] = 0
+        return L.faith_attention_backward(p, p, p, p, p, p, p, p, p, p, None, p, 1 << 27, 0, p, 1 << 27, 0, 0, 0, ctypes.addressof(strides), 4, 4, 4, 16, 0, 0, 0.5, None)
+    assert [backward_call(i) for i in range(8)] == [-3] * 5 + [-4] * 3

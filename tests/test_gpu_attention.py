@@ -344,3 +344,23 @@ def test_empty_batches():
         assert bool((out == 0).all()) and bool((lse == -math.inf).all())
         dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing, causal)
         assert bool((dq == 0).all()) and dk.shape == (0, 2, 32) and dv.shape == (0, 2, 32)
+
+
+def test_results_that_lie_on_each_other_are_refused():
+    from faith_amd import ops
+    lengths = [6, 10]
+    q, k, v, _ = tensors(lengths, lengths, 4, 2, 32, BF16)
+    packing = ops.Packing(lengths)
+    want = ops.attention(q, k, v, packing)
+    store = torch.zeros(16 * 4 * 40, device="cuda", dtype=BF16)
+    for strides in [(128, 0, 1), (32, 0, 1), (32, 32, 1), (64, 32, 1), (40, 480, 1)]:
+        with pytest.raises(ValueError, match="must not overlap"):
+            ops.attention(q, k, v, packing, out=store.as_strided((16, 4, 32), strides))
+    assert not store.any()
+    # token by token with room between the heads, and head by head
+    for strides in [(160, 40, 1), (32, 512, 1), (40, 640, 1)]:
+        out = store.as_strided((16, 4, 32), strides)
+        assert ops.attention(q, k, v, packing, out=out) is out and torch.equal(out, want)
+    one = ops.Packing([1])
+    out = store[:160].as_strided((1, 4, 32), (160, 40, 1))
+    assert torch.equal(ops.attention(q[:1], k[:1], v[:1], one, out=out), ops.attention(q[:1], k[:1], v[:1], one))
