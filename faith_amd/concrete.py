@@ -44,8 +44,13 @@ class _Attention(torch.autograd.Function):
 
 
 def attention(q, k, v, packing, causal=False, scale=None):
-    """ops.attention, differentiable with respect to q, k and v, for heads of any size up to 128 (one that does not fall into
-    whole groups of 16 bytes is carried with zeros behind it)."""
+    """ops.attention, differentiable with respect to q, k and v (not the scale, which is a number), for heads of any size up to 128
+    (one that does not fall into whole groups of 16 bytes is carried with zeros behind it)."""
+    if isinstance(scale, torch.Tensor):
+        if torch.is_grad_enabled() and scale.requires_grad:
+            raise ValueError("scale: has no gradient here; multiply q by it")
+        scale = float(scale)                              # the gradient's scale is that of this call, whatever the tensor holds by then
+    causal = bool(causal)
     size, per = q.shape[2], 16 // q.element_size()
     if size % per and size < 128:
         if scale is None:

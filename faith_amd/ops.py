@@ -1247,10 +1247,11 @@ def _attention_operands(q, k, v, packing):
     return heads, kv_heads, size, qs, ks, vs
 
 
-def _known_call(packing, which, causal, scale, q, k, v, *more):
+def _known_call(packing, which, causal, q, k, v, *more):
     """The arguments of an earlier call with operands of these shapes and types, all contiguous, on the packing's device and
     on 16 bytes: (key, what was kept or None).  A small call is bound by its host side, and most of that is checks whose
-    outcome depends on nothing else; whatever this does not recognise takes the long way."""
+    outcome depends on nothing else; whatever this does not recognise takes the long way.  causal: a bool, not the tensor
+    that may have held it, whose value changes where its identity does not; the scale is no part of what is kept."""
     try:
         index, dtype, address = packing.device.index, q.dtype, 0
         for t in (q, k, v, *more):
@@ -1259,7 +1260,7 @@ def _known_call(packing, which, causal, scale, q, k, v, *more):
             address |= t.data_ptr()
         if address & 15:
             return None, None
-        key = (which, causal, scale, dtype, q.shape, k.shape, v.shape)
+        key = (which, causal, dtype, q.shape, k.shape, v.shape)
         return key, packing._calls.get(key)
     except (AttributeError, TypeError):
         return None, None
@@ -1286,12 +1287,13 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
     """softmax(scale q k^T) v of every sequence of `packing`, for the network itself (not its bounds).
 
     q [tokens, heads, size], k, v [keys, kv_heads, size], float32, bfloat16 or float16; heads that share a key head are
-    consecutive.  causal: a query sees the keys up to its own place.  scale: default 1 / sqrt(size).  Returns out like q
+    consecutive.  causal: a query sees the keys up to its own place.  scale: a number, default 1 / sqrt(size).  Returns out like q
     (and, with return_lse, the logarithm of every row's sum of exponentials, float32 [heads, tokens], which
     attention_backward takes).  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, and
     their places in an `out` that the caller brings not written; such an `out` shares no
     memory with q, k or v."""
-    key, known = _known_call(packing, 0, causal, scale, q, k, v) if out is None else (None, None)
+    causal = bool(causal)
+    key, known = _known_call(packing, 0, causal, q, k, v) if out is None else (None, None)
     dev = packing.device if known is not None else None
     if known is None:
         heads, kv_heads, size, (qt, qh), (kt, kh), (vt, vh) = _attention_operands(q, k, v, packing)
@@ -1308,10 +1310,11 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
             if heads > 1 and (oh < size or (ot < (heads - 1) * oh + size and oh < (packing.tokens - 1) * ot + size and packing.tokens > 1)):
                 raise ValueError(f"out: its rows and heads must not overlap (strides {out.stride()})")
         known = (plan, floats, heads, (items, n, joins, kind, qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size,
-                                       _DTYPES[q.dtype], int(causal), _scale(scale, size)))
+                                       _DTYPES[q.dtype], int(causal)), size)
         if key is not None:
             packing._calls[key] = known
-    plan, floats, heads, rest = known
+    plan, floats, heads, rest, size = known
+    scale = _scale(scale, size)
     if out is None:
         out = _like_rows(q, packing.tokens)
     lse = _empty(heads, packing.tokens, device=dev) if return_lse else None
@@ -1324,7 +1327,7 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
     stream = _stream(q)
     packing._used_on(plan, stream)
     with _on(dev):
-        _lib.call("faith_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(scratch), *rest, stream)
+        _lib.call("faith_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(scratch), *rest, scale, stream)
     return (out, lse) if return_lse else out
 
 
@@ -1332,7 +1335,8 @@ def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=Non
     """Gradients of attention(): (dq, dk, dv), each of its operand's shape and type, from dout, the gradient of its result.
     out, lse: what the forward call returned (return_lse=True); the other arguments as in that call.  Sums in float32;
     the gradients of a key head add up those of the heads that share it.  The same bits on every call."""
-    key, known = _known_call(packing, 1, causal, scale, q, k, v, dout, out)
+    causal = bool(causal)
+    key, known = _known_call(packing, 1, causal, q, k, v, dout, out)
     if known is None or dout.shape != q.shape or out.shape != q.shape:
         import ctypes
         heads, kv_heads, size, qs, ks, vs = _attention_operands(q, k, v, packing)
@@ -1344,10 +1348,11 @@ def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=Non
             plans = [packing.plan(which, heads, kv_heads, q.element_size(), size, causal) for which in (_lib.ATTENTION_GRAD_QUERIES, _lib.ATTENTION_GRAD_KEYS)]
         floats = plans[1][4] * kv_heads * (32 if plans[1][5] else 128) * 2 * ((size + 31) // 32 * 32)
         known = (plans, floats, heads, (plans[0][1], plans[0][2], plans[0][5], *plans[1][1:6], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
-                                size, _DTYPES[q.dtype], int(causal), _scale(scale, size)), strides)
+                                size, _DTYPES[q.dtype], int(causal)), size, strides)
         if key is not None and dout.shape == q.shape and out.shape == q.shape:
             packing._calls[key] = known
-    plans, floats, heads, rest, _ = known
+    plans, floats, heads, rest, size, _ = known
+    scale = _scale(scale, size)
     _check("lse", lse, (heads, packing.tokens))
     dev = packing.device
     if lse.get_device() != dev.index:
@@ -1360,7 +1365,7 @@ def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=Non
     packing._used_on(plans[1], stream)
     with _on(dev):
         _lib.call("faith_attention_backward", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stat.data_ptr(), _ptr(parts), *rest, stream)
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stat.data_ptr(), _ptr(parts), *rest, scale, stream)
     return dq, dk, dv
 
 

@@ -266,3 +266,17 @@ def test_results_whose_heads_share_memory_are_refused():
         strides[2 * which + 1] = 0
         return L.faith_attention_backward(p, p, p, p, p, p, p, p, p, p, None, p, 1 << 27, 0, p, 1 << 27, 0, 0, 0, ctypes.addressof(strides), 4, 4, 4, 16, 0, 0, 0.5, None)
     assert [backward_call(i) for i in range(8)] == [-3] * 5 + [-4] * 3
+
+
+def test_what_is_kept_of_a_call_holds_no_number_of_it():
+    from types import SimpleNamespace
+    q = torch.zeros(4, 2, 16)
+    packing = SimpleNamespace(device=SimpleNamespace(index=q.get_device()), _calls={})
+    key, _ = ops._known_call(packing, 0, True, q, q, q)
+    assert key is not None and not any(isinstance(x, (torch.Tensor, float)) for x in key)
+
+
+def test_a_scale_that_asks_for_a_gradient_is_refused():
+    q = torch.zeros(4, 2, 16)
+    with pytest.raises(ValueError, match="scale"):
+        concrete.attention(q, q, q, ops.Packing([4]), scale=torch.tensor(0.5, requires_grad=True))

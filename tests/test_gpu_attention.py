@@ -364,3 +364,39 @@ def test_results_that_lie_on_each_other_are_refused():
     one = ops.Packing([1])
     out = store[:160].as_strided((1, 4, 32), (160, 40, 1))
     assert torch.equal(ops.attention(q[:1], k[:1], v[:1], one, out=out), ops.attention(q[:1], k[:1], v[:1], one))
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+def test_a_scale_or_mask_given_as_a_tensor_is_read_by_every_call(where):
+    """What a tensor holds now counts, not what it held when a call like this one was made first."""
+    from faith_amd import ops
+    lengths = [20, 5]
+    q, k, v, dout = tensors(lengths, lengths, 4, 2, 32, F32)
+    packing, fresh = ops.Packing(lengths), lambda: ops.Packing(lengths)
+    scale, causal = torch.full((), 0.5, device=where), torch.tensor(True, device=where)
+    for number, mask in ((0.5, True), (2.0, True), (2.0, False), (0.125, False), (0.5, True)):
+        scale.fill_(number)
+        causal.fill_(mask)
+        out, lse = ops.attention(q, k, v, packing, causal, scale, return_lse=True)
+        want, want_lse = ops.attention(q, k, v, fresh(), mask, number, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        got = ops.attention_backward(dout, q, k, v, out, lse, packing, causal, scale)
+        assert all(torch.equal(a, b) for a, b in zip(got, ops.attention_backward(dout, q, k, v, out, lse, fresh(), mask, number)))
+    # a scale that changes with every call (a temperature, a trained one) leaves nothing behind
+    known = len(packing._calls)
+    for i in range(20):
+        ops.attention(q, k, v, packing, True, 0.1 + i)
+    assert len(packing._calls) == known
+
+
+def test_the_gradient_takes_the_scale_of_its_forward_call():
+    from faith_amd import concrete, ops
+    lengths = [9, 30]
+    q, k, v, dout = tensors(lengths, lengths, 4, 4, 32, F32, 2)
+    q.requires_grad_(True)
+    scale = torch.tensor(0.5)
+    out = concrete.attention(q, k, v, ops.Packing(lengths), scale=scale)
+    scale.fill_(4.0)
+    (got,) = torch.autograd.grad(out, q, dout)
+    (want,) = torch.autograd.grad(concrete.attention(q, k, v, ops.Packing(lengths), scale=0.5), q, dout)
+    assert torch.equal(got, want)
