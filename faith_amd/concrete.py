@@ -200,13 +200,34 @@ def _steepest(g, p):
 def _into_ball(d, p, radii):
     if math.isinf(p) or p >= 10:
         return torch.maximum(torch.minimum(d, radii[:, None]), -radii[:, None])
-    return d * (radii / torch.linalg.vector_norm(d, ord=p, dim=1).clamp_min(1e-30)).clamp_max(1.0)[:, None]
+    # a little further in than the norm's own rounding may be off
+    inside = radii * (1 - 2.0 ** -40) if d.dtype == torch.float64 else radii
+    return d * (inside / torch.linalg.vector_norm(d, ord=p, dim=1).clamp_min(1e-30)).clamp_max(1.0)[:, None]
+
+
+def _toward(t, base):
+    """For every element of t the neighbour of its type that lies one step closer to `base`."""
+    kind = torch.int32 if t.element_size() == 4 else torch.int16
+    bits = t.view(kind)                                   # sign and magnitude: one less is one step towards zero
+    step = torch.where((t > 0) == (base < t), bits - 1, bits + 1)
+    smallest = torch.where(base < 0, torch.iinfo(kind).min + 1, 1)
+    return torch.where(t == 0, smallest, step).to(kind).view(t.dtype)
+
+
+def _moved(base, delta):
+    """base + delta (float64) in base's type, rounded to nearest but never past delta: every element moves by delta's at most, so the
+    perturbation that the network sees has no norm larger than delta's."""
+    moved = (base.double() + delta).to(base.dtype)
+    past = (moved.double() - base.double()).abs() > delta.abs()
+    return torch.where(past, _toward(moved, base), moved)
 
 
 def falsify(network, embeddings, positions, radii, label, p=2.0, steps=10, batch=None):
     """Searches, for every (position, radius) pair at once, for a perturbation of the embedding at that position, of p-norm at
     most the radius, with which the network no longer answers `label` with a positive margin: `steps` steps of projected steepest ascent from the
-    sentence itself.  embeddings [1, L, hidden].  Returns a list of bools; True is a proof, False only that none was found.
+    sentence itself.  embeddings [1, L, hidden].  Returns a list of bools; True is a proof, False only that none was found: what counts is
+    the perturbation of the embeddings as they are, rounded to their type (in 16 bits a radius under half a step of every element holds none
+    but zero), and a margin that is a finite number.
 
     A step is one pass forward and backward over as many copies of the sentence as there are pairs.  batch: their Batch,
     where the caller keeps one."""
@@ -222,6 +243,8 @@ def falsify(network, embeddings, positions, radii, label, p=2.0, steps=10, batch
             raise ValueError(f"radius {r!r} is not a radius")
     if not positions:
         return []
+    if embeddings.dim() != 3 or embeddings.shape[0] != 1:
+        raise ValueError(f"embeddings: expected one sentence [1, length, hidden], got {tuple(embeddings.shape)}")
     n, length = len(positions), embeddings.shape[1]
     at = [g[0] for g in _checked_positions([[i] for i in positions], length)]
     classes = network.classifier.weight.shape[0]
@@ -234,24 +257,26 @@ def falsify(network, embeddings, positions, radii, label, p=2.0, steps=10, batch
         raise ValueError(f"batch: expected {n} sentences of {length}")
     base = embeddings.detach().expand(n, length, embeddings.shape[2]).reshape(n * length, -1)
     where = batch.first + torch.tensor(at, dtype=torch.int64, device=dev)
-    r = torch.tensor([float(v) for v in radii], dtype=torch.float32, device=dev)
-    delta = torch.zeros(n, base.shape[1], device=dev)
+    r = torch.tensor([float(v) for v in radii], dtype=torch.float64, device=dev)
+    delta = torch.zeros(n, base.shape[1], dtype=torch.float64, device=dev)
     found = torch.zeros(n, dtype=torch.bool, device=dev)
     for step in range(steps + 1):
         with torch.enable_grad():
             # leaf: the perturbed rows, so that the parameters collect no gradients
-            moved = (base[where].float() + delta).to(base.dtype).requires_grad_(True)
+            moved = _moved(base[where], delta).requires_grad_(True)
             out = _logits(network, base.index_copy(0, where, moved), batch).float()
             others = out.index_fill(1, torch.tensor([label], device=dev), -math.inf).amax(1)
             margin = out[:, label] - others
-            # as in the propagation: an answer is safe only while its margin is positive
-            found |= ~(margin.detach() > 0)
+            # as in the propagation: an answer is safe only while its margin is positive.  NaN or an infinity is no answer: an
+            # overflow of the arithmetic, which proves nothing
+            found |= (margin.detach() <= 0) & torch.isfinite(margin.detach())
             if step == steps:
                 break
             (g,) = torch.autograd.grad(margin.sum(), moved)
-        # a first step to the border, then ones that can cross the ball
+        # a first step to the border, then ones that can cross the ball; none along a gradient that is no number
         size = r if step == 0 else r * (2.0 / steps)
-        delta = _into_ball(delta - _steepest(g.float(), p) * size[:, None], p, r)
+        usable = torch.isfinite(g).all(1, keepdim=True)
+        delta = torch.where(usable, _into_ball(delta - _steepest(g.float(), p).double() * size[:, None], p, r), delta)
     return found.tolist()
 
 

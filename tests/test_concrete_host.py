@@ -280,3 +280,89 @@ def test_a_scale_that_asks_for_a_gradient_is_refused():
     q = torch.zeros(4, 2, 16)
     with pytest.raises(ValueError, match="scale"):
         concrete.attention(q, q, q, ops.Packing([4]), scale=torch.tensor(0.5, requires_grad=True))
+
+
+def norm_of(d, p):
+    return torch.linalg.vector_norm(d.double(), ord=math.inf if p >= 10 else p, dim=1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("p", [1.0, 1.5, 2.0, math.inf])
+@pytest.mark.parametrize("radius", [1e-6, 1e-3, 1e-2, 0.05, 3.0])
+def test_the_perturbation_that_the_network_sees_is_in_the_ball(dtype, p, radius):
+    """Rounded to the embeddings' type, at radii far under, near and far over one step of it; zeros and the largest values too."""
+    g = torch.Generator().manual_seed(17)
+    base = torch.randn(40, 256, generator=g).to(dtype)
+    base[0], base[1, ::2], base[2, ::3] = 0, 0, torch.finfo(dtype).max
+    base[3] = torch.finfo(dtype).tiny
+    r = torch.full((40,), radius, dtype=torch.float64)
+    for d in (torch.randn(40, 256, generator=g), concrete._steepest(torch.randn(40, 256, generator=g), p)):
+        delta = concrete._into_ball(d.double() * radius, p, r)
+        moved = concrete._moved(base, delta)
+        assert moved.dtype == dtype and bool(torch.isfinite(moved).all())
+        assert bool((norm_of(moved.double() - base.double(), p) <= r).all())
+        # and no further in than one step of the type: eps of a magnitude that |base| + |delta| bounds
+        ulp = (base.double().abs() + delta.abs()) * torch.finfo(dtype).eps + torch.finfo(dtype).smallest_normal
+        short = (moved.double() - base.double() - delta).abs()
+        assert bool((short[3:] <= ulp[3:]).all())
+
+
+def searched(monkeypatch, logits, embeddings, radii, p=2.0, steps=4, label=0):
+    """falsify on the CPU, on a network that is one function of its rows; also every perturbation that it looked at."""
+    from types import SimpleNamespace
+    n, length = len(radii), embeddings.shape[1]
+    seen = []
+
+    def run(network, x, batch, activations=None):
+        rows = x.view(n, length, -1)
+        seen.append((rows.detach() - 0)[:, 1].double() - embeddings[0, 1].double())
+        return logits(rows)
+    monkeypatch.setattr(concrete, "_logits", run)
+    net = SimpleNamespace(classifier=SimpleNamespace(weight=torch.zeros(2, embeddings.shape[2])))
+    batch = SimpleNamespace(packing=SimpleNamespace(lengths=(length,) * n), first=torch.arange(n) * length)
+    return concrete.falsify(net, embeddings, [1] * n, radii, label, p, steps, batch), seen
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+def test_the_search_stays_in_the_ball(monkeypatch, dtype, p):
+    g = torch.Generator().manual_seed(3)
+    emb, w = torch.randn(1, 3, 256, generator=g).to(dtype), torch.randn(2, 256, generator=g)
+    radii = [0.0, 1e-4, 1e-3, 0.01, 0.05, 0.1, 1.0, 30.0]
+    found, seen = searched(monkeypatch, lambda rows: torch.tanh(rows[:, 1].float() @ w.t() / 16), emb, radii, p, label=int((emb[0, 1].float() @ w.t()).argmax()))
+    assert len(seen) == 5
+    for moved in seen:
+        assert bool((norm_of(moved, p) <= torch.tensor(radii, dtype=torch.float64)).all())
+    assert found[-1] and not found[0]
+
+
+def test_what_is_no_number_proves_nothing(monkeypatch):
+    emb = torch.ones(1, 3, 4)
+    column = lambda m: torch.stack([m, torch.zeros_like(m)], 1)
+    # a margin that is NaN everywhere, one that becomes NaN or infinite away from the sentence
+    for f in (lambda x: x[:, 1, 0] * math.nan, lambda x: torch.sqrt(x[:, 1, 0] - 0.999999), lambda x: 1 / (x[:, 1, 0] - 0.5).clamp_min(0) * 0 + 1,
+              lambda x: torch.where(x[:, 1, 0] < 1, -math.inf, 1.0) + 0 * x[:, 1, 0]):
+        found, _ = searched(monkeypatch, lambda rows: column(f(rows)), emb, [0.5, 0.6])
+        assert found == [False, False]
+
+    class Overflow(torch.autograd.Function):
+        """A margin of one whose gradient is infinite and NaN."""
+        @staticmethod
+        def forward(ctx, x):
+            return torch.ones(x.shape[0])
+
+        @staticmethod
+        def backward(ctx, g):
+            bad = torch.full((2, 3, 4), math.inf)
+            bad[1, 1, 2] = math.nan
+            return bad
+    found, seen = searched(monkeypatch, lambda rows: column(Overflow.apply(rows)), emb, [0.5, 0.6])
+    assert found == [False, False] and all(bool((d == 0).all()) for d in seen)
+
+
+def test_the_search_takes_one_sentence():
+    from types import SimpleNamespace
+    net = SimpleNamespace(classifier=SimpleNamespace(weight=torch.zeros(2, 8)))
+    for shape in ((2, 4, 8), (4, 8), (0, 4, 8)):
+        with pytest.raises(ValueError, match="one sentence"):
+            concrete.falsify(net, torch.zeros(shape), [1, 2], [0.1, 0.1], 0)

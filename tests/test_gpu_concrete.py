@@ -228,3 +228,25 @@ def test_sum_and_normalised_sum_both_carry_gradients():
             assert all(float((p.double() - q).norm()) <= 1e-5 * float(q.norm()) for p, q in zip(got, want)), (kind, given)
             only = torch.autograd.grad(concrete.residual_norm(*args, kind, 1e-6)[1].square().sum(), t[0])[0]
             assert float((only.double() - 2 * s.detach()).norm()) <= 1e-5 * float(s.detach().norm())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("p", [2.0, math.inf])
+def test_what_breaks_the_answer_in_half_precision_lies_in_the_ball(monkeypatch, dtype, p):
+    """Radii near one step of the type: every row that the network is asked about is within its radius of the sentence."""
+    from faith_amd import concrete
+    net = network(21, "no_var", layers=1, hidden=64)
+    cast = lambda o: SimpleNamespace(**{k: cast(v) for k, v in vars(o).items()}) if isinstance(o, SimpleNamespace) else (o.to(dtype) if isinstance(o, torch.Tensor) else o)
+    net.embedding_norm, net.pooler, net.classifier, net.layers = cast(net.embedding_norm), cast(net.pooler), cast(net.classifier), [cast(l) for l in net.layers]
+    emb = sentences([6], 22, 64)[0][None].to(dtype)
+    (label,) = concrete.predict(net, emb)
+    radii, seen, run = [0.0, 1e-3, 0.01, 0.05, 1.0, 100.0], [], concrete._logits
+
+    def watched(network, x, batch, activations=None):
+        seen.append(x.detach().view(len(radii), 6, 64)[:, 2].double() - emb[0, 2].double())
+        return run(network, x, batch, activations)
+    monkeypatch.setattr(concrete, "_logits", watched)
+    found = concrete.falsify(net, emb, [2] * len(radii), radii, label, p)
+    assert not found[0] and len(seen) == 11
+    for d in seen:
+        assert bool((torch.linalg.vector_norm(d, ord=p, dim=1) <= torch.tensor(radii, device="cuda", dtype=torch.float64)).all())
