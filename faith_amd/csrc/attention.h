@@ -287,6 +287,12 @@ template <class T, int DP, Reads READS = ROWS_TOO> __device__ __forceinline__ vo
     }
 }
 
+// Operands in fp16.  Its five exponent bits end at 2^-14 (2^-24 with ever fewer bits) and 65504, and a probability among
+// thousands of keys, or a small gradient times one, lies below.  So what is rounded to fp16 is first multiplied by a power of two, which
+// the 32-bit sums it goes into are divided by at the end: both are exact.  bf16 has the exponents of 32 bits and needs none.
+// Probabilities, at most 1: a constant.
+template <class T> constexpr int probability_up() { return std::is_same<T, _Float16>::value ? 14 : 0; }
+
 // over the two lanes that share a column
 __device__ __forceinline__ float max_halves(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -297,6 +303,36 @@ __device__ __forceinline__ float sum_halves(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     const unsigned a = s[0], b = s[1];
     return __uint_as_float(a) + __uint_as_float(b);
+}
+
+// Other values (fp16): a power of two for each column, 2^up, under which the largest of the column so far lies in [2^7, 2^15].  It starts
+// higher than any value asks for and only falls; the sums follow it.  13 sequences of 37 ... 1021, 12 heads of 80, forward and
+// gradients: 199 us with it, 190 without; 2048 keys and gradients of 2^-13: dq off by 0.38 %, all of it its own rounding, instead of 2.2.
+constexpr int UP_MOST = 120;
+template <int DP> __device__ __forceinline__ void raise(floatx16 &s, floatx16 (&acc)[DP / 32], int &up) {
+    float top = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, __builtin_fabsf(s[r]));
+    if (__any(__builtin_ldexpf(top, up) > 32768.f)) {
+        top = max_halves(top);
+        const int want = 8 - __builtin_amdgcn_frexp_expf(top), now = __builtin_ldexpf(top, up) > 32768.f && want < up ? want : up;
+        const float f = __builtin_ldexpf(1.f, now - up);
+        up = now;
+#pragma unroll
+        for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[m][r] *= f;
+    }
+    const float f = __builtin_ldexpf(1.f, up);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= f;
+}
+// acc times 2^-up
+template <int DP> __device__ __forceinline__ void lower(floatx16 (&acc)[DP / 32], int up) {
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[m][r] = __builtin_ldexpf(acc[m][r], -up);
 }
 
 // Wavefronts of a workgroup that share their columns and divide the reduction, each with tiles of its own: four, unless their

@@ -110,6 +110,9 @@ __global__ void __launch_bounds__(64 * WAVES, (KIND == KIND_KEYS && DP * sizeof(
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[m][r] = 0.f;
     float ref = LOWEST, sum = 0.f;           // the row's reference (powers of two) and this lane's part of its sum
+    // fp16: the reference lies that much under the row's maximum, so that smaller probabilities keep their bits as operands; the
+    // largest are then 2^(UP + LAZY) = 2^15
+    constexpr float UP = probability_up<T>() ? 7.f : 0.f;
 
     St ks;
     Sv vs;
@@ -144,8 +147,8 @@ __global__ void __launch_bounds__(64 * WAVES, (KIND == KIND_KEYS && DP * sizeof(
             for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[b][r]);
         // The reference follows the maximum only when it has fallen LAZY powers of two behind: sums and outputs are then at
         // most 2^LAZY times what they would be, which costs no precision, and most tiles rescale nothing.
-        if (__any(top * g.c > ref + LAZY)) {
-            const float now = __builtin_fmaxf(ref, max_halves(top) * g.c), f = __builtin_amdgcn_exp2f(ref - now);
+        if (__any(top * g.c > ref + (UP + LAZY))) {
+            const float now = __builtin_fmaxf(ref, max_halves(top) * g.c - UP), f = __builtin_amdgcn_exp2f(ref - now);
             ref = now;
             sum *= f;
 #pragma unroll

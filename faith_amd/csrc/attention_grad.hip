@@ -1,8 +1,8 @@
 // Gradients of the attention of a network's concrete pass (attention.hip), scores and probabilities computed again:
 //     p = exp(s - lse),  dp = do . v,  ds = p (dp - delta),  delta = do . out
 //     dq = scale sum_j ds k,   dk = scale sum_{i, heads of the group} ds q,   dv = sum_{i, heads of the group} p do
-// p and ds are held in 32 bits and rounded once, to the elements' type, as operands of the last three products; delta comes from
-// the output as it was stored.  Against one rounding of each result these are two or three independent ones of the same size:
+// p and ds are held in 32 bits and rounded once, to the elements' type, as operands of the last three products (in fp16 times a power
+// of two that keeps them in its range, see raise() in attention.h); delta comes from the output as it was stored.  Against one rounding of each result these are two or three independent ones of the same size:
 // 1.4 times the error of a computation in 32 bits at a few hundred keys, up to twice at a handful.
 // Two launches (a third joins parts where the plan cuts) and no atomics, so that the same call gives the same bits: one goes over the keys for a tile of query rows (and
 // leaves delta and the logarithm of the row's sum, in powers of two, to the other), one over the queries of all heads of the
@@ -20,7 +20,7 @@ struct GradArgs {
     const void *dout, *q, *k, *v, *out;
     const float *lse;
     void *dq, *dk, *dv;
-    float *stat;                             // [2][heads][lse_hs]: lse in powers of two, delta
+    float *stat;                             // [2][heads][lse_hs]: lse in powers of two less probability_up(), delta
     float *part;                             // [slots][key heads][keys of an item][2 DP]: parts of dk and dv
     const Item *items;
     Deal deal;
@@ -116,7 +116,9 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
 #pragma unroll
         for (int e = 0; e < PER; ++e) delta = fmaf((float)o.v[u][e], (float)d_o.v[u][e], delta);
     delta = sum_halves(delta);
-    const float lse = l == -__builtin_inff() ? 0.f : l * 1.4426950408889634f;      // a row that sees no key: every p below is masked
+    // a row that sees no key: every p below is masked.  p comes out times 2^probability_up(), and so does ds
+    const float lse = l == -__builtin_inff() ? 0.f : fmaf(l, 1.4426950408889634f, -(float)probability_up<T>());
+    int up = UP_MOST;                        // of ds, fp16
     if (row < rows && half == 0 && (!SPLIT || wave == 0)) {
         float *s = g.stat + (long long)head * g.lse_hs + place;
         s[0] = lse;
@@ -136,6 +138,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                 for (int r = 0; r < 16; ++r)
                     if (key0 + 32 * b + row_of(r, half) > last) s[r] = 0.f;
             }
+            if constexpr (probability_up<T>() > 0) raise<DP>(s, dq, up);
             columns_by_result<T, DP>(dq, kt + own, 32 * b, lane, s);
         }
     };
@@ -143,6 +146,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         alone<2 * St::LOADS, ONCE>(first, WAVES * BN, it.end,
                              [&](int n, int key0) { n ? stage(k1, v1, key0) : stage(k0, v0, key0); },
                              [&](int n, int key0) { n ? tile(k1, v1, key0) : tile(k0, v0, key0); });
+        if constexpr (probability_up<T>() > 0) lower<DP>(dq, up + probability_up<T>());
         add_waves<WAVES, DP, ALL * (int)sizeof(T) / 4>(dq, reinterpret_cast<float *>(k0), reinterpret_cast<float *>(v0), wave, lane);
         if (wave > 0) return;
     } else if (it.begin < it.end) {
@@ -155,13 +159,14 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
             if (key0 + 2 * BN < it.end) stage(k0, v0, key0 + 2 * BN);
             tile(k1, v1, key0 + BN);
         }
+        if constexpr (probability_up<T>() > 0) lower<DP>(dq, up + probability_up<T>());
     }
     if (g.causal && any_not_finite<DP>(dq)) {
         // see one_row in attention.hip: what the mask hides may have come in as 0 * NaN
         clear<DP>(dq);
         for (int j = 0; j <= last; ++j) {
             const T *kr = kb + (long long)j * g.k_ts;
-            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qrow, kr, g.size), g.c, -lse));
+            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qrow, kr, g.size), g.c, -lse - probability_up<T>()));
             add_row<T, DP>(dq, kr, p * (dot_rows(dorow, vb + (long long)j * g.v_ts, g.size) - delta), half, g.size);
         }
     }
@@ -205,6 +210,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
     floatx16 dk[DP / 32], dv[DP / 32];
     clear<DP>(dk);
     clear<DP>(dv);
+    int up = UP_MOST;                        // of ds, fp16
     St qs, ds;
     qs.init(lane, staged, g.size, g.q_ts);
     ds.init(lane, staged, g.size, g.do_ts);
@@ -269,6 +275,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                     if (it.k_len == 1 || t0 + 32 * b + row_of(r, half) == -shift) dp[b][r] = 0.f;
             }
             columns_by_result<T, DP>(dv, dt, 32 * b, lane, s[b]);
+            if constexpr (probability_up<T>() > 0) raise<DP>(dp[b], dk, up);
             columns_by_result<T, DP>(dk, qt, 32 * b, lane, dp[b]);
         }
     };
@@ -280,6 +287,10 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                                  [&](int n, int i) { n ? stage_at(q1, d1, l1, e1, i / tiles, token(i)) : stage_at(q0, d0, l0, e0, i / tiles, token(i)); },
                                  [&](int n, int i) { n ? tile_at(q1, d1, l1, e1, token(i)) : tile_at(q0, d0, l0, e0, token(i)); });
         constexpr int HALF = ALL * (int)sizeof(T) / 4;
+        if constexpr (probability_up<T>() > 0) {
+            lower<DP>(dk, up + probability_up<T>());
+            lower<DP>(dv, probability_up<T>());
+        }
         add_waves<WAVES, DP, HALF>(dk, reinterpret_cast<float *>(q0), reinterpret_cast<float *>(d0), wave, lane);
         add_waves<WAVES, DP, HALF>(dv, reinterpret_cast<float *>(q0), reinterpret_cast<float *>(d0), wave, lane);
         if (wave > 0) return;
@@ -304,6 +315,10 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
             if (i + 2 < total) stage(q0, d0, l0, e0);
             tile(q1, d1, l1, e1);
         }
+        if constexpr (probability_up<T>() > 0) {
+            lower<DP>(dk, up + probability_up<T>());
+            lower<DP>(dv, probability_up<T>());
+        }
     }
     if (g.causal && (any_not_finite<DP>(dk) || any_not_finite<DP>(dv))) {
         clear<DP>(dk);
@@ -313,7 +328,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                 const long long place = it.q_start + i;
                 const T *qr = at<T>(g.q, place, g.q_ts, h, g.q_hs), *dr = at<T>(g.dout, place, g.do_ts, h, g.do_hs);
                 const float *s = g.stat + (long long)h * g.lse_hs + place;
-                const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, krow, g.size), g.c, -s[0]));
+                const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, krow, g.size), g.c, -s[0] - probability_up<T>()));
                 add_row<T, DP>(dv, dr, p, half, g.size);
                 add_row<T, DP>(dk, qr, p * (dot_rows(dr, vrow, g.size) - s[stat_hs]), half, g.size);
             }

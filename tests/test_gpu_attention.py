@@ -400,3 +400,72 @@ def test_the_gradient_takes_the_scale_of_its_forward_call():
     (got,) = torch.autograd.grad(out, q, dout)
     (want,) = torch.autograd.grad(concrete.attention(q, k, v, ops.Packing(lengths), scale=0.5), q, dout)
     assert torch.equal(got, want)
+
+
+def small_gradient_reference(q, k, v, dout, scale):
+    """One sequence, every head seeing every key, in float64: (dq, dk, dv) and their tolerances.  Rounding ds and p to the operands'
+    type is half a step of each, at any size of theirs: nothing is added for values under the type's normal range but half the
+    smallest step of the result, where a result lies there."""
+    ut, u32 = R.half_step(q.dtype), R.U32
+    (n, heads, size), (m, kv_heads, _) = q.shape, k.shape
+    smallest = 2.0 ** -25
+    grads = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k, v)]
+    tols = [torch.full_like(g, smallest) for g in grads]
+    for h in range(heads):
+        g = h // (heads // kv_heads)
+        qh, kh, vh, do = q[:, h].double(), k[:, g].double(), v[:, g].double(), dout[:, h].double()
+        s = (qh @ kh.t()) * scale
+        p = torch.softmax(s, 1)
+        o = p @ vh
+        # scores in 32 bits, twice (in p and in the sum below it); sums of m terms
+        ep = 2 * (size + 4) * u32 * float((qh.abs() @ kh.abs().t()).max()) * scale + (m + 48) * u32
+        o_tol = (ep + ut + (m + 4) * u32) * (p @ vh.abs()) + ut * o.abs() + smallest
+        dp, delta = do @ vh.t(), (do * o).sum(1, keepdim=True)
+        ds = p * (dp - delta)
+        ds_tol = p * ((size + 4) * u32 * (do.abs() @ vh.abs().t() + (do.abs() * o.abs()).sum(1, keepdim=True)) + (do.abs() * o_tol).sum(1, keepdim=True)) \
+            + (ep + ut + 8 * u32) * ds.abs()
+        parts = [(0, slice(None), h, scale * (ds @ kh), scale * ((ds_tol + (m + 4) * u32 * ds.abs()) @ kh.abs())),
+                 (1, slice(None), g, scale * (ds.t() @ qh), scale * ((ds_tol + (n * heads + 4) * u32 * ds.abs()).t() @ qh.abs())),
+                 (2, slice(None), g, p.t() @ do, ((ep + ut + (n * heads + 4) * u32) * p).t() @ do.abs())]
+        for i, rows, head, value, tol in parts:
+            grads[i][rows, head] += value
+            tols[i][rows, head] += tol
+    return [(g, t + ut * g.abs()) for g, t in zip(grads, tols)]
+
+
+@pytest.mark.parametrize("n, m, heads, kv_heads", [(256, 4096, 2, 1), (1024, 1024, 2, 2), (40, 2048, 2, 1), (2048, 300, 3, 1), (7, 5000, 1, 1)])
+@pytest.mark.parametrize("power", [0, -7, -10, -13])
+def test_small_gradients_in_half_precision(n, m, heads, kv_heads, power):
+    """Many keys and a small gradient of the result: p and ds lie under fp16's normal range."""
+    from faith_amd import ops
+    q, k, v, dout = tensors([n], [m], heads, kv_heads, 64, F16, 21)
+    dout = (dout.float() * 2.0 ** power).to(F16)
+    packing = ops.Packing([n], [m])
+    out, lse = ops.attention(q, k, v, packing, return_lse=True)
+    grads = ops.attention_backward(dout, q, k, v, out, lse, packing)
+    for name, got, (want, tol) in zip(("dq", "dk", "dv"), grads, small_gradient_reference(q, k, v, dout, 0.125)):
+        R.check(name, got, want, tol)
+        # and over all of it: three independent roundings (p or ds, delta's, the result's) against one of the result
+        once = float((want.to(F16).double() - want).norm())
+        assert float((got.double() - want).norm()) <= 3 * once + 1e-5 * float(want.norm()), name
+
+
+@pytest.mark.parametrize("n, m", [(3, 2), (200, 4), (1, 40)])
+def test_large_gradients_in_half_precision(n, m):
+    """ds passes fp16's largest value where the gradients do not."""
+    from faith_amd import ops
+    q, k, v, dout = tensors([n], [m], 2, 1, 64, F16, 22)
+    q, k, v = (q.float() / 16).to(F16), (k.float() / 16).to(F16), (v.float() * 4).to(F16)
+    dout = (dout.float().clamp(-3.9, 3.9) * 2.0 ** 14).to(F16)
+    if n > 100:
+        dout[1:] *= 2.0 ** -14          # one row large, the others not: a sum over rows stays in range
+    packing = ops.Packing([n], [m])
+    out, lse = ops.attention(q, k, v, packing, return_lse=True)
+    grads = ops.attention_backward(dout, q, k, v, out, lse, packing)
+    r = small_gradient_reference(q, k, v, dout, 0.125)
+    p = torch.softmax((q[:, 0].double() @ k[:, 0].double().t()) * 0.125, 1)
+    dp = dout[:, 0].double() @ v[:, 0].double().t()
+    assert float((p * (dp - (p * dp).sum(1, keepdim=True))).abs().max()) > (65504 if m < 40 else 0)
+    for i in (0, 1):
+        assert float(r[i][0].abs().max()) < 60000
+        R.check("dq dk".split()[i], grads[i], *r[i])
