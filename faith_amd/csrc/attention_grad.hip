@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         int lane = (int)threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
         const int half = lane >> 5, col = lane & 31;
-        const bool part = t0 < all_see;
+        // rows behind the last query are staged as zeros, whose scores with an infinite key are NaN
+        const bool part = t0 < all_see || t0 + BQ > it.q_len;
         // a query that sees one key only: p = 1 and dp = delta, exactly
         const bool alone_here = it.k_len == 1 || (g.causal && t0 <= -shift && -shift < t0 + BQ);
         // all scores of the tile first, so that the exponentials of one block of 32 queries can run beside the products of
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
             for (int b = 0; b < BQ / 32; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (t0 + 32 * b + row_of(r, half) < first) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
+                    if (const int i = t0 + 32 * b + row_of(r, half); i < first || i >= it.q_len) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
         }
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {

@@ -469,3 +469,40 @@ def test_large_gradients_in_half_precision(n, m):
     for i in (0, 1):
         assert float(r[i][0].abs().max()) < 60000
         R.check("dq dk".split()[i], grads[i], *r[i])
+
+
+@pytest.mark.parametrize("dtype, size", [(F32, 64), (F32, 128), (BF16, 32), (BF16, 64), (BF16, 96), (BF16, 128), (F16, 80)])
+@pytest.mark.parametrize("n, m, heads, kv_heads", [(1, 1, 2, 1), (5, 3, 2, 1), (33, 33, 4, 2), (1, 65, 8, 2), (200, 129, 2, 2), (3, 3000, 2, 1), (700, 700, 8, 8)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_behind_the_last_sequence_never_come_in(dtype, size, n, m, heads, kv_heads, causal):
+    """Neither through a tile's end nor through a load's: all arrays hold NaN behind their last row."""
+    from faith_amd import ops
+    q, k, v, dout = tensors([n], [m], heads, kv_heads, size, dtype, 31)
+    far = lambda t: torch.cat([t, torch.full((200, *t.shape[1:]), math.nan, device="cuda", dtype=dtype)])
+    qf, kf, vf, df = (far(t) for t in (q, k, v, dout))
+    packing = ops.Packing([n], [m])
+    want, lse = ops.attention(q, k, v, packing, causal, return_lse=True)
+    got, lse_far = ops.attention(qf, kf, vf, packing, causal, return_lse=True)
+    assert torch.equal(got[:n], want) and torch.equal(lse, lse_far) and bool(torch.isfinite(want).all())
+    a = ops.attention_backward(dout, q, k, v, want, lse, packing, causal)
+    b = ops.attention_backward(df, qf, kf, vf, far(want), lse, packing, causal)
+    assert all(torch.equal(x, y[:x.shape[0]]) and bool(torch.isfinite(x).all()) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype, size", [(F32, 64), (BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("n", [1, 33, 40, 200])
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_key_that_no_query_minds(dtype, size, n, causal):
+    """A key whose scores are all -infinity has no probability: its gradients are zero, whatever the length of the queries'
+    last tile."""
+    from faith_amd import ops
+    m = n + 3
+    q, k, v, dout = tensors([n], [m], 2, 1, size, dtype, 32)
+    q[:, :, 0] = -q[:, :, 0].abs() - 0.1
+    k[1, :, 0] = math.inf
+    packing = ops.Packing([n], [m])
+    out, lse = ops.attention(q, k, v, packing, causal, return_lse=True)
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+    _, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing, causal)
+    assert bool((dv[1] == 0).all()) and bool((dk[1] == 0).all())
+    assert bool(torch.isfinite(dk).all()) and bool(torch.isfinite(dv).all())
