@@ -41,13 +41,18 @@ __device__ __forceinline__ float wave_sum(float v) {
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     return v;
 }
+// The larger of two magnitudes, NaN above everything: the bits of numbers without a sign are in their order as integers
+__device__ __forceinline__ float larger(float a, float b) {
+    const unsigned x = __float_as_uint(a), y = __float_as_uint(b);
+    return __uint_as_float(x > y ? x : y);
+}
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, d));
+    for (int d = 32; d > 0; d >>= 1) v = larger(v, __shfl_xor(v, d));
     return v;
 }
 
-// Sums (or the largest) of a row over the wavefronts that share it.  `slot` has to differ between two calls that no other
+// Sums (or the largest magnitude) of a row over the wavefronts that share it.  `slot` has to differ between two calls that no other
 // barrier separates.
 template <int WAVES, bool MAX> __device__ __forceinline__ float across(float v, float *slot, int wave) {
     v = MAX ? wave_max(v) : wave_sum(v);
@@ -56,7 +61,7 @@ template <int WAVES, bool MAX> __device__ __forceinline__ float across(float v, 
     __syncthreads();
     v = slot[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v = MAX ? __builtin_fmaxf(v, slot[w]) : v + slot[w];
+    for (int w = 1; w < WAVES; ++w) v = MAX ? larger(v, slot[w]) : v + slot[w];
     return v;
 }
 
@@ -71,6 +76,7 @@ struct NormArgs {
     float eps;
 };
 
+// A row with a NaN has a scale of NaN, and every value divided by it is one; one with an infinity an infinite scale
 __device__ __forceinline__ float divided(float y, float scale) { return scale > 0.f ? y / scale : (scale == 0.f ? 0.f : y * scale); }
 __device__ __forceinline__ unsigned char to_int8(float t) {
     t = __builtin_rintf(t);
@@ -158,7 +164,7 @@ __global__ void __launch_bounds__(threads_of(WAVES)) residual_norm(const NormArg
             if (g.weight) y *= w[e];
             if (g.bias) y += b[e];
             h[c][e] = y;
-            top = __builtin_fmaxf(top, __builtin_fabsf(y));
+            top = larger(top, __builtin_fabsf(y));
         }
         if (!g.bits) pack(reinterpret_cast<T *>(g.y) + at + e0, h[c]);
     }
@@ -216,7 +222,7 @@ template <class T> __global__ void __launch_bounds__(256) residual_norm_any(cons
     float scale = 0.f;
     if (g.bits) {
         float top = 0.f;
-        for (int e = threadIdx.x; e < g.n; e += 256) top = __builtin_fmaxf(top, __builtin_fabsf(y_at(e, sum_at(e))));
+        for (int e = threadIdx.x; e < g.n; e += 256) top = larger(top, __builtin_fabsf(y_at(e, sum_at(e))));
         scale = across<4, true>(top, slot[2], wave) / steps_of(g.bits);
         if (threadIdx.x == 0) g.scales[blockIdx.x] = scale;
     }

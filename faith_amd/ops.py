@@ -1436,7 +1436,7 @@ def residual_norm(x, residual=None, weight=None, bias=None, kind="rms", eps=1e-6
         kind "no_var"    z = h - mean(h)
     float32, bfloat16 or float16, contiguous; weight and bias of x's type.  Returns (y, h); h is x itself without a residual.
     quantize "int8" / "e4m3": returns (q, scales, h), 8-bit values with a float32 scale for every row, y ~ q * scale,
-    scale = max |y| / 127 or / 448.  return_stats: one more result, what residual_norm_backward takes as `stats`."""
+    scale = max |y| / 127 or / 448 (NaN or infinite, and q * scale NaN, for a row that holds what is no number).  return_stats: one more result, what residual_norm_backward takes as `stats`."""
     if kind not in _lib.NORM_KINDS or not _alike(x, (residual,), (weight, bias)):
         _norm_operands(x, (("residual", residual),), (("weight", weight), ("bias", bias)), kind)
     n = x.shape[-1]

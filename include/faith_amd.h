@@ -703,7 +703,8 @@ int faith_attention_backward(const void *dout, const void *q, const void *k, con
  * residual, weight, bias may be NULL; sum (h, rounded to dtype; y is computed from the unrounded one), stats ([rows]: 1 / sqrt(...),
  * 1 for FAITH_NORM_NO_VAR; what the gradient needs) too.  bits != 0: y holds 8-bit values and scales [rows] their scales,
  * y ~ q * scale, scale = max |y| / 127 (FAITH_BITS_INT8) or / 448 (FAITH_BITS_E4M3, the OCP format), q rounded to nearest
- * even; a row of zeros has scale 0.  A NaN in y becomes 0 in int8 and stays NaN in e4m3.
+ * even; a row of zeros has scale 0.  A row of y that holds a NaN has scale NaN, one that holds an infinity and no NaN scale infinity:
+ * q * scale is then NaN along the whole row (q: 0 where int8 or a finite y over infinity, NaN otherwise).
  */
 #define FAITH_NORM_RMS       0
 #define FAITH_NORM_STANDARD  1

@@ -250,3 +250,13 @@ def test_what_breaks_the_answer_in_half_precision_lies_in_the_ball(monkeypatch, 
     assert not found[0] and len(seen) == 11
     for d in seen:
         assert bool((torch.linalg.vector_norm(d, ord=p, dim=1) <= torch.tensor(radii, device="cuda", dtype=torch.float64)).all())
+
+
+def test_eight_bit_activations_do_not_hide_what_is_no_number():
+    from faith_amd import concrete
+    net = network(9, "standard", hidden=128)
+    xs = sentences([30, 64], 10, 128)
+    xs[0][4, 7] = math.nan
+    for bits in (None, "int8", "e4m3"):
+        got = concrete.logits(net, torch.cat(xs), [30, 64], activations=bits)
+        assert bool(torch.isnan(got[0]).all()) and bool(torch.isfinite(got[1]).all())

@@ -205,3 +205,28 @@ def test_leading_axes_and_refusals():
         ops.residual_norm_backward(dy, x, w, flat[2][:3], "standard")
     with pytest.raises(ValueError, match="dy"):
         ops.residual_norm_backward(dy[:3], x, w, flat[2], "standard")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bits", ["int8", "e4m3"])
+@pytest.mark.parametrize("kind", ["rms", "standard", "no_var"])
+@pytest.mark.parametrize("n", [64, 63, 1032, 4096, 8200, 20000])
+def test_eight_bits_of_rows_that_hold_no_numbers(n, kind, bits, dtype):
+    """A row with a NaN, or with an infinity, stands for no number anywhere: no finite scale, NaN in e4m3, and NaN whichever way it
+    is read back.  On the way that keeps the row in registers and on that for any width."""
+    from faith_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(6, n, generator=g, device="cuda").to(dtype)
+    clean = ops.residual_norm(x, None, None, None, kind, quantize=bits)
+    x[1, 3], x[2, n - 1], x[4, 5] = math.nan, math.inf, -math.inf
+    q, scales, _ = ops.residual_norm(x, None, None, None, kind, quantize=bits)
+    for row in (1, 2, 4):
+        assert bool(torch.isnan(scales[row])) and bool(torch.isnan(q[row].float() * scales[row]).all())
+        assert bool((q[row].float() == 0).all()) if bits == "int8" else bool(torch.isnan(q[row].float()).all())
+    for row in (0, 3, 5):
+        assert torch.equal(q[row].float(), clean[0][row].float()) and torch.equal(scales[row], clean[1][row])
+    # an infinite weight: an infinity, and none of the row's numbers has a finite scale
+    w = torch.ones(n, device="cuda", dtype=dtype)
+    w[7] = math.inf
+    q, scales, _ = ops.residual_norm(x[:1], None, w, None, kind, quantize=bits)
+    assert not bool(torch.isfinite(scales).any()) and bool(torch.isnan(q.float() * scales[:, None]).all())
