@@ -198,14 +198,11 @@ template <int DP, Reads READS> __device__ __forceinline__ float column_element(c
     }
 }
 
-// acc[r] += sum_d tile[row_of(r)][d] * b[d]: the 32 rows from row0 on against this lane's column, whose values are in `b`
+// acc[r] + sum_d tile[row_of(r)][d] * b[d]: the 32 rows from row0 on against this lane's column, whose values are in `b`
 template <class T, int DP> struct ColumnRegs { typename Vec<T>::x8 v[DP / 16]; };
 template <int DP> struct ColumnRegs<float, DP> { floatx4 v[DP / 8]; };
 
-template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(const T *tile, int row0, int col, int half, const ColumnRegs<T, DP> &b) {
-    floatx16 acc;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(const T *tile, int row0, int col, int half, const ColumnRegs<T, DP> &b, floatx16 acc) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int u = 0; u < DP / 8; ++u) {
@@ -218,6 +215,13 @@ template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(co
         for (int u = 0; u < DP / 16; ++u) acc = mfma(row_fragment<T, DP>(tile, row0, col, u, half), b.v[u], acc);
     }
     return acc;
+}
+
+template <class T, int DP> __device__ __forceinline__ floatx16 rows_by_column(const T *tile, int row0, int col, int half, const ColumnRegs<T, DP> &b) {
+    floatx16 none;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) none[r] = 0.f;
+    return rows_by_column<T, DP>(tile, row0, col, half, b, none);
 }
 
 // the values of one row (DP of them, zero behind `size`) in the order in which rows_by_column takes them; all loads first, with
@@ -305,27 +309,27 @@ __device__ __forceinline__ float sum_halves(float v) {
     return __uint_as_float(a) + __uint_as_float(b);
 }
 
-// Other values (fp16): a power of two for each column, 2^up, under which the largest of the column so far lies in [2^7, 2^15].  It starts
-// higher than any value asks for and only falls; the sums follow it.  13 sequences of 37 ... 1021, 12 heads of 80, forward and
-// gradients: 199 us with it, 190 without; 2048 keys and gradients of 2^-13: dq off by 0.38 %, all of it its own rounding, instead of 2.2.
-constexpr int UP_MOST = 120;
-template <int DP> __device__ __forceinline__ void raise(floatx16 &s, floatx16 (&acc)[DP / 32], int &up) {
+// Other values (fp16): a power of two for each column, 2^up, with which s comes here, and under which the largest of the column so far
+// lies at most at 2^15.  It starts higher than any value asks for (ds is at most 2^40: products of two fp16 values over 128 places) and
+// only falls, to where that value lies in [2^7, 2^8); the sums follow it.  13 sequences of 37 ... 1021, 12 heads of 80, forward and
+// gradients: 192 us with it, 187 without; 2048 keys and gradients of 2^-13: dq off by 0.38 %, all of it its own rounding, instead of 2.2.
+constexpr int UP_MOST = 80;
+template <int DP> __device__ __forceinline__ void follow(floatx16 &s, floatx16 (&acc)[DP / 32], int &up) {
     float top = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, __builtin_fabsf(s[r]));
-    if (__any(__builtin_ldexpf(top, up) > 32768.f)) {
+    if (__any(top > 32768.f)) {
         top = max_halves(top);
-        const int want = 8 - __builtin_amdgcn_frexp_expf(top), now = __builtin_ldexpf(top, up) > 32768.f && want < up ? want : up;
-        const float f = __builtin_ldexpf(1.f, now - up);
-        up = now;
+        const int down = top > 32768.f ? 8 - __builtin_amdgcn_frexp_expf(top) : 0;
+        const float f = __builtin_ldexpf(1.f, down);
+        up += down;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= f;
 #pragma unroll
         for (int m = 0; m < DP / 32; ++m)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[m][r] *= f;
     }
-    const float f = __builtin_ldexpf(1.f, up);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= f;
 }
 // acc times 2^-up
 template <int DP> __device__ __forceinline__ void lower(floatx16 (&acc)[DP / 32], int up) {

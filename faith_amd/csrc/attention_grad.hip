@@ -2,7 +2,7 @@
 //     p = exp(s - lse),  dp = do . v,  ds = p (dp - delta),  delta = do . out
 //     dq = scale sum_j ds k,   dk = scale sum_{i, heads of the group} ds q,   dv = sum_{i, heads of the group} p do
 // p and ds are held in 32 bits and rounded once, to the elements' type, as operands of the last three products (in fp16 times a power
-// of two that keeps them in its range, see raise() in attention.h); delta comes from the output as it was stored.  Against one rounding of each result these are two or three independent ones of the same size:
+// of two that keeps them in its range, see follow() in attention.h); delta comes from the output as it was stored.  Against one rounding of each result these are two or three independent ones of the same size:
 // 1.4 times the error of a computation in 32 bits at a few hundred keys, up to twice at a handful.
 // Two launches (a third joins parts where the plan cuts) and no atomics, so that the same call gives the same bits: one goes over the keys for a tile of query rows (and
 // leaves delta and the logarithm of the row's sum, in powers of two, to the other), one over the queries of all heads of the
@@ -20,7 +20,7 @@ struct GradArgs {
     const void *dout, *q, *k, *v, *out;
     const float *lse;
     void *dq, *dk, *dv;
-    float *stat;                             // [2][heads][lse_hs]: lse in powers of two less probability_up(), delta
+    float *stat;                             // [2][heads][lse_hs]: lse in powers of two less probability_up(); delta (fp16: -delta)
     float *part;                             // [slots][key heads][keys of an item][2 DP]: parts of dk and dv
     const Item *items;
     Deal deal;
@@ -116,13 +116,12 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
 #pragma unroll
         for (int e = 0; e < PER; ++e) delta = fmaf((float)o.v[u][e], (float)d_o.v[u][e], delta);
     delta = sum_halves(delta);
-    // a row that sees no key: every p below is masked.  p comes out times 2^probability_up(), and so does ds
-    const float lse = l == -__builtin_inff() ? 0.f : fmaf(l, 1.4426950408889634f, -(float)probability_up<T>());
-    int up = UP_MOST;                        // of ds, fp16
+    const float lse = l == -__builtin_inff() ? 0.f : l * 1.4426950408889634f;      // a row that sees no key: every p below is masked
+    int up = probability_up<T>() ? UP_MOST : 0;      // p comes out times 2^up, and so does ds
     if (row < rows && half == 0 && (!SPLIT || wave == 0)) {
         float *s = g.stat + (long long)head * g.lse_hs + place;
-        s[0] = lse;
-        s[(long long)g.kv_heads * g.group * g.lse_hs] = delta;
+        s[0] = lse - probability_up<T>();
+        s[(long long)g.kv_heads * g.group * g.lse_hs] = probability_up<T>() ? -delta : delta;
     }
     auto tile = [&](const T *kt, const T *vt, int key0) {
         if (key0 > any_sees) return;
@@ -132,13 +131,13 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
             floatx16 s = rows_by_column<T, DP>(kt + own, 32 * b, col, half, q);
             const floatx16 dp = rows_by_column<T, DP>(vt + own, 32 * b, col, half, d_o);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], g.c, -lse)) * (dp[r] - delta);
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], g.c, (float)up - lse)) * (dp[r] - delta);
             if (part) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (key0 + 32 * b + row_of(r, half) > last) s[r] = 0.f;
             }
-            if constexpr (probability_up<T>() > 0) raise<DP>(s, dq, up);
+            if constexpr (probability_up<T>() > 0) follow<DP>(s, dq, up);
             columns_by_result<T, DP>(dq, kt + own, 32 * b, lane, s);
         }
     };
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         alone<2 * St::LOADS, ONCE>(first, WAVES * BN, it.end,
                              [&](int n, int key0) { n ? stage(k1, v1, key0) : stage(k0, v0, key0); },
                              [&](int n, int key0) { n ? tile(k1, v1, key0) : tile(k0, v0, key0); });
-        if constexpr (probability_up<T>() > 0) lower<DP>(dq, up + probability_up<T>());
+        if constexpr (probability_up<T>() > 0) lower<DP>(dq, up);
         add_waves<WAVES, DP, ALL * (int)sizeof(T) / 4>(dq, reinterpret_cast<float *>(k0), reinterpret_cast<float *>(v0), wave, lane);
         if (wave > 0) return;
     } else if (it.begin < it.end) {
@@ -159,14 +158,14 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
             if (key0 + 2 * BN < it.end) stage(k0, v0, key0 + 2 * BN);
             tile(k1, v1, key0 + BN);
         }
-        if constexpr (probability_up<T>() > 0) lower<DP>(dq, up + probability_up<T>());
+        if constexpr (probability_up<T>() > 0) lower<DP>(dq, up);
     }
     if (g.causal && any_not_finite<DP>(dq)) {
         // see one_row in attention.hip: what the mask hides may have come in as 0 * NaN
         clear<DP>(dq);
         for (int j = 0; j <= last; ++j) {
             const T *kr = kb + (long long)j * g.k_ts;
-            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qrow, kr, g.size), g.c, -lse - probability_up<T>()));
+            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qrow, kr, g.size), g.c, -lse));
             add_row<T, DP>(dq, kr, p * (dot_rows(dorow, vb + (long long)j * g.v_ts, g.size) - delta), half, g.size);
         }
     }
@@ -210,7 +209,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
     floatx16 dk[DP / 32], dv[DP / 32];
     clear<DP>(dk);
     clear<DP>(dv);
-    int up = UP_MOST;                        // of ds, fp16
+    int up = UP_MOST - probability_up<T>();  // of ds beyond that of p, fp16
     St qs, ds;
     qs.init(lane, staged, g.size, g.q_ts);
     ds.init(lane, staged, g.size, g.do_ts);
@@ -236,8 +235,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         int lane = (int)threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
         const int half = lane >> 5, col = lane & 31;
-        // rows behind the last query are staged as zeros, whose scores with an infinite key are NaN
-        const bool part = t0 < all_see || t0 + BQ > it.q_len;
+        const bool part = t0 < all_see;
         // a query that sees one key only: p = 1 and dp = delta, exactly
         const bool alone_here = it.k_len == 1 || (g.causal && t0 <= -shift && -shift < t0 + BQ);
         // all scores of the tile first, so that the exponentials of one block of 32 queries can run beside the products of
@@ -250,24 +248,54 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
 #pragma unroll
                 for (int u = 0; u < DP / 16; ++u) v.v[u] = row_fragment<T, DP>(v_rows + wave * 32 * DP, 0, col, u, half);
             }
-            dp[b] = rows_by_column<T, DP>(dt, 32 * b, col, half, v);
+            if constexpr (probability_up<T>() > 0) {
+                floatx16 minus_delta;
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const floatx4 e = *reinterpret_cast<const floatx4 *>(et + 32 * b + row_of(r, half));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) minus_delta[r + i] = e[i];
+                }
+                dp[b] = rows_by_column<T, DP>(dt, 32 * b, col, half, v, minus_delta);
+            } else {
+                dp[b] = rows_by_column<T, DP>(dt, 32 * b, col, half, v);
+            }
         }
         if (part) {
 #pragma unroll
             for (int b = 0; b < BQ / 32; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (const int i = t0 + 32 * b + row_of(r, half); i < first || i >= it.q_len) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
+                    if (t0 + 32 * b + row_of(r, half) < first) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
+        }
+        // Rows behind the last query are staged as zeros.  Their scores are zeros too, and do no harm, unless the key is not finite: then they
+        // are NaN, the last of the tile's among them
+        if (t0 + BQ > it.q_len && __builtin_expect(__any(s[BQ / 32 - 1][15] != s[BQ / 32 - 1][15]), 0)) {
+#pragma unroll
+            for (int b = 0; b < BQ / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t0 + 32 * b + row_of(r, half) >= it.q_len) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
         }
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const floatx4 l = *reinterpret_cast<const floatx4 *>(lt + 32 * b + row_of(r, half)), e = *reinterpret_cast<const floatx4 *>(et + 32 * b + row_of(r, half));
+                const floatx4 l = *reinterpret_cast<const floatx4 *>(lt + 32 * b + row_of(r, half));
+                if constexpr (probability_up<T>() > 0) {
+                    const float lift = __builtin_ldexpf(1.f, up);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[b][r + i] = __builtin_amdgcn_exp2f(fmaf(s[b][r + i], g.c, -l[i]));
-                    dp[b][r + i] = s[b][r + i] * (dp[b][r + i] - e[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        s[b][r + i] = __builtin_amdgcn_exp2f(fmaf(s[b][r + i], g.c, -l[i]));
+                        dp[b][r + i] *= s[b][r + i] * lift;
+                    }
+                } else {
+                    const floatx4 e = *reinterpret_cast<const floatx4 *>(et + 32 * b + row_of(r, half));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[b][r + i] = __builtin_amdgcn_exp2f(fmaf(s[b][r + i], g.c, -l[i]));
+                        dp[b][r + i] = s[b][r + i] * (dp[b][r + i] - e[i]);
+                    }
                 }
             }
             if (alone_here) {
@@ -276,7 +304,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                     if (it.k_len == 1 || t0 + 32 * b + row_of(r, half) == -shift) dp[b][r] = 0.f;
             }
             columns_by_result<T, DP>(dv, dt, 32 * b, lane, s[b]);
-            if constexpr (probability_up<T>() > 0) raise<DP>(dp[b], dk, up);
+            if constexpr (probability_up<T>() > 0) follow<DP>(dp[b], dk, up);
             columns_by_result<T, DP>(dk, qt, 32 * b, lane, dp[b]);
         }
     };
@@ -331,7 +359,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                 const float *s = g.stat + (long long)h * g.lse_hs + place;
                 const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, krow, g.size), g.c, -s[0] - probability_up<T>()));
                 add_row<T, DP>(dv, dr, p, half, g.size);
-                add_row<T, DP>(dk, qr, p * (dot_rows(dr, vrow, g.size) - s[stat_hs]), half, g.size);
+                add_row<T, DP>(dk, qr, p * (dot_rows(dr, vrow, g.size) + (probability_up<T>() ? s[stat_hs] : -s[stat_hs])), half, g.size);
             }
     }
     if (key >= it.k_len) return;

@@ -1266,9 +1266,7 @@ def _known_call(packing, which, causal, q, k, v, *more):
         return None, None
 
 
-def _scale(scale, size):
-    if scale is None:
-        return 1.0 / math.sqrt(size)
+def _scale(scale):
     scale = float(scale)
     if not 0 < scale < 1e30:
         raise ValueError(f"scale={scale}: must be positive and finite")
@@ -1310,11 +1308,11 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
             if heads > 1 and (oh < size or (ot < (heads - 1) * oh + size and oh < (packing.tokens - 1) * ot + size and packing.tokens > 1)):
                 raise ValueError(f"out: its rows and heads must not overlap (strides {out.stride()})")
         known = (plan, floats, heads, (items, n, joins, kind, qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size,
-                                       _DTYPES[q.dtype], int(causal)), size)
+                                       _DTYPES[q.dtype], int(causal)), 1.0 / math.sqrt(size))
         if key is not None:
             packing._calls[key] = known
-    plan, floats, heads, rest, size = known
-    scale = _scale(scale, size)
+    plan, floats, heads, rest, usual = known
+    scale = usual if scale is None else _scale(scale)
     if out is None:
         out = _like_rows(q, packing.tokens)
     lse = _empty(heads, packing.tokens, device=dev) if return_lse else None
@@ -1348,11 +1346,11 @@ def attention_backward(dout, q, k, v, out, lse, packing, causal=False, scale=Non
             plans = [packing.plan(which, heads, kv_heads, q.element_size(), size, causal) for which in (_lib.ATTENTION_GRAD_QUERIES, _lib.ATTENTION_GRAD_KEYS)]
         floats = plans[1][4] * kv_heads * (32 if plans[1][5] else 128) * 2 * ((size + 31) // 32 * 32)
         known = (plans, floats, heads, (plans[0][1], plans[0][2], plans[0][5], *plans[1][1:6], ctypes.addressof(strides), packing.tokens, heads, kv_heads,
-                                size, _DTYPES[q.dtype], int(causal)), size, strides)
+                                size, _DTYPES[q.dtype], int(causal)), 1.0 / math.sqrt(size), strides)
         if key is not None and dout.shape == q.shape and out.shape == q.shape:
             packing._calls[key] = known
-    plans, floats, heads, rest, size, _ = known
-    scale = _scale(scale, size)
+    plans, floats, heads, rest, usual, _ = known
+    scale = usual if scale is None else _scale(scale)
     _check("lse", lse, (heads, packing.tokens))
     dev = packing.device
     if lse.get_device() != dev.index:
