@@ -314,17 +314,21 @@ __device__ __forceinline__ float sum_halves(float v) {
 // only falls, to where that value lies in [2^7, 2^8); the sums follow it.  13 sequences of 37 ... 1021, 12 heads of 80, forward and
 // gradients: 192 us with it, 187 without; 2048 keys and gradients of 2^-13: dq off by 0.38 %, all of it its own rounding, instead of 2.2.
 constexpr int UP_MOST = 80;
-template <int DP> __device__ __forceinline__ void follow(floatx16 &s, floatx16 (&acc)[DP / 32], int &up) {
+template <int DP, int N> __device__ __forceinline__ void follow(floatx16 (&s)[N], floatx16 (&acc)[DP / 32], int &up) {
     float top = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, __builtin_fabsf(s[r]));
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, __builtin_fabsf(s[b][r]));
     if (__any(top > 32768.f)) {
         top = max_halves(top);
         const int down = top > 32768.f ? 8 - __builtin_amdgcn_frexp_expf(top) : 0;
         const float f = __builtin_ldexpf(1.f, down);
         up += down;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= f;
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] *= f;
 #pragma unroll
         for (int m = 0; m < DP / 32; ++m)
 #pragma unroll
@@ -337,6 +341,58 @@ template <int DP> __device__ __forceinline__ void lower(floatx16 (&acc)[DP / 32]
     for (int m = 0; m < DP / 32; ++m)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[m][r] = __builtin_ldexpf(acc[m][r], -up);
+}
+
+// ------------------------------------------------------------------------------------------ what a mask hides
+// A mask may hide anything, and the products above multiply what it hides by zero, which NaN and infinity survive.  A wavefront whose
+// causal result is not finite therefore looks at what was hidden from its rows, the ends of one or two tiles, and only if that holds
+// what is no number, does its rows again: every lane its own row over what the row sees, in 32 bits and on the vector units.  A NaN that is seen
+// is in the first result, and costs nothing beyond the look; so does an input that is NaN throughout, whose rows know it from their sums.
+// The slow way is some 140 times the first pass: 4096 causal tokens, 32 / 8 heads of 128, bf16, every value NaN and no key: 22 ms instead of 0.16.
+template <class T> __device__ __forceinline__ bool rows_not_finite(const T *base, long long stride, int from, int to, int size, int lane) {
+    bool bad = false;
+    for (int i = from; i < to; ++i)
+        for (int d = lane; d < size; d += 64) bad |= !(__builtin_fabsf((float)base[i * stride + d]) < __builtin_inff());
+    return __any(bad);
+}
+// rows start on 16 bytes and are whole groups of them
+template <class T> __device__ __forceinline__ float dot_rows(const T *a, const T *b, int size) {
+    constexpr int PER = 16 / (int)sizeof(T);
+    typedef T group __attribute__((ext_vector_type(PER)));
+    float s = 0.f;
+#pragma unroll 2
+    for (int d = 0; d < size; d += PER) {
+        const group x = *reinterpret_cast<const group *>(a + d), y = *reinterpret_cast<const group *>(b + d);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) s = fmaf((float)x[e], (float)y[e], s);
+    }
+    return s;
+}
+// o += f * row, for this lane's registers (those behind the head's size are not stored)
+template <class T, int DP> __device__ __forceinline__ void add_row(floatx16 (&o)[DP / 32], const T *row, float f, int half, int size) {
+    typedef T four __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m) {
+        __builtin_amdgcn_sched_barrier(0);           // a block's loads at a time: no registers for speed here
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * m + row_of(r, half);
+            const four v = *reinterpret_cast<const four *>(row + (d < size ? d : 0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[m][r + i] = fmaf(f, (float)v[i], o[m][r + i]);
+        }
+    }
+}
+
+// Wavefronts on a SIMD that a kernel is compiled for: as many as LDS and the registers of its tiles' loop allow.  (Left to itself the compiler takes
+// more registers for what comes behind the loop.)
+enum Pass { FORWARD, GRAD_QUERIES, GRAD_KEYS };
+constexpr int resident(Pass pass, int kind, int element_size, int padded) {
+    constexpr int N[3][2][4][3] = {        // pass; elements of 2, 4 bytes; heads of 32, 64, 96, 128; ROWS, KEYS, ONCE
+        {{{4, 4, 4}, {3, 2, 4}, {2, 1, 3}, {2, 1, 2}}, {{4, 2, 4}, {4, 1, 2}, {3, 1, 2}, {2, 1, 1}}},
+        {{{4, 3, 5}, {4, 2, 5}, {3, 1, 3}, {2, 1, 2}}, {{4, 2, 4}, {3, 1, 2}, {1, 1, 2}, {1, 1, 1}}},
+        {{{2, 3, 5}, {2, 2, 4}, {2, 1, 3}, {2, 1, 2}}, {{3, 2, 4}, {2, 1, 2}, {1, 1, 2}, {1, 1, 1}}}};
+    return N[pass][element_size / 4][padded / 32 - 1][kind];
 }
 
 // Wavefronts of a workgroup that share their columns and divide the reduction, each with tiles of its own: four, unless their

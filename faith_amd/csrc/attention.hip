@@ -36,42 +36,24 @@ struct FwdArgs {
     float c;                                 // scale * log2(e)
 };
 
-// The softmax of one row over keys that this lane goes over by itself, in fp32 throughout: the way taken for the rows of a
-// wavefront whose result came out not finite.  The products above multiply masked values by zero, which a NaN or an
-// infinity in a place that the mask hides survives; this loop never touches what is masked.
+// The output of one row over the keys that it sees, by this lane alone (see "what a mask hides" in attention.h); its reference stands, for
+// a score that is hidden is replaced, not multiplied.
 template <class T, int DP>
-__device__ void one_row(const FwdArgs &g, const Item &it, int hk, const T *qrow, int last, int half, float *ref, float *sum, floatx16 (&o)[DP / 32]) {
+__device__ void one_row(const FwdArgs &g, const Item &it, int hk, const T *qrow, int last, int half, float ref, floatx16 (&o)[DP / 32]) {
     const T *k = reinterpret_cast<const T *>(g.k) + (long long)hk * g.k_hs, *v = reinterpret_cast<const T *>(g.v) + (long long)hk * g.v_hs;
     const int end = it.end < last + 1 ? it.end : last + 1;
-    float top = LOWEST, l = 0.f;
 #pragma unroll
     for (int m = 0; m < DP / 32; ++m)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[m][r] = 0.f;
-    for (int pass = 0; pass < 2; ++pass)
-        for (int j = it.begin; j < end; ++j) {
-            const T *kr = k + (long long)(it.k_start + j) * g.k_ts;
-            float s = 0.f;
-            for (int d = 0; d < g.size; ++d) s = fmaf((float)qrow[d], (float)kr[d], s);
-            s *= g.c;
-            if (pass == 0) { top = s > top ? s : top; continue; }
-            const float p = __builtin_amdgcn_exp2f(s - top);
-            l += p;
-            const T *vr = v + (long long)(it.k_start + j) * g.v_ts;
-#pragma unroll
-            for (int m = 0; m < DP / 32; ++m)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = 32 * m + row_of(r, half);
-                    if (d < g.size) o[m][r] = fmaf(p, (float)vr[d], o[m][r]);
-                }
-        }
-    *ref = top;
-    *sum = l;
+    for (int j = it.begin; j < end; ++j) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qrow, k + (long long)(it.k_start + j) * g.k_ts, g.size), g.c, -ref));
+        add_row<T, DP>(o, v + (long long)(it.k_start + j) * g.v_ts, p, half, g.size);
+    }
 }
 
 template <class T, int DP, int BN, int KIND, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, (KIND == KIND_KEYS && DP * sizeof(T) >= 192) || (KIND == KIND_ONCE && DP * sizeof(T) >= 512) ? 1 : 2) attention_forward(const FwdArgs g) {
+__global__ void __launch_bounds__(64 * WAVES, resident(FORWARD, KIND, sizeof(T), DP)) attention_forward(const FwdArgs g) {
     constexpr bool KEYS = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
     constexpr int TILE = BN * DP, ALL = TILE * (KEYS ? WAVES : 1);
     typedef Stager<T, DP, BN, KEYS ? 1 : 4> St;                     // keys: read by rows
@@ -288,7 +270,10 @@ __global__ void __launch_bounds__(64 * WAVES, (KIND == KIND_KEYS && DP * sizeof(
         for (int m = 0; m < DP / 32; ++m)
 #pragma unroll
             for (int r = 0; r < 16; ++r) bad = fmaf(0.f, o[m][r], bad);      // finite values leave it finite
-        if (__any(!(__builtin_fabsf(bad) < __builtin_inff()))) one_row<T, DP>(g, it, hk, qrow, last, half, &ref, &sum, o);
+        // not where every row's own scores are NaN; nor where nothing that was hidden is to blame
+        if (__any(!(__builtin_fabsf(bad) < __builtin_inff())) && __any(sum == sum) &&
+            rows_not_finite(vb, g.v_ts, all_see + 1 > it.begin ? all_see + 1 : it.begin, it.k_len < any_sees + BN ? it.k_len : any_sees + BN, g.size, lane))
+            one_row<T, DP>(g, it, hk, qrow, last, half, ref, o);
     }
     if (row >= rows) return;
     if (it.slot >= 0) {

@@ -33,12 +33,6 @@ template <class T> __device__ __forceinline__ const T *at(const void *base, long
     return reinterpret_cast<const T *>(base) + row * ts + (long long)head * hs;
 }
 
-template <class T> __device__ __forceinline__ float dot_rows(const T *a, const T *b, int n) {
-    float s = 0.f;
-    for (int d = 0; d < n; ++d) s = fmaf((float)a[d], (float)b[d], s);
-    return s;
-}
-
 template <int DP> __device__ __forceinline__ void clear(floatx16 (&o)[DP / 32]) {
 #pragma unroll
     for (int m = 0; m < DP / 32; ++m)
@@ -53,20 +47,9 @@ template <int DP> __device__ __forceinline__ bool any_not_finite(const floatx16 
         for (int r = 0; r < 16; ++r) bad = fmaf(0.f, o[m][r], bad);
     return __any(bad != 0.f);                // 0 * NaN, 0 * infinity
 }
-// o += f * row, for this lane's registers
-template <class T, int DP> __device__ __forceinline__ void add_row(floatx16 (&o)[DP / 32], const T *row, float f, int half, int size) {
-#pragma unroll
-    for (int m = 0; m < DP / 32; ++m)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int d = 32 * m + row_of(r, half);
-            if (d < size) o[m][r] = fmaf(f, (float)row[d], o[m][r]);
-        }
-}
-
 // SPLIT: the wavefronts share 32 rows and divide the keys, as in attention.hip
 template <class T, int DP, int BN, int KIND, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_grad_queries(const GradArgs g) {
+__global__ void __launch_bounds__(64 * WAVES, resident(GRAD_QUERIES, KIND, sizeof(T), DP)) attention_grad_queries(const GradArgs g) {
     constexpr bool SPLIT = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
     constexpr int TILE = BN * DP, ALL = TILE * (SPLIT ? WAVES : 1);
     typedef Stager<T, DP, BN, SPLIT ? 1 : WAVES> St;
@@ -128,7 +111,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         const bool part = key0 + BN - 1 > all_see;
 #pragma unroll
         for (int b = 0; b < BN / 32; ++b) {
-            floatx16 s = rows_by_column<T, DP>(kt + own, 32 * b, col, half, q);
+            floatx16 one[1] = {rows_by_column<T, DP>(kt + own, 32 * b, col, half, q)}, &s = one[0];
             const floatx16 dp = rows_by_column<T, DP>(vt + own, 32 * b, col, half, d_o);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], g.c, (float)up - lse)) * (dp[r] - delta);
@@ -137,7 +120,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                 for (int r = 0; r < 16; ++r)
                     if (key0 + 32 * b + row_of(r, half) > last) s[r] = 0.f;
             }
-            if constexpr (probability_up<T>() > 0) follow<DP>(s, dq, up);
+            if constexpr (probability_up<T>() > 0) follow<DP>(one, dq, up);
             columns_by_result<T, DP>(dq, kt + own, 32 * b, lane, s);
         }
     };
@@ -160,8 +143,9 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
         }
         if constexpr (probability_up<T>() > 0) lower<DP>(dq, up);
     }
-    if (g.causal && any_not_finite<DP>(dq)) {
-        // see one_row in attention.hip: what the mask hides may have come in as 0 * NaN
+    if (g.causal && any_not_finite<DP>(dq) && __any(lse == lse) &&
+        rows_not_finite(kb, g.k_ts, all_see + 1 > 0 ? all_see + 1 : 0, it.k_len < any_sees + BN ? it.k_len : any_sees + BN, g.size, lane)) {
+        // see "what a mask hides" in attention.h
         clear<DP>(dq);
         for (int j = 0; j <= last; ++j) {
             const T *kr = kb + (long long)j * g.k_ts;
@@ -175,7 +159,7 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
 }
 
 template <class T, int DP, int BQ, int KIND, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_grad_keys(const GradArgs g) {
+__global__ void __launch_bounds__(64 * WAVES, resident(GRAD_KEYS, KIND, sizeof(T), DP)) attention_grad_keys(const GradArgs g) {
     constexpr bool SPLIT = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
     constexpr int TILE = BQ * DP, EACH = SPLIT ? WAVES : 1, ALL = TILE * EACH;
     typedef Stager<T, DP, BQ, SPLIT ? 1 : WAVES> St;
@@ -261,22 +245,6 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                 dp[b] = rows_by_column<T, DP>(dt, 32 * b, col, half, v);
             }
         }
-        if (part) {
-#pragma unroll
-            for (int b = 0; b < BQ / 32; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (t0 + 32 * b + row_of(r, half) < first) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
-        }
-        // Rows behind the last query are staged as zeros.  Their scores are zeros too, and do no harm, unless the key is not finite: then they
-        // are NaN, the last of the tile's among them
-        if (t0 + BQ > it.q_len && __builtin_expect(__any(s[BQ / 32 - 1][15] != s[BQ / 32 - 1][15]), 0)) {
-#pragma unroll
-            for (int b = 0; b < BQ / 32; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (t0 + 32 * b + row_of(r, half) >= it.q_len) { s[b][r] = -__builtin_inff(); dp[b][r] = 0.f; }
-        }
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
 #pragma unroll
@@ -298,13 +266,35 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
                     }
                 }
             }
-            if (alone_here) {
+        }
+        // hidden: replaced behind the exponential, whatever the row's sum and delta are
+        if (part) {
+#pragma unroll
+            for (int b = 0; b < BQ / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t0 + 32 * b + row_of(r, half) < first) s[b][r] = dp[b][r] = 0.f;
+        }
+        // Rows behind the last query are staged as zeros.  Their scores are zeros too, and do no harm, unless the key is not finite: then they
+        // are NaN, the last of the tile's among them
+        if (t0 + BQ > it.q_len && __builtin_expect(__any(s[BQ / 32 - 1][15] != s[BQ / 32 - 1][15]), 0)) {
+#pragma unroll
+            for (int b = 0; b < BQ / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t0 + 32 * b + row_of(r, half) >= it.q_len) s[b][r] = dp[b][r] = 0.f;
+        }
+        if (alone_here) {
+#pragma unroll
+            for (int b = 0; b < BQ / 32; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (it.k_len == 1 || t0 + 32 * b + row_of(r, half) == -shift) dp[b][r] = 0.f;
-            }
+        }
+        if constexpr (probability_up<T>() > 0) follow<DP>(dp, dk, up);
+#pragma unroll
+        for (int b = 0; b < BQ / 32; ++b) {
             columns_by_result<T, DP>(dv, dt, 32 * b, lane, s[b]);
-            if constexpr (probability_up<T>() > 0) follow<DP>(dp[b], dk, up);
             columns_by_result<T, DP>(dk, qt, 32 * b, lane, dp[b]);
         }
     };
@@ -349,7 +339,21 @@ __global__ void __launch_bounds__(64 * WAVES, KIND == KIND_KEYS || (sizeof(T) ==
             lower<DP>(dv, probability_up<T>());
         }
     }
-    if (g.causal && (any_not_finite<DP>(dk) || any_not_finite<DP>(dv))) {
+    // hidden from some of this wavefront's keys: the queries that see the first but not the last of them, and the tile's in front of those
+    auto hidden_not_finite = [&]() {
+        const int from = any_sees - BQ > it.begin ? any_sees - BQ : it.begin, to = all_see < it.q_len ? all_see : it.q_len;
+        // the last query sees every key: where its sum is NaN, so are all gradients
+        const float last = g.stat[(long long)(hk * g.group + h_first) * g.lse_hs + it.q_start + it.q_len - 1];
+        if (last != last) return false;
+        bool bad = false;
+        for (int h = hk * g.group + h_first; h < hk * g.group + h_first + h_count; ++h) {
+            bad = bad || rows_not_finite(at<T>(g.q, it.q_start, g.q_ts, h, g.q_hs), g.q_ts, from, to, g.size, lane) ||
+                  rows_not_finite(at<T>(g.dout, it.q_start, g.do_ts, h, g.do_hs), g.do_ts, from, to, g.size, lane);
+        }
+        return bad;
+    };
+    if (g.causal && (any_not_finite<DP>(dk) || any_not_finite<DP>(dv)) && hidden_not_finite()) {
+        // see "what a mask hides" in attention.h
         clear<DP>(dk);
         clear<DP>(dv);
         for (int h = hk * g.group + h_first; h < hk * g.group + h_first + h_count; ++h)

@@ -506,3 +506,87 @@ def test_a_key_that_no_query_minds(dtype, size, n, causal):
     _, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, packing, causal)
     assert bool((dv[1] == 0).all()) and bool((dk[1] == 0).all())
     assert bool(torch.isfinite(dk).all()) and bool(torch.isfinite(dv).all())
+
+
+def attention_where_seen(q, k, v, lengths, key_lengths, scale, dout):
+    """Causal attention and its gradients in float64, every row from what it sees alone: a masked value is never multiplied, not
+    even by zero.  A NaN that is seen stays one."""
+    heads, group = q.shape[1], q.shape[1] // k.shape[1]
+    q, k, v, dout = (t.double() for t in (q, k, v, dout))
+    out, dq, dk, dv = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    a = b = 0
+    for n, m in zip(lengths, key_lengths):
+        for h in range(heads):
+            g = h // group
+            for i in range(n):
+                e = i + m - n + 1
+                if e <= 0:
+                    continue
+                kk, vv, qi, do = k[b:b + e, g], v[b:b + e, g], q[a + i, h], dout[a + i, h]
+                p = torch.softmax((kk * qi).sum(1) * scale, 0)
+                o = (p[:, None] * vv).sum(0)
+                ds = p * ((vv * do).sum(1) - (do * o).sum())
+                out[a + i, h] = o
+                dq[a + i, h] = scale * (ds[:, None] * kk).sum(0)
+                dk[b:b + e, g] += scale * ds[:, None] * qi
+                dv[b:b + e, g] += p[:, None] * do
+        a, b = a + n, b + m
+    return out, dq, dk, dv
+
+
+@pytest.mark.parametrize("dtype, size", [(F32, 64), (F32, 128), (BF16, 32), (BF16, 64), (BF16, 128), (F16, 64), (F16, 96)])
+@pytest.mark.parametrize("lengths, keys, heads, kv_heads", [([50], [50], 2, 1), ([130, 20], [130, 33], 2, 2), ([3], [400], 4, 1), ([40], [25], 2, 1)])
+@pytest.mark.parametrize("what", ["k", "v", "q", "dout", "all"])
+def test_what_is_no_number_reaches_exactly_those_that_see_it(dtype, size, lengths, keys, heads, kv_heads, what):
+    """In the middle of the sequence and in its last place, NaN and infinities: what sees them and what does not lie in one tile."""
+    from faith_amd import ops
+    q, k, v, dout = tensors(lengths, keys, heads, kv_heads, size, dtype, 51)
+    for name, t in (("k", k), ("v", v), ("q", q), ("dout", dout)):
+        if what in (name, "all"):
+            # a column of its own for each, so that no two infinities meet that the order of a sum could tell apart
+            for place, column, bad in ((t.shape[0] // 2, 1, math.nan), (t.shape[0] - 1, 3, math.nan), (t.shape[0] // 3, 2, math.inf)):
+                t[place, -1, column] = bad
+    packing = ops.Packing(lengths, keys)
+    scale = 1 / math.sqrt(size)
+    out, lse = ops.attention(q, k, v, packing, causal=True, return_lse=True)
+    got = (out, *ops.attention_backward(dout, q, k, v, out, lse, packing, causal=True))
+    want = attention_where_seen(q, k, v, lengths, keys, scale, dout)
+    clean = [torch.nan_to_num(t, 0, 0, 0) for t in (q, k, v, dout)]
+    r = R.attention(*clean[:3], lengths, keys, True, scale, clean[3])
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        finite = torch.isfinite(b)
+        assert bool((torch.isfinite(a) == finite).all()), f"{name}: finite at other places than expected"
+        # where nothing of it comes in, the error is that of a call without it
+        off = torch.where(finite, (a.double() - b).abs() - r[name + "_tol"] * 1.01, 0.0)
+        assert bool((off <= 0).all()), f"{name}: off by more than roundings account for"
+
+
+def test_a_long_prompt_of_what_is_no_number_is_no_slower():
+    """A NaN that everything sees, and nothing but NaN (a run that has diverged): the first result stands, and the time is the ordinary one."""
+    from faith_amd import ops
+    n = 8192
+    q, k, v, dout = tensors([n], [n], 8, 2, 64, BF16, 52)
+    packing = ops.Packing([n])
+
+    def run(*t):
+        out, lse = ops.attention(*t[:3], packing, causal=True, return_lse=True)
+        return (out, *ops.attention_backward(t[3], *t[:3], out, lse, packing, causal=True))
+
+    def milliseconds(*t):
+        run(*t)
+        times = []
+        for _ in range(3):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            got = run(*t)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times), got
+    usual, _ = milliseconds(q, k, v, dout)
+    k[0], v[0] = math.nan, math.nan
+    took, got = milliseconds(q, k, v, dout)
+    assert all(bool(torch.isnan(t[1:]).all()) for t in got) and took <= 2 * usual
+    nothing = [torch.full_like(t, math.nan) for t in (q, k, v, dout)]
+    took, got = milliseconds(*nothing)
+    assert all(bool(torch.isnan(t[1:]).all()) for t in got) and took <= 2 * usual
