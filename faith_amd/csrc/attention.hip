@@ -22,7 +22,7 @@ using namespace faith;
 using namespace faith::attn;
 
 constexpr int MFMA = 0x8, VALU = 0x2, DS_READ = 0x100;      // classes of __builtin_amdgcn_sched_group_barrier
-constexpr float LOWEST = -3.0e38f;           // stands for "no key yet": finite, so that differences stay numbers
+constexpr float LOWEST = -3.402823466e38f;   // the least finite number stands for "no key yet": differences stay numbers
 constexpr float LAZY = 8.f;                  // powers of two by which a row's largest score may pass its reference
 
 struct FwdArgs {
@@ -290,14 +290,14 @@ __global__ void __launch_bounds__(64 * WAVES, resident(FORWARD, KIND, sizeof(T),
             }
         return;
     }
-    const float inverse = sum > 0.f || sum != sum ? 1.f / sum : 0.f;   // no key: zeros
+    const float inverse = last < 0 ? 0.f : 1.f / sum;                  // no key: zeros.  (Scores of -infinity only: 0 / 0)
     T *dst = reinterpret_cast<T *>(g.out) + (long long)(it.q_start + token) * g.o_ts + (long long)head * g.o_hs;
     store_column<T, DP>(dst, o, inverse, half, g.size);
     if (g.lse && half == 0)
-        g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+        g.lse[(long long)head * g.lse_hs + it.q_start + token] = last < 0 ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
 }
 
-// Joins the parts of the rows of one item: {first token, tokens, -, -, first row, parts, -, first slot}; W wavefronts
+// Joins the parts of the rows of one item: {first token, tokens, -, keys, first row, parts, -, first slot}; W wavefronts
 // to a row, taking turns at its parts, their lanes along the head: four for few rows in many parts, one for 128 rows in a few.
 // The order of the sums depends on the number of parts only.
 template <class T, int DP, int ROWS, int W>
@@ -359,13 +359,14 @@ __global__ void __launch_bounds__(256) attention_join(const FwdArgs g, const Ite
             }
         }
         const int row = it.row0 + i, token = row / g.group, head = hk * g.group + (row - token * g.group);
-        const float inverse = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        const bool none = it.k_len == 0 || (g.causal && token + it.k_len < it.q_len);             // sees no key
+        const float inverse = none ? 0.f : 1.f / sum;
         T *dst = reinterpret_cast<T *>(g.out) + (long long)(it.q_start + token) * g.o_ts + (long long)head * g.o_hs;
 #pragma unroll
         for (int e = 0; e < N; ++e)
             if (64 * e + lane < g.size) dst[64 * e + lane] = (T)(o[e] * inverse);
         if (g.lse && lane == 0)
-            g.lse[(long long)head * g.lse_hs + it.q_start + token] = sum == 0.f ? -__builtin_inff() : (now + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+            g.lse[(long long)head * g.lse_hs + it.q_start + token] = none ? -__builtin_inff() : (now + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
     }
 }
 

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident(GRAD_QUERIES, KIND, sizeo
 #pragma unroll
         for (int e = 0; e < PER; ++e) delta = fmaf((float)o.v[u][e], (float)d_o.v[u][e], delta);
     delta = sum_halves(delta);
-    const float lse = l == -__builtin_inff() ? 0.f : l * 1.4426950408889634f;      // a row that sees no key: every p below is masked
+    const float lse = last < 0 ? 0.f : l * 1.4426950408889634f;                    // a row that sees no key: every p below is masked
     int up = probability_up<T>() ? UP_MOST : 0;      // p comes out times 2^up, and so does ds
     if (row < rows && half == 0 && (!SPLIT || wave == 0)) {
         float *s = g.stat + (long long)head * g.lse_hs + place;
@@ -153,7 +153,12 @@ __global__ void __launch_bounds__(64 * WAVES, resident(GRAD_QUERIES, KIND, sizeo
             add_row<T, DP>(dq, kr, p * (dot_rows(dorow, vb + (long long)j * g.v_ts, g.size) - delta), half, g.size);
         }
     }
-    if (last == 0) clear<DP>(dq);            // p = 1 and dp = delta, exactly
+    if (last == 0) {                         // p = 1 and dp = delta, exactly; what is no number stays none
+#pragma unroll
+        for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[m][r] = fmaf(dq[m][r], 0.f, 0.f);
+    }
     if (row >= rows) return;
     store_column<T, DP>(const_cast<T *>(at<T>(g.dq, place, g.dq_ts, head, g.dq_hs)), dq, g.scale, half, g.size);
 }
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident(GRAD_KEYS, KIND, sizeof(T
             for (int b = 0; b < BQ / 32; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (it.k_len == 1 || t0 + 32 * b + row_of(r, half) == -shift) dp[b][r] = 0.f;
+                    if (it.k_len == 1 || t0 + 32 * b + row_of(r, half) == -shift) dp[b][r] = fmaf(dp[b][r], 0.f, 0.f);
         }
         if constexpr (probability_up<T>() > 0) follow<DP>(dp, dk, up);
 #pragma unroll
@@ -363,7 +368,9 @@ __global__ void __launch_bounds__(64 * WAVES, resident(GRAD_KEYS, KIND, sizeof(T
                 const float *s = g.stat + (long long)h * g.lse_hs + place;
                 const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, krow, g.size), g.c, -s[0] - probability_up<T>()));
                 add_row<T, DP>(dv, dr, p, half, g.size);
-                add_row<T, DP>(dk, qr, p * (dot_rows(dr, vrow, g.size) + (probability_up<T>() ? s[stat_hs] : -s[stat_hs])), half, g.size);
+                float grad = p * (dot_rows(dr, vrow, g.size) + (probability_up<T>() ? s[stat_hs] : -s[stat_hs]));
+                if (i == -shift || it.k_len == 1) grad = fmaf(grad, 0.f, 0.f);
+                add_row<T, DP>(dk, qr, grad, half, g.size);
             }
     }
     if (key >= it.k_len) return;

@@ -674,7 +674,8 @@ int faith_attention_plan(const int *query_lengths, const int *key_lengths, int s
  *   lse       [heads, lse_head_stride] natural logarithm of each row's sum of exponentials, or NULL
  *   parts     scratch (see faith_attention_plan), NULL if the plan has no joins
  *   items ... kind: as the plan laid them down for FAITH_ATTENTION_FORWARD
- * A row that sees no key is zero, its lse -inf.  What masked keys and values hold does not matter, NaN included.
+ * A row that sees no key is zero, its lse -inf; one whose scores are all -inf is NaN, as 0 / 0.  What masked keys and values hold does not
+ * matter, NaN included.
  */
 int faith_attention(const void *q, const void *k, const void *v, void *out, float *lse, float *parts, const int *items,
                     int n_items, int n_joins, int kind, long long q_token_stride, long long q_head_stride,

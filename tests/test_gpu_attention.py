@@ -590,3 +590,40 @@ def test_a_long_prompt_of_what_is_no_number_is_no_slower():
     nothing = [torch.full_like(t, math.nan) for t in (q, k, v, dout)]
     took, got = milliseconds(*nothing)
     assert all(bool(torch.isnan(t[1:]).all()) for t in got) and took <= 2 * usual
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, m, causal", [(3, 1, False), (1, 1, True), (200, 1, False), (40, 40, True)])
+def test_a_score_that_is_no_number_has_no_gradient_that_is_one(dtype, n, m, causal):
+    """One key alone: dq = 0 because its probability is 1, which it is not where the score is NaN or infinite."""
+    from faith_amd import ops
+    for bad in (math.nan, math.inf, -math.inf):
+        q, k, v, dout = tensors([n], [m], 1, 1, 64, dtype, 41)
+        q[0, 0, 3] = bad
+        packing = ops.Packing([n], [m])
+        out, lse = ops.attention(q, k, v, packing, causal, return_lse=True)
+        dq, dk, _ = ops.attention_backward(dout, q, k, v, out, lse, packing, causal)
+        assert bool(torch.isnan(out[0]).all()) and bool(torch.isnan(dq[0]).all()) and bool(torch.isnan(dk[0]).any())
+        alone = dq[1:] if m == 1 else dq[:0]
+        assert bool((alone == 0).all()) and bool(torch.isfinite(out[1:]).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, m, heads, causal", [(5, 7, 2, False), (200, 300, 2, True), (1, 9000, 1, False), (128, 9000, 1, True), (700, 64, 4, False)])
+def test_scores_that_are_all_minus_infinity_give_no_number(dtype, n, m, heads, causal):
+    """softmax of nothing but -infinity is 0 / 0; only a row that sees no key at all is zero."""
+    from faith_amd import ops
+    q, k, v, dout = tensors([n], [m], heads, 1, 64, dtype, 42)
+    q[:, :, 0], k[:, :, 0] = 1, -math.inf
+    q[0, :, 0] = -1                                             # all +infinity: as little a number
+    packing = ops.Packing([n], [m])
+    out, lse = ops.attention(q, k, v, packing, causal, return_lse=True)
+    assert bool(torch.isnan(out).all()) and bool((lse[:, 1:] == -math.inf).all())
+    grads = ops.attention_backward(dout, q, k, v, out, lse, packing, causal)
+    assert bool(torch.isnan(grads[0]).all()) and bool(torch.isnan(grads[2]).all())
+    # beside rows that see none, and a sequence of ordinary ones
+    packing = ops.Packing([n, 9, 6], [m, 4, 6])
+    q, k, v, dout = (torch.cat([a, b]) for a, b in zip((q, k, v, dout), tensors([9, 6], [4, 6], heads, 1, 64, dtype, 43)))
+    out, lse = ops.attention(q, k, v, packing, True, return_lse=True)
+    assert bool(torch.isnan(out[:n]).all()) == (n <= m) and bool((out[n:n + 5] == 0).all()) and bool(torch.isfinite(out[n:]).all())
+    assert bool((lse[:, n:n + 5] == -math.inf).all())
