@@ -485,6 +485,10 @@ int norm_shapes(const char *fn, long long rows, int n, int kind, int dtype) {
     return FAITH_OK;
 }
 
+// Fewer than 2^32 threads: 256 to a row, or to four of one wavefront each, 512 to a row of eight.  (Four rows to a workgroup would allow more
+// than 2^24 rows; they are refused alike, so that the limit does not depend on the width.)
+bool one_launch(long long rows, int waves) { return rows < (1LL << 24) && rows * (waves == 8 ? 512 : 256) < (1LL << 32); }
+
 int grad_blocks(long long rows, int waves) {
     if (rows <= 0) return 0;
     const int per = waves == 1 ? 4 : 1;
@@ -501,13 +505,13 @@ extern "C" int faith_residual_norm(const void *x, const void *residual, const vo
     FAITH_REQUIRE(bits == 0 || bits == FAITH_BITS_INT8 || bits == FAITH_BITS_E4M3, FAITH_ERR_UNSUPPORTED, "%s: output %d", __func__, bits);
     FAITH_REQUIRE(eps >= 0.f && eps < 1e30f, FAITH_ERR_UNSUPPORTED, "%s: eps must be finite and not negative", __func__);
     if (rows == 0) return FAITH_OK;
-    FAITH_REQUIRE(rows < (1LL << 24), FAITH_ERR_UNSUPPORTED, "%s: %lld rows are more than one launch holds", __func__, rows);
     FAITH_NOT_NULL(x);
     FAITH_NOT_NULL(y);
     FAITH_REQUIRE(!bits || scales, FAITH_ERR_NULL, "%s: an output in 8 bits has a scale for each row", __func__);
     const NormArgs g = {x, residual, weight, bias, y, sum, stats, scales, rows, n, kind, bits, eps};
     const bool whole = aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) && aligned(bias, 16) && aligned(y, 16) && aligned(sum, 16);
     const Shape s = shape_of(n, dtype, whole);
+    FAITH_REQUIRE(one_launch(rows, s.waves), FAITH_ERR_UNSUPPORTED, "%s: %lld rows of %d are more than one launch holds", __func__, rows, n);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == FAITH_F32) return launch_norm<float>(g, s, st);
     if (dtype == FAITH_BF16) return launch_norm<__bf16>(g, s, st);

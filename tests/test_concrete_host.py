@@ -366,3 +366,17 @@ def test_the_search_takes_one_sentence():
     for shape in ((2, 4, 8), (4, 8), (0, 4, 8)):
         with pytest.raises(ValueError, match="one sentence"):
             concrete.falsify(net, torch.zeros(shape), [1, 2], [0.1, 0.1], 0)
+
+
+def test_rows_of_the_norm_that_pass_one_launch_are_refused():
+    """Before anything is launched: 2^32 threads, which rows of eight wavefronts reach at half as many."""
+    L = _lib.lib
+    buf = (ctypes.c_float * 256)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+
+    def call(rows, n, dtype):
+        return L.faith_residual_norm(p, None, None, None, p, None, None, p, rows, n, 0, dtype, 0, 1e-6, None)
+    for n, dtype in ((8192, _lib.BF16), (16384, _lib.F16), (8192, _lib.F32), (4096, _lib.F32)):
+        assert call(1 << 23, n, dtype) == -3 and b"launch" in L.faith_last_error()
+    for n, dtype in ((64, _lib.BF16), (4096, _lib.BF16), (2048, _lib.F32), (7, _lib.F32), (40000, _lib.F32)):
+        assert call(1 << 24, n, dtype) == -3 and b"launch" in L.faith_last_error()
