@@ -479,7 +479,8 @@ template <class T> int launch_grad(const NormGradArgs &g, const Shape &s, hipStr
 }
 
 int norm_shapes(const char *fn, long long rows, int n, int kind, int dtype) {
-    FAITH_REQUIRE(rows >= 0 && rows < (1LL << 31) && n > 0, FAITH_ERR_SHAPE, "%s: %lld rows of %d", fn, rows, n);
+    // the kernels count along a row in 32 bits, a step of the workgroup past its end
+    FAITH_REQUIRE(rows >= 0 && rows < (1LL << 31) && n > 0 && n <= (1 << 30), FAITH_ERR_SHAPE, "%s: %lld rows of %d", fn, rows, n);
     FAITH_REQUIRE(kind >= FAITH_NORM_RMS && kind <= FAITH_NORM_NO_VAR, FAITH_ERR_UNSUPPORTED, "%s: kind %d", fn, kind);
     FAITH_REQUIRE(dtype == FAITH_F32 || dtype == FAITH_BF16 || dtype == FAITH_F16, FAITH_ERR_UNSUPPORTED, "%s: element type %d", fn, dtype);
     return FAITH_OK;

@@ -1438,6 +1438,8 @@ def residual_norm(x, residual=None, weight=None, bias=None, kind="rms", eps=1e-6
     if kind not in _lib.NORM_KINDS or not _alike(x, (residual,), (weight, bias)):
         _norm_operands(x, (("residual", residual),), (("weight", weight), ("bias", bias)), kind)
     n = x.shape[-1]
+    if n > 1 << 30:
+        raise ValueError(f"x: rows of {n} elements, at most 2^30 are taken")
     rows, code = x.numel() // n, _lib.NORM_KINDS[kind]
     eps = float(eps)
     if not 0 <= eps < 1e30:
@@ -1468,6 +1470,8 @@ def residual_norm_backward(dy, h, weight, stats, kind="rms", dsum=None, with_wei
         _row_tensor("dy", dy)
         _norm_operands(h, (("dy", dy), ("dsum", dsum)), (("weight", weight),), kind)
     n = h.shape[-1]
+    if n > 1 << 30:
+        raise ValueError(f"h: rows of {n} elements, at most 2^30 are taken")
     rows, code = h.numel() // n, _lib.NORM_KINDS[kind]
     _row_tensor("stats", stats, h, h.shape[:-1], torch.float32)
     dev = h.device

@@ -698,7 +698,7 @@ int faith_attention_backward(const void *dout, const void *q, const void *k, con
                              int heads, int kv_heads, int size, int dtype, int causal, float scale, void *stream);
 
 /*
- * The residual connection and the normalisation behind it, along rows of n:
+ * The residual connection and the normalisation behind it, along rows of n (at most 2^30):
  *   h = x + residual;  c = h - mean(h)  (FAITH_NORM_RMS: c = h);  z = c / sqrt(mean(c^2) + eps)  (FAITH_NORM_NO_VAR: z = c);
  *   y = weight z + bias
  * residual, weight, bias may be NULL; sum (h, rounded to dtype; y is computed from the unrounded one), stats ([rows]: 1 / sqrt(...),

@@ -380,3 +380,12 @@ def test_rows_of_the_norm_that_pass_one_launch_are_refused():
         assert call(1 << 23, n, dtype) == -3 and b"launch" in L.faith_last_error()
     for n, dtype in ((64, _lib.BF16), (4096, _lib.BF16), (2048, _lib.F32), (7, _lib.F32), (40000, _lib.F32)):
         assert call(1 << 24, n, dtype) == -3 and b"launch" in L.faith_last_error()
+
+
+def test_rows_of_the_norm_longer_than_its_counters_are_refused():
+    L = _lib.lib
+    buf = (ctypes.c_float * 256)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    for n in ((1 << 30) + 1, (1 << 31) - 1, (1 << 31) - 256):
+        assert L.faith_residual_norm(p, None, None, None, p, None, None, p, 1, n, 0, 0, 0, 1e-6, None) == -2
+        assert L.faith_residual_norm_backward(p, None, p, None, p, p, None, None, None, 1, n, 0, 0, None) == -2

@@ -230,3 +230,14 @@ def test_eight_bits_of_rows_that_hold_no_numbers(n, kind, bits, dtype):
     w[7] = math.inf
     q, scales, _ = ops.residual_norm(x[:1], None, w, None, kind, quantize=bits)
     assert not bool(torch.isfinite(scales).any()) and bool(torch.isnan(q.float() * scales[:, None]).all())
+
+
+@pytest.mark.parametrize("n", [(1 << 31) + 8, (1 << 32) + 64])
+def test_rows_longer_than_32_bits_count_are_refused(n):
+    """Not taken for the shorter row that their length is in 32 bits."""
+    from faith_amd import ops
+    x = torch.empty(1, n, device="cuda", dtype=BF16)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.residual_norm(x)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.residual_norm_backward(x, x, None, torch.ones(1, device="cuda"), with_weight=False)
