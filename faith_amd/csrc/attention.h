@@ -484,10 +484,11 @@ inline bool attention_rows(const char *fn, const char *name, const void *p, long
     else set_error("%s: %s must start on 16 bytes and have strides of whole 16-byte groups, the tokens' at least %d and under 2^24 bytes", fn, name, size);
     return false;
 }
-// heads that are read may lie on each other; written, they would race
-inline bool attention_heads_apart(const char *fn, const char *name, long long head_stride, int heads, int size) {
-    if (heads == 1 || head_stride >= size) return true;
-    set_error("%s: the heads of %s, which is written, must not overlap", fn, name);
+// Rows and heads that are read may lie on each other; written, they would race.  Token by token, or head by head: how many tokens, and with
+// that how far apart heads have to be, the items say on the device; two at least are taken for granted.
+inline bool attention_heads_apart(const char *fn, const char *name, long long token_stride, long long head_stride, int heads, int size) {
+    if (heads == 1 || (head_stride >= size && (token_stride >= (heads - 1) * head_stride + size || head_stride >= token_stride + size))) return true;
+    set_error("%s: the rows and heads of %s, which is written, must not overlap", fn, name);
     return false;
 }
 

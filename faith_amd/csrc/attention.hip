@@ -552,7 +552,7 @@ extern "C" int faith_attention(const void *q, const void *k, const void *v, void
     const int es = dtype == FAITH_F32 ? 4 : 2;
     if (!attention_rows(__func__, "q", q, q_token_stride, q_head_stride, size, es) || !attention_rows(__func__, "k", k, k_token_stride, k_head_stride, size, es) ||
         !attention_rows(__func__, "v", v, v_token_stride, v_head_stride, size, es) || !attention_rows(__func__, "out", out, out_token_stride, out_head_stride, size, es) ||
-        !attention_heads_apart(__func__, "out", out_head_stride, heads, size))
+        !attention_heads_apart(__func__, "out", out_token_stride, out_head_stride, heads, size))
         return FAITH_ERR_ALIGN;
     if (!attention_grid(__func__, n_items, kv_heads)) return FAITH_ERR_UNSUPPORTED;
     FwdArgs g;

@@ -460,7 +460,7 @@ extern "C" int faith_attention_backward(const void *dout, const void *q, const v
     for (int i = 0; i < 8; ++i) {
         if ((rows[i].keys ? n_key_items : n_query_items) == 0) continue;
         if (!attention_rows(__func__, rows[i].name, rows[i].p, strides[2 * i], strides[2 * i + 1], size, es)) return rows[i].p ? FAITH_ERR_ALIGN : FAITH_ERR_NULL;
-        if (i >= 5 && !attention_heads_apart(__func__, rows[i].name, strides[2 * i + 1], rows[i].keys ? kv_heads : heads, size)) return FAITH_ERR_ALIGN;
+        if (i >= 5 && !attention_heads_apart(__func__, rows[i].name, strides[2 * i], strides[2 * i + 1], rows[i].keys ? kv_heads : heads, size)) return FAITH_ERR_ALIGN;
     }
     FAITH_REQUIRE(n_query_items == 0 || (lse && stat && query_items), FAITH_ERR_NULL, "%s: lse, stat or the query items are NULL", __func__);
     FAITH_REQUIRE(n_key_items == 0 || key_items, FAITH_ERR_NULL, "%s: the key items are NULL", __func__);

@@ -1220,14 +1220,19 @@ def _rows(name, t, rows, heads, size, like=None):
         raise ValueError(f"{name}: expected shape ({rows} or more, {heads or 'heads'}, {size or 'size'}), got {tuple(t.shape)}")
     per = 16 // t.element_size()
     ts, hs, es = t.stride()
-    if t.shape[0] == 1:
-        ts = t.shape[1] * t.shape[2]
     if t.shape[1] == 1:
         hs = t.shape[2]
+    if t.shape[0] == 1:
+        ts = _stride_of_one(hs, t.shape[1], t.shape[2])
     if (es != 1 and t.shape[2] > 1) or ts % per or hs % per or t.data_ptr() % 16 or ts < t.shape[2] or hs < 0 or ts * t.element_size() >= 1 << 24:
         raise ValueError(f"{name}: the elements of a head must be contiguous, rows must not overlap, and rows and heads must start on "
                          f"16 bytes (strides {t.stride()})")
     return ts, hs
+
+
+def _stride_of_one(hs, heads, size):
+    """A token stride for a single token, where any would do: one with which a second token would not lie on the first."""
+    return size if hs >= 2 * size else max(heads * size, (heads - 1) * hs + size)
 
 
 def _attention_operands(q, k, v, packing):
@@ -1307,6 +1312,8 @@ def attention(q, k, v, packing, causal=False, scale=None, return_lse=False, out=
             # token by token, or head by head; anything in between would be written twice
             if heads > 1 and (oh < size or (ot < (heads - 1) * oh + size and oh < (packing.tokens - 1) * ot + size and packing.tokens > 1)):
                 raise ValueError(f"out: its rows and heads must not overlap (strides {out.stride()})")
+            if packing.tokens <= 1:
+                ot = _stride_of_one(oh, heads, size)
         known = (plan, floats, heads, (items, n, joins, kind, qt, qh, kt, kh, vt, vh, ot, oh, packing.tokens, heads, kv_heads, size,
                                        _DTYPES[q.dtype], int(causal)), 1.0 / math.sqrt(size))
         if key is not None:

@@ -670,7 +670,9 @@ int faith_attention_plan(const int *query_lengths, const int *key_lengths, int s
  * out = softmax(scale * q k^T) v over packed sequences; head h uses key head h / (heads / kv_heads).
  *   q, out    [tokens, heads, size] by their strides (elements); k, v [keys, kv_heads, size] likewise.  16-byte aligned,
  *             strides in whole 16-byte groups; size <= 128 in whole 16-byte groups.  Rows behind the last sequence are
- *             neither read nor written.  No two places of out may share memory, with each other or with q, k, v.
+ *             neither read nor written.  No two places of out may share memory, with each other or with q, k, v: its token
+ *             stride reaches past all heads, or its head stride past all tokens (with a single token, whose stride does
+ *             not matter: past two).
  *   lse       [heads, lse_head_stride] natural logarithm of each row's sum of exponentials, or NULL
  *   parts     scratch (see faith_attention_plan), NULL if the plan has no joins
  *   items ... kind: as the plan laid them down for FAITH_ATTENTION_FORWARD

@@ -389,3 +389,32 @@ def test_rows_of_the_norm_longer_than_its_counters_are_refused():
     for n in ((1 << 30) + 1, (1 << 31) - 1, (1 << 31) - 256):
         assert L.faith_residual_norm(p, None, None, None, p, None, None, p, 1, n, 0, 0, 0, 1e-6, None) == -2
         assert L.faith_residual_norm_backward(p, None, p, None, p, p, None, None, None, 1, n, 0, 0, None) == -2
+
+
+def test_results_whose_rows_share_memory_with_other_heads_are_refused():
+    """Token by token or head by head; what lies in between is written by two workgroups."""
+    L = _lib.lib
+    buf = (ctypes.c_float * 256)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+
+    def forward_call(ts, hs, heads=4):          # refused (-3) for its number of items where the strides pass
+        return L.faith_attention(p, p, p, p, None, None, p, 1 << 27, 0, 0, 64, 16, 64, 16, 64, 16, ts, hs, 4, heads, heads, 16, 0, 0, 0.5, None)
+    for ts, hs in ((16, 16), (32, 16), (60, 16), (24, 32), (64, 20)):
+        assert forward_call(ts, hs) == -4 and b"overlap" in L.faith_last_error()
+    for ts, hs in ((64, 16), (76, 20), (16, 32), (16, 1000), (24, 40)):
+        assert forward_call(ts, hs) == -3
+    assert forward_call(16, 16, heads=1) == -3
+
+    def backward_call(which, ts, hs):
+        strides = (ctypes.c_longlong * 16)(*[64, 16] * 8)
+        strides[2 * which], strides[2 * which + 1] = ts, hs
+        return L.faith_attention_backward(p, p, p, p, p, p, p, p, p, p, None, p, 1 << 27, 0, p, 1 << 27, 0, 0, 0, ctypes.addressof(strides), 4, 4, 4, 16, 0, 0, 0.5, None)
+    assert [backward_call(i, 16, 16) for i in range(8)] == [-3] * 5 + [-4] * 3
+    assert [backward_call(i, 16, 640) for i in range(8)] == [-3] * 8
+
+
+@pytest.mark.parametrize("hs", [0, 32, 40, 63, 64, 4096, 1 << 24])
+def test_the_stride_of_a_single_token_passes_for_two(hs):
+    ts = ops._stride_of_one(hs, 4, 32)
+    assert hs < 32 or ts >= 3 * hs + 32 or hs >= ts + 32
+    assert ts < 1 << 22

@@ -627,3 +627,14 @@ def test_scores_that_are_all_minus_infinity_give_no_number(dtype, n, m, heads, c
     out, lse = ops.attention(q, k, v, packing, True, return_lse=True)
     assert bool(torch.isnan(out[:n]).all()) == (n <= m) and bool((out[n:n + 5] == 0).all()) and bool(torch.isfinite(out[n:]).all())
     assert bool((lse[:, n:n + 5] == -math.inf).all())
+
+
+def test_one_token_into_a_result_of_any_strides():
+    from faith_amd import ops
+    q, k, v, _ = tensors([1], [9], 4, 2, 32, BF16, 61)
+    packing = ops.Packing([1], [9])
+    want = ops.attention(q, k, v, packing)
+    store = torch.zeros(1 << 20, device="cuda", dtype=BF16)
+    for rows, strides in ((1, (8, 32, 1)), (1, (160, 40, 1)), (16, (40, 32, 1)), (16, (32, 1 << 14, 1)), (1, (1 << 10, 1 << 18, 1))):
+        out = store.as_strided((rows, 4, 32), strides)
+        assert torch.equal(ops.attention(q, k, v, packing, out=out)[:1], want)
