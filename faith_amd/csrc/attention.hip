@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident(FORWARD, KIND, sizeof(T),
     typedef Stager<T, DP, BN, KEYS ? 1 : 4> St;                     // keys: read by rows
     typedef Stager<T, DP, BN, KEYS ? 1 : 4, COLUMNS> Sv;            // values: by columns only
     // two stages in arrays of their own, so that the compiler sees that loads into one do not touch the other
-    __shared__ T k0[ALL], v0[ALL], k1[ONCE ? 1 : ALL], v1[ONCE ? 1 : ALL];
+    __shared__ __align__(16) T k0[ALL], v0[ALL], k1[ONCE ? 1 : ALL], v1[ONCE ? 1 : ALL];
 
     int hk, n;
     if (!dealt(g.deal, &hk, &n)) return;
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident(FORWARD, KIND, sizeof(T),
         __syncthreads();
         constexpr int WIDTH = DP / 32 * 16, HALF = ALL * (int)sizeof(T) / 4;
         static_assert((WAVES - 1) * 64 * WIDTH <= 2 * HALF, "the results fit a stage");
-        __shared__ float ml[(WAVES - 1) * 128];
+        __shared__ __align__(16) float ml[(WAVES - 1) * 128];
         float *lo = reinterpret_cast<float *>(k0), *hi = reinterpret_cast<float *>(v0);
         auto cell = [&](int w, int e) -> float & {                 // result w, register e of this lane
             const int x = (w * WIDTH + e) * 64 + lane;
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident(FORWARD, KIND, sizeof(T),
 template <class T, int DP, int ROWS, int W>
 __global__ void __launch_bounds__(256) attention_join(const FwdArgs g, const Item *joins) {
     constexpr int N = (DP + 63) / 64;
-    __shared__ float ml[4][2], os[3][64 * N];
+    __shared__ __align__(16) float ml[4][2], os[3][64 * N];
     const Item it = joins[blockIdx.x];
     const int hk = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int rows = it.q_len * g.group, parts = it.begin;

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident(GRAD_QUERIES, KIND, sizeo
     constexpr bool SPLIT = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
     constexpr int TILE = BN * DP, ALL = TILE * (SPLIT ? WAVES : 1);
     typedef Stager<T, DP, BN, SPLIT ? 1 : WAVES> St;
-    __shared__ T k0[ALL], v0[ALL], k1[ONCE ? 1 : ALL], v1[ONCE ? 1 : ALL];
+    __shared__ __align__(16) T k0[ALL], v0[ALL], k1[ONCE ? 1 : ALL], v1[ONCE ? 1 : ALL];
 
     int hk, n;
     if (!dealt(g.deal, &hk, &n)) return;
@@ -168,8 +168,8 @@ __global__ void __launch_bounds__(64 * WAVES, resident(GRAD_KEYS, KIND, sizeof(T
     constexpr bool SPLIT = KIND != KIND_ROWS, ONCE = KIND == KIND_ONCE;
     constexpr int TILE = BQ * DP, EACH = SPLIT ? WAVES : 1, ALL = TILE * EACH;
     typedef Stager<T, DP, BQ, SPLIT ? 1 : WAVES> St;
-    __shared__ T q0[ALL], d0[ALL], q1[ONCE ? 1 : ALL], d1[ONCE ? 1 : ALL];
-    __shared__ float l0[64 * EACH], e0[64 * EACH], l1[ONCE ? 1 : 64 * EACH], e1[ONCE ? 1 : 64 * EACH];           // lse, delta of the staged queries
+    __shared__ __align__(16) T q0[ALL], d0[ALL], q1[ONCE ? 1 : ALL], d1[ONCE ? 1 : ALL];
+    __shared__ __align__(16) float l0[64 * EACH], e0[64 * EACH], l1[ONCE ? 1 : 64 * EACH], e1[ONCE ? 1 : 64 * EACH];           // lse, delta of the staged queries
 
     int hk, n;
     if (!dealt(g.deal, &hk, &n)) return;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident(GRAD_KEYS, KIND, sizeof(T
     const ColumnRegs<T, DP> k = column_regs<T, DP>(krow, half, g.size);
     // The values' rows stay in LDS where registers for them would halve the wavefronts on a SIMD
     constexpr bool V_IN_LDS = !SPLIT && sizeof(T) == 2 && DP == 128;
-    __shared__ T v_rows[V_IN_LDS ? 128 * DP : 1];
+    __shared__ __align__(16) T v_rows[V_IN_LDS ? 128 * DP : 1];
     ColumnRegs<T, DP> v;
     if constexpr (V_IN_LDS) {
         Stager<T, DP, 128, 4> vs;

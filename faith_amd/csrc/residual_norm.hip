@@ -96,7 +96,7 @@ constexpr int threads_of(int waves) { return 64 * waves * rows_of(waves); }
 template <class T, int WAVES, int CH>
 __global__ void __launch_bounds__(threads_of(WAVES)) residual_norm(const NormArgs g) {
     constexpr int N = Group<T>::N, LANES = 64 * WAVES;
-    __shared__ float slot[3][WAVES];
+    __shared__ __align__(16) float slot[3][WAVES];
     const int wave = threadIdx.x >> 6, t = (int)threadIdx.x % LANES;
     const long long row = (long long)blockIdx.x * rows_of(WAVES) + wave / WAVES;
     if (WAVES < 4 && row >= g.rows) return;                   // a whole wavefront; no barrier follows in this shape
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(threads_of(WAVES)) residual_norm(const NormArg
 
 // any width and alignment: a workgroup to a row, which it goes over again for each of its sums
 template <class T> __global__ void __launch_bounds__(256) residual_norm_any(const NormArgs g) {
-    __shared__ float slot[3][4];
+    __shared__ __align__(16) float slot[3][4];
     const int wave = threadIdx.x >> 6;
     const long long at = (long long)blockIdx.x * g.n;
     const T *x = reinterpret_cast<const T *>(g.x) + at, *res = g.residual ? reinterpret_cast<const T *>(g.residual) + at : nullptr;
@@ -258,7 +258,7 @@ template <class T, int WAVES, int CH, bool BIAS>
 __global__ void __launch_bounds__(threads_of(WAVES)) residual_norm_grad(const NormGradArgs g) {
     constexpr int N = Group<T>::N, LANES = 64 * WAVES;
     typedef typename Packed<T>::type Raw;
-    __shared__ float slot[2][2][WAVES], mean_slot[2][WAVES];
+    __shared__ __align__(16) float slot[2][2][WAVES], mean_slot[2][WAVES];
     const int wave = threadIdx.x >> 6, t = (int)threadIdx.x % LANES;
     const float inv_n = 1.f / (float)g.n;
     float dw[CH][N], db[BIAS ? CH : 1][N];
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(threads_of(WAVES)) residual_norm_grad(const No
 
 // any width and alignment: dx, a workgroup to a row
 template <class T> __global__ void __launch_bounds__(256) residual_norm_grad_any(const NormGradArgs g) {
-    __shared__ float slot[3][4];
+    __shared__ __align__(16) float slot[3][4];
     const int wave = threadIdx.x >> 6;
     const long long row = blockIdx.x, at = row * g.n;
     const T *dy = reinterpret_cast<const T *>(g.dy) + at, *hh = reinterpret_cast<const T *>(g.h) + at, *w = reinterpret_cast<const T *>(g.weight);
@@ -412,7 +412,7 @@ template <class T> __global__ void __launch_bounds__(256) residual_norm_columns_
 
 // columns of `partial` added up: 32 columns to a workgroup, 32 threads down each
 template <class T> __global__ void __launch_bounds__(1024) residual_norm_columns(const NormGradArgs g) {
-    __shared__ float part[32][33];
+    __shared__ __align__(16) float part[32][33];
     const int c = threadIdx.x & 31, s = threadIdx.x >> 5, e = (int)blockIdx.x * 32 + c;
     const bool bias = blockIdx.y == (g.dweight ? 1 : 0);
     float v = 0.f;

@@ -418,3 +418,19 @@ def test_the_stride_of_a_single_token_passes_for_two(hs):
     ts = ops._stride_of_one(hs, 4, 32)
     assert hs < 32 or ts >= 3 * hs + 32 or hs >= ts + 32
     assert ts < 1 << 22
+
+
+def test_arrays_in_lds_are_aligned_for_their_widest_read():
+    """16 bytes a lane: not left to where the compiler puts an array of 2-byte elements."""
+    import glob
+    import os
+    import re
+    import faith_amd
+    folder = os.path.join(os.path.dirname(faith_amd.__file__), "csrc")
+    seen = 0
+    for path in [p for name in ("attention", "residual_norm") for p in glob.glob(os.path.join(folder, name + "*"))]:
+        for line in open(path):
+            if re.search(r"\b__shared__\b", line) and "[" in line:
+                seen += 1
+                assert "__align__(16)" in line, f"{os.path.basename(path)}: {line.strip()}"
+    assert seen >= 8
