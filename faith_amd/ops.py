@@ -173,7 +173,7 @@ class _Tuned:
 def _on(device, op=None, shape=None):
     """Device guard for the launch; free when the tensor already lives on the current device.
     With a tuning table in use (autotune.use) the entry for (op, shape) is applied around the launch."""
-    if device.index is None or device.index == torch._C._cuda_getDevice():
+    if device.index is None or device.index == torch.cuda.current_device():
         guard = _NO_GUARD
     else:
         guard = torch.cuda.device(device)

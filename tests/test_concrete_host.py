@@ -434,3 +434,11 @@ def test_arrays_in_lds_are_aligned_for_their_widest_read():
                 seen += 1
                 assert "__align__(16)" in line, f"{os.path.basename(path)}: {line.strip()}"
     assert seen >= 8
+
+
+def test_the_device_guard_asks_for_the_current_device(monkeypatch):
+    """By the public name: every operator of the library goes through it."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    assert ops._on(torch.device("cuda", 1)) is ops._NO_GUARD and ops._on(torch.device("cuda")) is ops._NO_GUARD
+    other = ops._on(torch.device("cuda", 0))
+    assert isinstance(other, torch.cuda.device) and other.idx == 0
