@@ -119,7 +119,7 @@ def encoder_layer(x, layer, packing, layer_norm="no_var", hidden_act="relu", cau
     ask -- the last layer in front of a pooler."""
     att = layer.attention.self
     heads, size = att.num_attention_heads, att.attention_head_size
-    kv_heads = getattr(att, "num_key_value_heads", heads)
+    kv_heads = getattr(att, "num_key_value_heads", None) or heads
     asking = x if queries is None else x[queries[0]]
     q = _dense(asking, att.query).view(-1, heads, size)
     k, v = _dense(x, att.key).view(-1, kv_heads, size), _dense(x, att.value).view(-1, kv_heads, size)

@@ -334,7 +334,7 @@ def _bounded(network):
         raise ValueError('bounds are not propagated through layer_norm = "rms"')
     for layer in network.layers:
         att = layer.attention.self
-        if getattr(att, "num_key_value_heads", att.num_attention_heads) != att.num_attention_heads:
+        if (getattr(att, "num_key_value_heads", None) or att.num_attention_heads) != att.num_attention_heads:
             raise ValueError("bounds are not propagated through heads that share keys")
 
 

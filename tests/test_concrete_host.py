@@ -442,3 +442,14 @@ def test_the_device_guard_asks_for_the_current_device(monkeypatch):
     assert ops._on(torch.device("cuda", 1)) is ops._NO_GUARD and ops._on(torch.device("cuda")) is ops._NO_GUARD
     other = ops._on(torch.device("cuda", 0))
     assert isinstance(other, torch.cuda.device) and other.idx == 0
+
+
+def test_networks_that_say_none_for_shared_key_heads_have_their_own():
+    """None is what a configuration without them holds: such a network was propagated before there was an attribute to look at."""
+    from types import SimpleNamespace
+    from faith_amd.workloads import random_layer
+    net = SimpleNamespace(embedding_norm=None, layers=[random_layer(torch.Generator().manual_seed(3), 16, 4, 32)], layer_norm="no_var", hidden_act="relu")
+    net.layers[0].attention.self.num_key_value_heads = None
+    forward._bounded(net)
+    net.layers[0].attention.self.num_key_value_heads = 4
+    forward._bounded(net)

@@ -260,3 +260,13 @@ def test_eight_bit_activations_do_not_hide_what_is_no_number():
     for bits in (None, "int8", "e4m3"):
         got = concrete.logits(net, torch.cat(xs), [30, 64], activations=bits)
         assert bool(torch.isnan(got[0]).all()) and bool(torch.isfinite(got[1]).all())
+
+
+def test_none_for_shared_key_heads_is_no_sharing():
+    from faith_amd import concrete
+    net = network(3, "no_var")
+    x = sentences([9], 4)[0][None]
+    want = concrete.logits(net, x)
+    for layer in net.layers:
+        layer.attention.self.num_key_value_heads = None
+    assert torch.equal(concrete.logits(net, x), want)
