@@ -172,6 +172,8 @@ def logits(network, embeddings, lengths=None, activations=None):
     """The network's output [sentences, classes] for embeddings [sentences, L, hidden], or packed [words, hidden] with the
     sentences' lengths (a list, or a Batch that the caller keeps).  Differentiable.  activations "int8" / "e4m3": what leaves a normalisation is held in 8 bits
     with a scale for each row, as a network deployed that way would hold it (no gradient)."""
+    if activations is not None and activations not in ops._BITS:
+        raise ValueError(f"activations={activations!r}: one of {', '.join(ops._BITS)} or None")
     rows, batch = _rows_of(embeddings, lengths)
     if activations is not None:
         with torch.no_grad():

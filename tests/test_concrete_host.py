@@ -453,3 +453,12 @@ def test_networks_that_say_none_for_shared_key_heads_have_their_own():
     forward._bounded(net)
     net.layers[0].attention.self.num_key_value_heads = 4
     forward._bounded(net)
+
+
+@pytest.mark.parametrize("mode", ["no", "standard"])
+def test_activations_of_another_name_are_refused_whatever_the_network_normalises(mode):
+    from types import SimpleNamespace
+    net = SimpleNamespace(layer_norm=mode)
+    for ask in (concrete.logits, concrete.predict):
+        with pytest.raises(ValueError, match="activations"):
+            ask(net, torch.zeros(1, 3, 8), activations="int4")
