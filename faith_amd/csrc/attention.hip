@@ -3,13 +3,13 @@
 //
 // One pass over the keys with the running maximum and sum of the softmax.  A row is one (token, head of the group) pair,
 // row = token * group + head: all rows of a tile share the keys and values that it stages, so a group reads them once.
-// Two shapes of workgroup, four wavefronts each, 32 rows to a wavefront:
+// Two shapes of workgroup, four wavefronts each (keys: two in fp32 with heads of more than 64), 32 rows to a wavefront:
 //   rows    128 rows; every wavefront goes over every key tile (64 keys, 32 in fp32), staged once for the four
 //   keys    at most 32 rows (a single token's group, a short sentence); the wavefronts take turns at the key tiles of 32
 //           keys, each staged by its wavefront alone with no barrier, and join their results through LDS at the end
 // Few rows against many keys leave most of the device idle: the keys are then cut into several items, whose partial
 // results (maximum, sum, unnormalised output, all in fp32) a second small launch joins in a fixed order.
-// Measured, 32 / 8 heads of 128 in bf16: 16384 causal tokens 1.94 ms, 1133 TFLOP/s, bound by power (1.47 ms at an earlier step with
+// Measured, 32 / 8 heads of 128 in bf16: 16384 causal tokens 1.94 ms, 1132 TFLOP/s, bound by power (1.47 ms at an earlier step with
 // zeros for data, 2.07 without); one query each against 64 caches of 100 to 8192, 1.08 GB, 192 us, 5.6 TB/s, bound by HBM.
 #include "attention.h"
 
@@ -402,8 +402,8 @@ struct Plan {
 // Items of one pass, longest first.
 // Wavefronts share their rows and divide the rest (KEYS) for 32 rows or fewer, and
 //   backward  where workgroups of 128 rows would leave half of the compute units without one: 1000 tokens, 4 heads of 64, bf16
-//             27 us instead of 52; 2048 tokens, 8 / 2 heads of 128 152 instead of 467 (95 since the group is cut, below); 20 sequences of 256 with 4 heads (160
-//             workgroups) would take 33 instead of 21
+//             27 us instead of 52; 2048 tokens, 8 / 2 heads of 128 152 instead of 467 (95 since the group is cut, below);
+//             20 sequences of 256 with 4 heads (160 workgroups) would take 33 instead of 21
 //   forward   there too, in fp32, if none has a second turn: 30 sequences of 128, 4 heads of 64 11.2 us instead of 13.4.  With
 //             more keys, or 2-byte elements, 128 rows and cut keys are faster (1000 tokens as above: 14 against 28).
 // The gradients of keys are cut by the heads of the group where there are fewer workgroups of 128 keys than the device holds:

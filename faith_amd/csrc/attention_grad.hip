@@ -1,14 +1,15 @@
 // Gradients of the attention of a network's concrete pass (attention.hip), scores and probabilities computed again:
 //     p = exp(s - lse),  dp = do . v,  ds = p (dp - delta),  delta = do . out
 //     dq = scale sum_j ds k,   dk = scale sum_{i, heads of the group} ds q,   dv = sum_{i, heads of the group} p do
-// p and ds are held in 32 bits and rounded once, to the elements' type, as operands of the last three products (in fp16 times a power
-// of two that keeps them in its range, see follow() in attention.h); delta comes from the output as it was stored.  Against one rounding of each result these are two or three independent ones of the same size:
-// 1.4 times the error of a computation in 32 bits at a few hundred keys, up to twice at a handful.
-// Two launches (a third joins parts where the plan cuts) and no atomics, so that the same call gives the same bits: one goes over the keys for a tile of query rows (and
-// leaves delta and the logarithm of the row's sum, in powers of two, to the other), one over the queries of all heads of the
-// group for a tile of keys.  That computes s and dp twice -- seven products where five would do -- and needs neither an array
-// of sums in 32 bits that many workgroups add to nor a pass that rounds it.
-// Measured, 5 causal sequences of 300 to 4096, 32 / 8 heads of 128 in bf16: queries 0.61 ms, matrix units 51 % busy; keys 1.00 ms, 42 %.
+// p and ds are held in 32 bits and rounded once, to the elements' type, as operands of the last three products (in fp16 times a
+// power of two that keeps them in its range, see follow() in attention.h); delta comes from the output as it was stored.  Against
+// one rounding of each result these are two or three independent ones of the same size: 1.4 times the error of a computation in 32
+// bits at a few hundred keys, up to twice at a handful.
+// Two launches (a third joins parts where the plan cuts) and no atomics, so that the same call gives the same bits: one goes over
+// the keys for a tile of query rows (and leaves delta and the logarithm of the row's sum, in powers of two, to the other), one over
+// the queries of all heads of the group for a tile of keys.  That computes s and dp twice -- seven products where five would do -- and
+// needs neither an array of sums in 32 bits that many workgroups add to nor a pass that rounds it.
+// Measured, 5 causal sequences of 300 to 4096, 32 / 8 heads of 128 in bf16: queries 0.60 ms, matrix units 55 % busy; keys 1.00 ms, 41 %.
 #include "attention.h"
 
 namespace {

@@ -2,11 +2,12 @@
 // row of n
 //     c = h - mean(h)  (root mean square: c = h),   z = c / sqrt(mean(c^2) + eps)  (without the variance: z = c),   y = w z + b
 // and the gradients.  Everything is bound by HBM: forward 4 n elements a row (x, residual in; h, y out), backward 4 n (dy, h,
-// dsum in; dx out).  Measured: 16384 rows of 4096 bf16 forward 94 us, 5.7 TB/s.  A row is read once and stays in registers between the statistics and the result: a wavefront to a row
-// up to 128 groups of 16 bytes, four or eight wavefronts beyond that; rows that do not fall into 16-byte
-// groups, and rows wider than the registers hold, take a kernel that goes over the row again (it comes from the L2).
-// Statistics are sums in 32 bits over at most a few dozen values a lane and a tree above; the variance is that of the
-// centred values, so nothing cancels.
+// dsum in; dx out).  Measured: 16384 rows of 4096 bf16 forward 94 us, 5.7 TB/s.  A row is read once and stays in registers
+// between the statistics and the result: a wavefront to a row up to 128 groups of 16 bytes, four or eight wavefronts beyond that;
+// rows that do not fall into 16-byte groups, and rows wider than the registers hold, take a kernel that goes over the row again (it
+// comes from the L2).
+// Statistics are sums in 32 bits: over at most 32 values a lane where the row stays in registers, n / 256 values a lane in the
+// kernel for any width, and a tree above; the variance is that of the centred values, so nothing cancels.
 #include "common.h"
 
 namespace {
@@ -247,13 +248,12 @@ struct NormGradArgs {
 
 // dh = r (g - z mean(g z) [with the variance] - mean(g) [with the mean]) + dsum, g = w dy.  z comes from h as it was stored,
 // and so does the mean: against that of the unrounded sum a row of almost equal values would come out off by its rounding
-// over its spread.  A workgroup goes over rows
-// blockIdx.x, + gridDim.x, ...; its columns' sums of dy z and dy stay in registers until the end and go to a row of
-// `partial` of its own, which a second launch adds up in a fixed order: no atomics, the same bits every time.
+// over its spread.  A workgroup goes over rows blockIdx.x, + gridDim.x, ...; its columns' sums of dy z and dy stay in registers
+// until the end and go to a row of `partial` of its own, which a second launch adds up in a fixed order: no atomics, the same bits
+// every time.
 //
 // The next row is on its way while this one is worked on: without that a row's loads wait for the sums of the row before
-// (8191 rows of 5120 bf16: 114 -> 84 us, now 81, 4.1 TB/s; sixteen wavefronts to a row instead
-// of four take 95).
+// (8191 rows of 5120 bf16: 114 -> 84 us, now 80, 4.2 TB/s; sixteen wavefronts to a row instead of four take 95).
 template <class T, int WAVES, int CH, bool BIAS>
 __global__ void __launch_bounds__(threads_of(WAVES)) residual_norm_grad(const NormGradArgs g) {
     constexpr int N = Group<T>::N, LANES = 64 * WAVES;
