@@ -312,7 +312,7 @@ __device__ __forceinline__ float sum_halves(float v) {
 // Other values (fp16): a power of two for each column, 2^up, with which s comes here, and under which the largest of the column so far
 // lies at most at 2^15.  It starts higher than any value asks for (ds is at most 2^40: products of two fp16 values over 128 places) and
 // only falls, to where that value lies in [2^7, 2^8); the sums follow it.  13 sequences of 37 ... 1021, 12 heads of 80, forward and
-// gradients: 192 us with it, 187 without; 2048 keys and gradients of 2^-13: dq off by 0.38 %, all of it its own rounding, instead of 2.2.
+// gradients: 185 us with it, 183 without; 2048 keys and gradients of 2^-13: dq off by 0.38 %, all of it its own rounding, instead of 2.2.
 constexpr int UP_MOST = 80;
 template <int DP, int N> __device__ __forceinline__ void follow(floatx16 (&s)[N], floatx16 (&acc)[DP / 32], int &up) {
     float top = 0.f;
